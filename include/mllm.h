@@ -439,6 +439,169 @@ MLLM_API void mllm_page_table_map(mllm_page_table *pt, int logical_page, int phy
 MLLM_API int mllm_page_table_lookup(const mllm_page_table *pt, int logical_page);
 MLLM_API const int *mllm_page_table_entries(const mllm_page_table *pt);
 
+/* ------------------------------- paged 16- or 8-bit KV cache (serving) */
+/* No reference counterpart: the reference keeps its caches in fp32 and runs one
+ * token at a time.  These operators serve callers whose caches are half or a
+ * quarter of that size, whose prompts run as a whole, and whose sequences
+ * share, copy and give back pages.  Everything is device memory but the
+ * structs themselves and mllm_rotary_freqs; every call is capturable. */
+#define MLLM_F32 0
+#define MLLM_F16 1
+#define MLLM_BF16 2
+#define MLLM_E4M3 3                /* caches only */
+
+/* A cache of K and V rows in pages.  Row r of page p and kv head h starts at
+ * element p * page_stride + r * row_stride + h * head_stride of k and of v, its
+ * head_dim elements side by side, so [page][row][head] and [page][head][row]
+ * pools both fit.  tables[seq * table_ld + s / page_size] is the page of
+ * sequence seq's row s; a row whose page is unmapped (outside [0, n_pages)) or
+ * past max_blocks takes no part in attention and is not stored.  A sequence in
+ * one piece is a page of its own length.  MLLM_E4M3: an element stands for
+ * code * 2^(e - 127), e = k_exp / v_exp[(p * n_kv_head + h) * page_size + r].
+ * head_dim a multiple of 16 up to 256; k, v and the strides multiples of 16
+ * bytes.  Pools may be longer than 32 bits count. */
+typedef struct {
+    int type;                      /* MLLM_F16, MLLM_BF16, MLLM_E4M3 */
+    int n_kv_head, head_dim;
+    int n_pages, page_size;
+    void *k, *v;
+    uint8_t *k_exp, *v_exp;        /* MLLM_E4M3 only */
+    long page_stride, row_stride, head_stride;
+    const int *tables;
+    int n_seqs, max_blocks;
+    long table_ld;
+} mllm_paged_kv;
+
+/* Rotary positions: per head the pairs (j, j + r/2) (MLLM_ROPE_HALF) or
+ * (2j, 2j + 1) (MLLM_ROPE_PAIRS), j < r/2, r = rope_dim (even, <= head_dim; 0:
+ * none), turned by pos * freqs[j] radians and multiplied by mscale; elements
+ * from r on are left as they are.  Angles are formed in 64 bits.
+ * freqs is device memory, made on the host by mllm_rotary_freqs: base^(-2j/r),
+ * for long contexts
+ *   LINEAR  divided by factor
+ *   NTK     with base * factor^(r / (r - 2))
+ *   YARN    divided by factor for the pairs that turn less than beta_slow times
+ *           in ctx positions, as they are above beta_fast times, a linear ramp
+ *           over the pairs between; mscale 0.1 ln(factor) + 1 (factor > 1)
+ *   BANDS   the same by wavelength: divided by factor where ctx holds fewer than
+ *           beta_slow turns, as they are above beta_fast, blended by the number
+ *           of turns between
+ * beta_fast / beta_slow <= 0 take 32 / 1 (YARN) and 4 / 1 (BANDS). */
+#define MLLM_ROPE_HALF 0
+#define MLLM_ROPE_PAIRS 1
+#define MLLM_ROPE_NONE 0
+#define MLLM_ROPE_LINEAR 1
+#define MLLM_ROPE_NTK 2
+#define MLLM_ROPE_YARN 3
+#define MLLM_ROPE_BANDS 4
+typedef struct {
+    int layout, rope_dim;
+    const double *freqs;           /* device, [rope_dim / 2] */
+    float mscale;
+} mllm_rotary;
+MLLM_API int mllm_rotary_freqs(int scaling, int rope_dim, double base, double factor, double ctx, double beta_fast,
+                               double beta_slow, double *freqs, float *mscale);
+
+/* T new tokens: q [NH heads] turned into q_out (out_type), k turned and, with
+ * v, stored as row rows[t] (NULL: pos[t]) of sequence seqs[t] (NULL: t) of kv;
+ * k also to k_out (out_type) where that is given.  Token t's heads lie side by
+ * side at q + t * q_ld (elements of in_type), so the three may be parts of one
+ * fused buffer.  q, or k with v, may be NULL (no such part); kv may be NULL
+ * (nothing is stored, v is not read).  q_out may be q and k_out may be k where
+ * the types and strides are the same; other overlaps are not supported.  A
+ * token with pos < 0 is left out (its outputs keep their contents); one whose
+ * sequence or row is outside the tables, or on an unmapped page, is not
+ * stored.  in_type and out_type: MLLM_F32, _F16, _BF16.  To an MLLM_E4M3 cache
+ * a row is rounded once, from 64 bits, under the least 2^e, -100 <= e <= 100,
+ * that brings its largest element to 448 or below (e = 0 for a row of zeros; a
+ * row that holds an infinity or a NaN takes e = 0, those elements become NaN
+ * and the others saturate). */
+MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void *q, long q_ld, const void *k, long k_ld,
+                                const void *v, long v_ld, const int *pos, int T, int NH, int NKH, int HD, int out_type,
+                                void *q_out, long q_out_ld, void *k_out, long k_out_ld, const mllm_paged_kv *kv,
+                                const int *seqs, const int *rows, void *stream);
+
+/* Attention over a paged cache, query head h reading kv head
+ * h / (NH / n_kv_head):
+ *   out = sum_s exp(z_s) v_s / (sum_s exp(z_s) + exp(sinks[h])), z_s = scale * q . k_s,
+ * over the mapped rows s <= p that the query at position p sees, with window
+ * w > 0 only those of s > p - w (the sink's term only where sinks is given,
+ * fp32 [NH]).  A query that sees no row gives zeros.  lens[i] (device) is the
+ * number of cached rows of the i-th sequence, the new tokens' own among them;
+ * it is taken as at most max_len.  The i-th sequence reads table row seqs[i]
+ * (NULL: i); one outside the tables has no rows.
+ *   decode: one query per sequence, at position lens[i] - 1
+ *   prompt: sequence i has the queries starts[i] .. starts[i + 1] - 1 (device,
+ *           [B + 1], ascending, within T), the last at position lens[i] - 1;
+ *           rows of out behind starts[B] are left as they were
+ * q [.][NH * HD] with row stride q_ld, out likewise, in q_type and out_type:
+ * MLLM_F32 or the cache's own type (MLLM_BF16 for MLLM_E4M3), 16-byte aligned
+ * rows.  Scores, softmax and sums are fp32; with 16-bit q and out the weights
+ * are rounded to 16 bits for the product with V, with fp32 in either place q
+ * and the weights keep fp32's precision.  NH / n_kv_head is not limited.
+ * Workspace: mllm_paged_attn_workspace_size bytes (tokens T, for decode B);
+ * one for a T, B and max_len serves every smaller one, and calls that overlap
+ * need one each.  Results are the same from call to call. */
+MLLM_API long mllm_paged_attn_workspace_size(const mllm_paged_kv *kv, int T, int B, int NH, int max_len, int window);
+MLLM_API int mllm_paged_attn_decode(const mllm_paged_kv *kv, int q_type, const void *q, long q_ld, const int *seqs,
+                                    const int *lens, int max_len, int B, int NH, float scale, int window,
+                                    const float *sinks, int out_type, void *out, long out_ld, void *workspace,
+                                    long ws_bytes, void *stream);
+MLLM_API int mllm_paged_attn_prompt(const mllm_paged_kv *kv, int q_type, const void *q, long q_ld, const int *seqs,
+                                    const int *starts, const int *lens, int max_len, int T, int B, int NH, float scale,
+                                    int window, const float *sinks, int out_type, void *out, long out_ld,
+                                    void *workspace, long ws_bytes, void *stream);
+
+/* Who holds which page, on the device: tables [n_seqs][table_ld] (the first
+ * max_blocks of each row; -1 unmapped) and refs [n_pages], the number of table
+ * entries that name a page; a page of refs 0 is free.  Pages are given lowest
+ * free first, in the order of the requests, so the result of a call depends on
+ * nothing but its inputs.  An entry outside [0, n_pages) counts as unmapped. */
+typedef struct {
+    int *tables;
+    int n_seqs, max_blocks;
+    long table_ld;
+    int *refs;
+    int n_pages, page_size;
+} mllm_page_map;
+/* Memory that holds a slice of every page: layer l, page p at base +
+ * l * layer_bytes + p * page_bytes (one for K, one for V, each with all its
+ * layers, and one for each kind of scales; up to MLLM_PAGE_PLANES). */
+#define MLLM_PAGE_PLANES 8
+typedef struct {
+    void *base;
+    long page_bytes, layer_bytes;
+    int n_layers;
+} mllm_page_plane;
+/* Bytes for a call with n requests. */
+MLLM_API long mllm_pages_workspace_size(const mllm_page_map *map, int n);
+/* Sequence seqs[i] gets pages for its unmapped blocks below lens[i] rows. */
+MLLM_API int mllm_pages_reserve(const mllm_page_map *map, int n, const int *seqs, const int *lens, int *status,
+                                void *workspace, long ws_bytes, void *stream);
+/* Sequence seqs[i] gives back its blocks past the first lens[i] rows (lens NULL: all). */
+MLLM_API int mllm_pages_free(const mllm_page_map *map, int n, const int *seqs, const int *lens, void *stream);
+/* children[i] takes over the first lens[i] rows of parents[i]: whole pages are
+ * shared, a part-filled last one is copied (all planes) to a page of its own,
+ * and the child's former pages are given back -- as if all at once, so a
+ * sequence may be parent and child in one call; parents[i] == children[i]
+ * changes nothing. */
+MLLM_API int mllm_pages_fork(const mllm_page_map *map, const mllm_page_plane *planes, int n_planes, int n,
+                             const int *parents, const int *children, const int *lens, int *status, void *workspace,
+                             long ws_bytes, void *stream);
+/* Of L live pages those at L or above move, lowest first, to the free ones
+ * below, lowest first, so that the pages [L, n_pages) are free; every table
+ * entry and all planes follow. */
+MLLM_API int mllm_pages_compact(const mllm_page_map *map, const mllm_page_plane *planes, int n_planes, int *status,
+                                void *workspace, long ws_bytes, void *stream);
+/* Page dst[i] := page src[i], i < n (device arrays).  No dst is a src or twice
+ * in the list; a pair outside [0, n_pages) is skipped. */
+MLLM_API int mllm_pages_copy(const mllm_page_plane *planes, int n_planes, int n_pages, int n, const int *src,
+                             const int *dst, void *stream);
+/* status (device int, written by each call): reserve and fork: the blocks that
+ * found no free page (they stay unmapped) plus the requests left out: a
+ * sequence outside [0, n_seqs), one listed before in the same call (reserve: in
+ * seqs, fork: in children), lens outside the tables' rows; compact: L. */
+
 #ifdef __cplusplus
 }
 #endif

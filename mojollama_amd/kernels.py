@@ -54,6 +54,35 @@ class KVView(ctypes.Structure):
 
 ATTN_CE, ATTN_GQA_C = 0, 1   # CE:141-158 gqa / gqa_attention.c:93 softmax
 
+# Element types, and the layouts and scalings of rotary positions (include/mllm.h).
+T_F32, T_F16, T_BF16, T_E4M3 = range(4)
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
+_cl = ctypes.c_long
+
+
+class PagedKV(ctypes.Structure):
+    """mllm_paged_kv (include/mllm.h): a paged 16- or 8-bit KV cache."""
+    _fields_ = [("type", ci), ("n_kv_head", ci), ("head_dim", ci), ("n_pages", ci), ("page_size", ci), ("k", cvp),
+                ("v", cvp), ("k_exp", cvp), ("v_exp", cvp), ("page_stride", _cl), ("row_stride", _cl),
+                ("head_stride", _cl), ("tables", cvp), ("n_seqs", ci), ("max_blocks", ci), ("table_ld", _cl)]
+
+
+class Rotary(ctypes.Structure):
+    """mllm_rotary (include/mllm.h): layout, width and frequencies of rotary positions."""
+    _fields_ = [("layout", ci), ("rope_dim", ci), ("freqs", cvp), ("mscale", ctypes.c_float)]
+
+
+class PageMap(ctypes.Structure):
+    """mllm_page_map (include/mllm.h): which sequence holds which page."""
+    _fields_ = [("tables", cvp), ("n_seqs", ci), ("max_blocks", ci), ("table_ld", _cl), ("refs", cvp), ("n_pages", ci),
+                ("page_size", ci)]
+
+
+class PagePlane(ctypes.Structure):
+    """mllm_page_plane (include/mllm.h): memory that holds a slice of every page."""
+    _fields_ = [("base", cvp), ("page_bytes", _cl), ("layer_bytes", _cl), ("n_layers", ci)]
+
 
 class GptOssDesc(ctypes.Structure):
     """mllm_gptoss_desc (include/mllm.h): host pointers to gptoss_forward's weights."""
@@ -217,6 +246,33 @@ def load_kernels(path=LIB_PATH):
     so.mllm_kv_append.restype = ci
     so.mllm_rope.argtypes = [cvp, ci, ci, ci, cvp, cvp, cvp, ci, cvp]
     so.mllm_rope.restype = ci
+    # --- paged 16- or 8-bit KV cache: rotary positions, attention, pages
+    pkv, pmap, pplane = ctypes.POINTER(PagedKV), ctypes.POINTER(PageMap), ctypes.POINTER(PagePlane)
+    so.mllm_rotary_freqs.argtypes = [ci, ci] + [ctypes.c_double] * 5 + [ctypes.POINTER(ctypes.c_double), cf]
+    so.mllm_rotary_freqs.restype = ci
+    so.mllm_rotary_append.argtypes = ([ctypes.POINTER(Rotary), ci, cvp, _cl, cvp, _cl, cvp, _cl, cvp, ci, ci, ci, ci, ci,
+                                       cvp, _cl, cvp, _cl, pkv, cvp, cvp, cvp])
+    so.mllm_rotary_append.restype = ci
+    so.mllm_paged_attn_workspace_size.argtypes = [pkv, ci, ci, ci, ci, ci]
+    so.mllm_paged_attn_workspace_size.restype = _cl
+    so.mllm_paged_attn_decode.argtypes = [pkv, ci, cvp, _cl, cvp, cvp, ci, ci, ci, ctypes.c_float, ci, cvp, ci, cvp,
+                                          _cl, cvp, _cl, cvp]
+    so.mllm_paged_attn_decode.restype = ci
+    so.mllm_paged_attn_prompt.argtypes = [pkv, ci, cvp, _cl, cvp, cvp, cvp, ci, ci, ci, ci, ctypes.c_float, ci, cvp, ci,
+                                          cvp, _cl, cvp, _cl, cvp]
+    so.mllm_paged_attn_prompt.restype = ci
+    so.mllm_pages_workspace_size.argtypes = [pmap, ci]
+    so.mllm_pages_workspace_size.restype = _cl
+    so.mllm_pages_reserve.argtypes = [pmap, ci, cvp, cvp, cvp, cvp, _cl, cvp]
+    so.mllm_pages_reserve.restype = ci
+    so.mllm_pages_free.argtypes = [pmap, ci, cvp, cvp, cvp]
+    so.mllm_pages_free.restype = ci
+    so.mllm_pages_fork.argtypes = [pmap, pplane, ci, ci, cvp, cvp, cvp, cvp, cvp, _cl, cvp]
+    so.mllm_pages_fork.restype = ci
+    so.mllm_pages_compact.argtypes = [pmap, pplane, ci, cvp, cvp, _cl, cvp]
+    so.mllm_pages_compact.restype = ci
+    so.mllm_pages_copy.argtypes = [pplane, ci, ci, ci, cvp, cvp, cvp]
+    so.mllm_pages_copy.restype = ci
     # gptoss_forward (GO:96-130 argument list)
     pcu, pcf, pci = ctypes.POINTER(cu), ctypes.POINTER(cf), ctypes.POINTER(ci)
     so.gptoss_forward.argtypes = ([pci, ci, cf, ci] + [pcu] * 4 + [pcf] * 2 + [pci] * 8 + [cu, ci, ci, ci, cf, cf, pci,
@@ -393,6 +449,230 @@ class DeviceOps:
         self._check(self.so.mllm_rope(buf.data_ptr(), T, NH, HD, pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(),
                                       rope_dim, self._stream()), "mllm_rope")
         return buf
+
+    # ------------------------------------------- paged 16- or 8-bit KV cache
+    def _type(self, t, what):
+        """mllm type of a tensor on the current GPU whose last dimension is dense."""
+        torch = self.torch
+        code = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}.get(
+            t.dtype)
+        if code is None:
+            raise TypeError(f"{what}: {t.dtype} is not served")
+        self._here(t, what)
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{what}: the last dimension is not dense")
+        return code
+
+    def _here(self, t, what):
+        if t.device.type != "cuda" or t.device.index != self.torch.cuda.current_device():
+            raise ValueError(f"{what}: a tensor on {t.device}, not on the current GPU")
+
+    def _ints(self, t, what, n=None):
+        """Address of a dense int32 tensor on the current GPU (None: a null pointer)."""
+        if t is None:
+            return None
+        self._here(t, what)
+        if t.dtype != self.torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
+            raise ValueError(f"{what}: a dense int32 tensor{'' if n is None else ' of %d' % n} is needed")
+        return t.data_ptr()
+
+    def paged_kv(self, k, v, tables, k_exp=None, v_exp=None):
+        """An mllm_paged_kv over pools k, v [n_pages, page_size, n_kv_head, head_dim] (float16, bfloat16 or
+        float8_e4m3fn; any strides, the last dimension dense, so a [page][head][row] pool is passed permuted) and
+        tables int32 [n_seqs, max_blocks]; float8 pools with their exponents uint8 [n_pages, n_kv_head, page_size].
+        The view keeps the tensors alive."""
+        torch = self.torch
+        code = self._type(k, "k")
+        if code != self._type(v, "v") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4:
+            raise ValueError("k and v: two pools [page, row, head, element] of one type, shape and strides")
+        self._here(tables, "tables")
+        if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1:
+            raise ValueError("tables: int32 [n_seqs, max_blocks], rows dense")
+        n_pages, page, heads, hd = k.shape
+        for e in (k_exp, v_exp):
+            if (e is None) != (code != T_E4M3):
+                raise ValueError("k_exp and v_exp belong to float8 pools")
+            if e is not None:
+                self._here(e, "exponents")
+                if e.dtype != torch.uint8 or tuple(e.shape) != (n_pages, heads, page) or not e.is_contiguous():
+                    raise ValueError("exponents: dense uint8 [n_pages, n_kv_head, page_size]")
+        p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        view = PagedKV(code, heads, hd, n_pages, page, p(k), p(v), p(k_exp), p(v_exp), k.stride(0), k.stride(1),
+                       k.stride(2), p(tables), tables.shape[0], tables.shape[1], tables.stride(0))
+        view._tensors = (k, v, tables, k_exp, v_exp)
+        return view
+
+    def rotary(self, rope_dim, layout=ROPE_HALF, base=10000.0, scaling=ROPE_NONE, factor=1.0, ctx=0.0, beta_fast=0.0,
+               beta_slow=0.0):
+        """An mllm_rotary with its frequencies on the current GPU (mllm_rotary_freqs)."""
+        f, m = (ctypes.c_double * max(rope_dim // 2, 1))(), ctypes.c_float()
+        self._check(self.so.mllm_rotary_freqs(scaling, rope_dim, base, factor, ctx, beta_fast, beta_slow, f,
+                                              ctypes.byref(m)), "mllm_rotary_freqs")
+        freqs = self.torch.tensor(list(f), dtype=self.torch.float64).cuda()
+        rot = Rotary(layout, rope_dim, freqs.data_ptr(), m.value)
+        rot._tensors = (freqs,)
+        return rot
+
+    def rotary_append(self, rot, q, k, v, pos, NH=0, NKH=0, HD=0, kv=None, seqs=None, rows=None, q_out=None, k_out=None):
+        """mllm_rotary_append: q [T, NH*HD], k, v [T, NKH*HD] (parts of a fused buffer may be passed as slices; q, or k
+        and v, may be None), pos int32 [T]; k and v go to rows `rows` (None: pos) of sequences `seqs` (None: 0, 1, ...)
+        of kv, the turned q to q_out and k to k_out.  Heads and head size come from kv where it is given."""
+        T = self._ints(pos, "pos") and pos.numel()
+        if kv is not None:
+            NKH, HD = kv.n_kv_head, kv.head_dim
+        parts = []
+        for t, n, what in ((q, NH * HD, "q"), (k, NKH * HD, "k"), (v, NKH * HD, "v"), (q_out, NH * HD, "q_out"),
+                           (k_out, NKH * HD, "k_out")):
+            if t is None:
+                parts += [None, None, 0]
+                continue
+            code = self._type(t, what)
+            if t.dim() != 2 or t.shape[0] != T or t.shape[1] != n:
+                raise ValueError(f"{what}: [{T}, {n}] is needed, got {list(t.shape)}")
+            parts += [code, t.data_ptr(), t.stride(0) if T > 1 else max(t.stride(0), n)]
+        ins, outs = {c for c in parts[0:9:3] if c is not None}, {c for c in parts[9::3] if c is not None}
+        if len(ins) > 1 or len(outs) > 1:
+            raise TypeError("q, k and v have one type, and q_out and k_out")
+        self._check(self.so.mllm_rotary_append(
+            rot, ins.pop() if ins else T_F32, parts[1], parts[2], parts[4], parts[5], parts[7], parts[8], pos.data_ptr(),
+            T, NH, NKH, HD, outs.pop() if outs else T_F32, parts[10], parts[11], parts[13], parts[14], kv,
+            self._ints(seqs, "seqs", T), self._ints(rows, "rows", T), self.torch.cuda.current_stream().cuda_stream),
+            "mllm_rotary_append")
+
+    def paged_attn_workspace(self, kv, T, B, NH, max_len, window=0):
+        """A workspace for paged_attn_decode (T = B) and paged_attn_prompt calls up to these sizes."""
+        n = self.so.mllm_paged_attn_workspace_size(kv, T, B, NH, max_len, window)
+        if n < 0:
+            raise ValueError("paged_attn_workspace: sizes that are not served")
+        return self.torch.empty(n, dtype=self.torch.uint8, device="cuda")
+
+    def _attn(self, kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws):
+        if q.dim() != 2 or q.shape[1] != NH * kv.head_dim:
+            raise ValueError(f"q: [tokens, {NH * kv.head_dim}] is needed, got {list(q.shape)}")
+        qt = self._type(q, "q")
+        if out is None:
+            out = self.torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+        elif out.shape != q.shape:
+            raise ValueError("out: the shape of q is needed")
+        if sinks is not None:
+            self._here(sinks, "sinks")
+            if sinks.dtype != self.torch.float32 or sinks.numel() != NH or not sinks.is_contiguous():
+                raise ValueError("sinks: dense float32 [NH]")
+        if ws is None:
+            ws = self.paged_attn_workspace(kv, T, B, NH, max_len, window)
+        else:
+            self._here(ws, "workspace")
+        n = q.shape[1]
+        return (qt, q.data_ptr(), q.stride(0) if T > 1 else max(q.stride(0), n), out, self._type(out, "out"),
+                out.data_ptr(), out.stride(0) if T > 1 else max(out.stride(0), n), ws,
+                sinks.data_ptr() if sinks is not None else None)
+
+    def paged_attn_decode(self, kv, q, lens, max_len, NH, scale=None, window=0, sinks=None, seqs=None, out=None,
+                          out_dtype=None, ws=None):
+        """mllm_paged_attn_decode: q [B, NH*HD], lens int32 [B] (cached rows, the new one among them, at most max_len);
+        scale None: 1/sqrt(HD); out in out_dtype (None: q's)."""
+        B = q.shape[0]
+        qt, qp, ql, out, ot, op, ol, ws, sk = self._attn(kv, q, B, B, NH, max_len, window, sinks, out, out_dtype, ws)
+        self._check(self.so.mllm_paged_attn_decode(
+            kv, qt, qp, ql, self._ints(seqs, "seqs", B), self._ints(lens, "lens", B), max_len, B, NH,
+            kv.head_dim ** -0.5 if scale is None else scale, window, sk, ot, op, ol, ws.data_ptr(),
+            ws.numel() * ws.element_size(), self.torch.cuda.current_stream().cuda_stream), "mllm_paged_attn_decode")
+        return out
+
+    def paged_attn_prompt(self, kv, q, starts, lens, max_len, NH, scale=None, window=0, sinks=None, seqs=None, out=None,
+                          out_dtype=None, ws=None):
+        """mllm_paged_attn_prompt: q [T, NH*HD] holds the new tokens of B sequences, starts int32 [B + 1], lens int32
+        [B] (cached rows, the new ones among them, at most max_len)."""
+        T, B = q.shape[0], lens.numel()
+        qt, qp, ql, out, ot, op, ol, ws, sk = self._attn(kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws)
+        self._check(self.so.mllm_paged_attn_prompt(
+            kv, qt, qp, ql, self._ints(seqs, "seqs", B), self._ints(starts, "starts", B + 1), self._ints(lens, "lens", B),
+            max_len, T, B, NH, kv.head_dim ** -0.5 if scale is None else scale, window, sk, ot, op, ol, ws.data_ptr(),
+            ws.numel() * ws.element_size(), self.torch.cuda.current_stream().cuda_stream), "mllm_paged_attn_prompt")
+        return out
+
+    def page_map(self, tables, refs, page_size):
+        """An mllm_page_map over tables int32 [n_seqs, max_blocks] (-1 unmapped) and refs int32 [n_pages]."""
+        self._here(tables, "tables")
+        if tables.dtype != self.torch.int32 or tables.dim() != 2 or tables.stride(1) != 1:
+            raise ValueError("tables: int32 [n_seqs, max_blocks], rows dense")
+        m = PageMap(tables.data_ptr(), tables.shape[0], tables.shape[1], tables.stride(0), self._ints(refs, "refs"),
+                    refs.numel(), page_size)
+        m._tensors = (tables, refs)
+        return m
+
+    def page_planes(self, pools):
+        """mllm_page_plane entries of pools [n_layers, n_pages, ...], each layer's pages dense (K, V, and the exponents
+        of float8 pools)."""
+        planes = (PagePlane * len(pools))()
+        for p, t in zip(planes, pools):
+            self._here(t, "pool")
+            if t.dim() < 2 or not t[0].is_contiguous():
+                raise ValueError("pools: [n_layers, n_pages, ...], each layer dense")
+            p.base, p.n_layers = t.data_ptr(), t.shape[0]
+            p.page_bytes, p.layer_bytes = t.stride(1) * t.element_size(), t.stride(0) * t.element_size()
+        planes._tensors, planes._n_pages = tuple(pools), min((t.shape[1] for t in pools), default=None)
+        return planes
+
+    def pages_workspace(self, m, n):
+        """A workspace for pages_reserve and pages_fork calls of up to n requests, and pages_compact."""
+        return self.torch.empty(self.so.mllm_pages_workspace_size(m, n), dtype=self.torch.uint8, device="cuda")
+
+    def _pages_args(self, m, n, status, ws):
+        torch = self.torch
+        if status is None:
+            status = torch.empty(1, dtype=torch.int32, device="cuda")
+        if ws is None:
+            ws = self.pages_workspace(m, n)
+        self._here(ws, "workspace")
+        return status, self._ints(status, "status"), ws
+
+    @staticmethod
+    def _pages_in(planes, n_pages):
+        if planes._n_pages is not None and planes._n_pages < n_pages:
+            raise ValueError(f"a pool holds {planes._n_pages} pages, not {n_pages}")
+
+    def pages_reserve(self, m, seqs, lens, status=None, ws=None):
+        """mllm_pages_reserve: pages for rows below lens[i] of sequences seqs[i]; returns status (a device int32, 0 when
+        every request was met)."""
+        n = seqs.numel()
+        status, sp, ws = self._pages_args(m, n, status, ws)
+        self._check(self.so.mllm_pages_reserve(m, n, self._ints(seqs, "seqs"), self._ints(lens, "lens", n), sp,
+                                               ws.data_ptr(), ws.numel() * ws.element_size(), self._stream()),
+                    "mllm_pages_reserve")
+        return status
+
+    def pages_free(self, m, seqs, lens=None):
+        """mllm_pages_free: sequences seqs[i] give back their pages past the first lens[i] rows (None: all)."""
+        n = seqs.numel()
+        self._check(self.so.mllm_pages_free(m, n, self._ints(seqs, "seqs"), self._ints(lens, "lens", n), self._stream()),
+                    "mllm_pages_free")
+
+    def pages_fork(self, m, planes, parents, children, lens, status=None, ws=None):
+        """mllm_pages_fork: children[i] takes over the first lens[i] rows of parents[i], all at once; returns status."""
+        n = parents.numel()
+        self._pages_in(planes, m.n_pages)
+        status, sp, ws = self._pages_args(m, n, status, ws)
+        self._check(self.so.mllm_pages_fork(m, planes, len(planes), n, self._ints(parents, "parents"),
+                                            self._ints(children, "children", n), self._ints(lens, "lens", n), sp,
+                                            ws.data_ptr(), ws.numel() * ws.element_size(), self._stream()),
+                    "mllm_pages_fork")
+        return status
+
+    def pages_compact(self, m, planes, status=None, ws=None):
+        """mllm_pages_compact: the live pages move to the front; returns their number (a device int32)."""
+        self._pages_in(planes, m.n_pages)
+        status, sp, ws = self._pages_args(m, 0, status, ws)
+        self._check(self.so.mllm_pages_compact(m, planes, len(planes), sp, ws.data_ptr(),
+                                               ws.numel() * ws.element_size(), self._stream()), "mllm_pages_compact")
+        return status
+
+    def pages_copy(self, planes, n_pages, src, dst):
+        """mllm_pages_copy: page dst[i] := page src[i] in every plane."""
+        n = src.numel()
+        self._pages_in(planes, n_pages)
+        self._check(self.so.mllm_pages_copy(planes, len(planes), n_pages, n, self._ints(src, "src"),
+                                            self._ints(dst, "dst", n), self._stream()), "mllm_pages_copy")
 
     def moe_prepare(self, qts, N, M, E, K, gates, ups, downs, router, renorm):
         """gates/ups/downs: per-expert raw GGUF uint8 tensors (GPU) in the
