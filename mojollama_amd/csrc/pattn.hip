@@ -1,20 +1,9 @@
 // pattn.hip — attention of new tokens over a paged 16- or 8-bit KV cache.
 #include <math.h>
-#include "paged.h"
+#include <algorithm>
+#include "pattn.h"
 
 namespace {
-
-struct pa_args {
-    const void *q;
-    void *out;
-    long q_ld, out_ld;
-    int q_type, out_type;
-    mllm_paged_kv kv;
-    const int *seqs, *starts, *lens;
-    int max_len, T, B, NH, window;
-    float scale;
-    const float *sinks;
-};
 
 // One workgroup per query and head: 256 positions at a time, a score per thread, the running maximum
 // and sum, then an element of the output per thread.
@@ -114,7 +103,8 @@ const char *pa_refusal(const mllm_paged_kv *kv, int q_type, const void *q, long 
     if (const char *why = pk_refusal(kv)) return why;
     if (T < 0 || B < 0 || max_len < 0 || NH <= 0 || NH % kv->n_kv_head || window < 0)
         return "NH is a multiple of n_kv_head, counts and window are not negative";
-    if ((long)T * NH > 1 << 30 || NH > 65535) return "at most 2^30 queries times heads, 65535 heads";
+    if ((long)T * NH > 1 << 30 || NH > 65535 || B > 65535 || max_len > 1 << 30)
+        return "at most 2^30 queries times heads, 65535 heads and sequences, max_len 2^30";
     if ((T && (!q || !out)) || (B && !lens)) return "q, lens and out are needed";
     const int own = kv->type == MLLM_F16 ? MLLM_F16 : MLLM_BF16;
     if ((q_type != MLLM_F32 && q_type != own) || (out_type != MLLM_F32 && out_type != own))
@@ -125,9 +115,97 @@ const char *pa_refusal(const mllm_paged_kv *kv, int q_type, const void *q, long 
     return nullptr;
 }
 
-int pa_launch(const char *who, pa_args &a, void *stream)
+// The splits of a query's rows joined: their sums under one maximum.  One row (query and head) per
+// workgroup; HD / 4 threads cover a split's sums, the groups of so many threads take every
+// (256 / (HD / 4))-th split.
+__global__ __launch_bounds__(256) void k_pa_join(pa_args a)
 {
-    hipLaunchKernelGGL(k_pattn, dim3(a.T, a.NH), dim3(256), 0, (hipStream_t)stream, a);
+    __shared__ float wt[256], red[2][4];
+    __shared__ __attribute__((aligned(16))) float acc[256 * 4];
+    const int h = blockIdx.y, t = blockIdx.x, tid = threadIdx.x, HD = a.kv.head_dim;
+    if (a.starts && (t < a.starts[0] || t >= a.starts[a.B])) return;
+    const long row = (long)t * a.NH + h;
+    float2 ml = make_float2(kLowest, 0.0f);
+    if (tid < a.splits) ml = *(const float2 *)(a.stat + (row * a.splits + tid) * 2);
+    float m = ml.x;
+    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (!(tid & 63)) red[0][tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float f = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    wt[tid] = f;
+    float l = f * ml.y;
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d, 64);
+    if (!(tid & 63)) red[1][tid >> 6] = l;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    const int n = HD / 4, ng = 256 / n, gi = tid / n, d = 4 * (tid - gi * n);
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (gi < ng)
+        for (int s = gi; s < a.splits; s += ng) {
+            const float u = wt[s];
+            if (u == 0.0f) continue;                 // an empty split's sums are not written
+            const float4 x = *(const float4 *)(a.part + (row * a.splits + s) * HD + d);
+            y.x = fmaf(u, x.x, y.x); y.y = fmaf(u, x.y, y.y); y.z = fmaf(u, x.z, y.z); y.w = fmaf(u, x.w, y.w);
+        }
+    *(float4 *)(acc + 4 * tid) = y;
+    __syncthreads();
+    if (gi) return;
+    for (int s = 1; s < ng; s++) {
+        const float4 x = *(const float4 *)(acc + 4 * (tid + s * n));
+        y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+    }
+    pa_finish(a, h, t, d, m, l, y);
+}
+
+constexpr int kMaxSplits = 256, kMinRows = 256;      // rows of a split at least
+constexpr long kTargetWG = 1024;
+
+// Rows that a query can see, as far as the host knows.
+long seen(int max_len, int window) { return window > 0 ? std::min<long>(max_len, (long)window + 31) : max_len; }
+
+// Splits of a launch of `wgs` workgroups that each would take all of n rows.
+int pa_splits(long wgs, long n)
+{
+    const long want = std::min<long>((kTargetWG + wgs - 1) / wgs, (n + kMinRows - 1) / kMinRows);
+    return (int)std::max<long>(1, std::min<long>(want, kMaxSplits));
+}
+
+void pa_divisor(pa_args &a)
+{
+    // s / d = s * m >> (31 + l) for s < 2^31, with l = ceil(log2 d), m = floor(2^(31 + l) / d) + 1 (Granlund
+    // and Montgomery); m is below 2^32
+    const uint64_t d = (uint64_t)a.kv.page_size;
+    int l = 0;
+    while ((1ull << l) < d) l++;
+    a.div_mul = (unsigned)(((1ull << (31 + l)) / d) + 1);
+    a.div_sh = 31 + l;
+}
+
+int pa_launch(const char *who, pa_args &a, void *ws, void *stream)
+{
+    hipStream_t st = (hipStream_t)stream;
+    pa_divisor(a);
+    a.rep = a.NH / a.kv.n_kv_head;
+    const bool wide = a.q_type == MLLM_F32 || a.out_type == MLLM_F32;
+    const int es = pk_size(a.kv.type);
+    if (!a.starts) {
+        const bool uniform = a.kv.page_size % 16 == 0 && a.kv.row_stride * 16 * es < 0x7FFFFFFF &&
+                             (es == 2 || !(((uintptr_t)a.kv.k_exp | (uintptr_t)a.kv.v_exp) & 3));
+        a.groups = (a.rep + 15) / 16;
+        const long n = seen(a.max_len, a.window);
+        a.splits = pa_splits((long)a.B * a.kv.n_kv_head * a.groups, n);
+        a.chunk = (int)std::min<long>(0x7FFFFF80, (n + a.splits - 1) / a.splits / 128 * 128 + 128);
+        a.splits = (int)std::max<long>(1, (n + a.chunk - 1) / a.chunk);
+        a.stat = (float *)ws;
+        a.part = a.stat + ((long)a.T * a.NH * a.splits * 2 + 3) / 4 * 4;
+        if (a.kv.type == MLLM_F16) pa_decode_f16(a, wide, uniform, st);
+        else if (a.kv.type == MLLM_BF16) pa_decode_bf16(a, wide, uniform, st);
+        else pa_decode_e4m3(a, wide, uniform, st);
+        if (a.splits > 1) hipLaunchKernelGGL(k_pa_join, dim3(a.T, a.NH), dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL(k_pattn, dim3(a.T, a.NH), dim3(256), 0, st, a);
+    }
     return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed");
 }
 
@@ -138,7 +216,11 @@ extern "C" {
 MLLM_API long mllm_paged_attn_workspace_size(const mllm_paged_kv *kv, int T, int B, int NH, int max_len, int window)
 {
     if (pk_refusal(kv) || T < 0 || B < 0 || NH <= 0 || NH % kv->n_kv_head || max_len < 0 || window < 0) return -1;
-    return 256;
+    // rows (query and head) times splits: each row has at most its range's, all rows together the target
+    // number of workgroups' worth and one each; both grow with every size, so a workspace serves smaller calls
+    const long rows = (long)T * NH, rep = std::min<long>(NH / kv->n_kv_head, 16), n = seen(max_len, window);
+    const long most = std::max<long>(1, std::min<long>((n + kMinRows - 1) / kMinRows, kMaxSplits));
+    return 4 * (std::min(rows * most, rep * kTargetWG + rows) * (kv->head_dim + 2) + 64);
 }
 
 MLLM_API int mllm_paged_attn_decode(const mllm_paged_kv *kv, int q_type, const void *q, long q_ld, const int *seqs,
@@ -154,7 +236,7 @@ MLLM_API int mllm_paged_attn_decode(const mllm_paged_kv *kv, int q_type, const v
         return pk_fail(who, "workspace below mllm_paged_attn_workspace_size");
     if (!B) return 0;
     pa_args a{q, out, q_ld, out_ld, q_type, out_type, *kv, seqs, nullptr, lens, max_len, B, B, NH, window, scale, sinks};
-    return pa_launch(who, a, stream);
+    return pa_launch(who, a, workspace, stream);
 }
 
 MLLM_API int mllm_paged_attn_prompt(const mllm_paged_kv *kv, int q_type, const void *q, long q_ld, const int *seqs,
@@ -171,7 +253,7 @@ MLLM_API int mllm_paged_attn_prompt(const mllm_paged_kv *kv, int q_type, const v
         return pk_fail(who, "workspace below mllm_paged_attn_workspace_size");
     if (!T || !B) return 0;
     pa_args a{q, out, q_ld, out_ld, q_type, out_type, *kv, seqs, starts, lens, max_len, T, B, NH, window, scale, sinks};
-    return pa_launch(who, a, stream);
+    return pa_launch(who, a, workspace, stream);
 }
 
 } // extern "C"
