@@ -17,6 +17,7 @@ struct pa_args {
     unsigned div_mul;              // s / page_size = s * div_mul >> div_sh for 0 <= s < 2^31
     int div_sh;
     int chunk, splits;             // rows per split, splits of a query's range of rows
+    int tiles;                     // tiles of 128 rows at most (prompt)
     float *part, *stat;            // with splits > 1: sums [T * NH][splits][HD], (maximum, sum) [T * NH][splits]
 };
 
@@ -34,9 +35,6 @@ __device__ __forceinline__ int pa_table(const pa_args &a, int seq, int blk)
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-template <int CT> struct pa_half { typedef bf16x8 v8; };
-template <> struct pa_half<MLLM_F16> { typedef f16x8 v8; };
 
 template <int CT> __device__ __forceinline__ f32x4 pa_mfma16(uint4 x, uint4 y, f32x4 c)
 {
@@ -103,3 +101,6 @@ __device__ __forceinline__ void pa_finish(const pa_args &a, int h, int t, int d,
 void pa_decode_bf16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_f16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_e4m3(const pa_args &a, bool wide, bool uniform, hipStream_t st);
+void pa_prompt_bf16(const pa_args &a, bool wide, hipStream_t st);
+void pa_prompt_f16(const pa_args &a, bool wide, hipStream_t st);
+void pa_prompt_e4m3(const pa_args &a, bool wide, hipStream_t st);

@@ -1,0 +1,2 @@
+#include "pattn_prompt.h"
+void pa_prompt_e4m3(const pa_args &a, bool wide, hipStream_t st) { pa_prompt<MLLM_E4M3>(a, wide, st); }

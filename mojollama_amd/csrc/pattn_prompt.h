@@ -1,0 +1,424 @@
+// pattn_prompt.h — the tiled prompt kernel over a paged cache, instantiated per cache type.
+#pragma once
+#include <math.h>
+#include <type_traits>
+#include "pattn.h"
+
+template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, f32x16 c)
+{
+    if constexpr (CT == MLLM_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+
+// Rows that hold nothing are read from here.
+static __device__ const uint4 pa_zeros[1] = {};
+
+// 128 rows of queries against the rows of one kv head, 64 of these at a time (32 at head sizes
+// above 128).  A row is a (token, head) pair of the heads that share the kv head, tokens outer, so a
+// tile of K and V serves all of them and a few drafted tokens fill a wave; each of four waves owns 32.
+//   S^T = K Q^T   (32x32x16): q stays in registers as the second operand; a lane holds half of the
+//                 scores of one row (lane % 32), so maximum and sum are the lane's own
+//   O^T += V^T P  the scores' registers are this product's second operand as they stand: slot
+//                 8 (lane / 32) + e of its k index is row 8 (e / 4) + 4 (lane / 32) + e % 4, and V's
+//                 operand is read transposed from LDS (ds_read_b64_tr_b16) in the same order
+// K and V go straight to LDS, one step ahead, in two buffers (separate objects: a wait for one is no
+// wait for the other); 16-byte pieces are permuted within their row so that the operand reads of 16
+// lanes (K: 16 rows; V: 4 rows of 64 bytes) fall on distinct banks.  8-bit caches pass through
+// registers, where they become bf16.
+//
+// A weight of 0 times an infinity or a NaN that a masked row of V holds is NaN, so in the tiles where
+// some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
+// element by element to the queries that do see them.  Rows that no query of the sequence sees (past
+// the length, on unmapped pages) are read as zeros.
+template <int CT, bool HP, int HDB>
+__global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa_prompt(pa_args a)
+{
+    constexpr bool E8 = CT == MLLM_E4M3;
+    constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1;
+    constexpr int TK = HDB > 128 ? 32 : 64, NB = TK / 32;    // rows per step, in blocks of 32
+    constexpr int KS = HDB / 16, OB = HDB / 32;
+    constexpr int RB = HDB * 2;                              // bytes of a row in LDS
+    constexpr int LPR = HDB * ES / 16, RI = 64 / LPR, NI = TK / (4 * RI);   // lanes per row, rows per load, loads per wave
+    __shared__ __attribute__((aligned(1024))) uint8_t k0[TK * RB], v0[TK * RB], k1[TK * RB], v1[TK * RB];
+    __shared__ uint32_t odd[2][4];                           // rows of V that hold infinities or NaN, per wave's part
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hh = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int NKH = a.kv.n_kv_head, j = blockIdx.x % NKH, HD = a.kv.head_dim, sp = blockIdx.y, rep = a.rep;
+
+    // which sequence and tile: 64 sequences at a time
+    int t = blockIdx.x / NKH, b = -1, tiles = 0;
+    for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
+        const int bb = b0 + lane;
+        const int n = bb < a.B ? (int)(((long)max(0, a.starts[bb + 1] - a.starts[bb]) * rep + 127) / 128) : 0;
+        int sum = n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += y;
+        }
+        const unsigned long long in = __ballot(t < sum);
+        if (in) {
+            const int f = __builtin_ctzll(in);
+            b = b0 + f;
+            tiles = __shfl(n, f, 64);
+            t -= __shfl(sum, f, 64) - tiles;
+        } else {
+            t -= __shfl(sum, 63, 64);
+        }
+    }
+    if (b < 0) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    const int tile = __builtin_amdgcn_readfirstlane(tiles - 1 - t);     // the last rows, which see most, first
+    const int q0 = a.starts[b], nq = a.starts[b + 1] - q0;
+    const int seq = a.seqs ? a.seqs[b] : b;
+    const int len0 = min(a.lens[b], a.max_len);
+    int len = seq >= 0 && seq < a.kv.n_seqs ? len0 : 0;
+    len = min(len, (int)min((long)a.kv.max_blocks * a.kv.page_size, 0x7FFFFFFFl));
+    const int nrows = (int)min(128l, (long)nq * rep - tile * 128l);      // of the tile
+    const int first = (int)((long)tile * 128 / rep), last = (int)(((long)tile * 128 + nrows - 1) / rep);   // tokens
+    // positions of a token's query: len0 - nq + token; it sees (p - window, p]
+    const int off = len0 - nq;
+    const int lo = a.window > 0 ? max(0, off + first - a.window + 1) : 0, hi = min(len, off + last + 1);
+    const int begin = lo / TK * TK + sp * a.chunk, end = min(hi, begin + a.chunk);
+    // this lane's row
+    const int rr = 32 * w + c, r = min(rr, nrows - 1), tok = (int)((tile * 128l + r) / rep), h = j * rep + (int)((tile * 128l + r) - (long)tok * rep);
+    const int pr = off + tok, lr = a.window > 0 ? max(0, pr - a.window + 1) : 0;
+    const bool busy = 32 * w < nrows;                        // the wave has rows
+    // of the wave's rows: the least last position and the largest first one
+    const int wtok0 = (int)((tile * 128l + min(32 * w, nrows - 1)) / rep), wtok1 = (int)((tile * 128l + min(32 * w + 31, nrows - 1)) / rep);
+    const int pmin = off + wtok0, pmax = off + wtok1, lmax = a.window > 0 ? max(0, pmax - a.window + 1) : 0;
+    const int lmin = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
+    const long orow = (long)(q0 + tok) * a.NH + h;
+
+    if (begin >= end && a.splits > 1) {
+        if (hh == 0 && rr < nrows) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(kLowest, 0.0f);
+        return;
+    }
+
+    uint4 qf[NP][KS];
+    float zs = a.scale * kLog2e;
+    {
+        const long at = (long)(q0 + tok) * a.q_ld + (long)h * HD;
+        int e = 0;
+        if constexpr (HP && CT == MLLM_F16) {
+            // fp16 planes: the row's largest element to [2^14, 2^15)
+            float big = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                float x[8];
+                load8(a.q, at + min(16 * s + 8 * hh, HD - 8), a.q_type, true, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[i]));
+            }
+            big = fmaxf(big, __shfl_xor(big, 32, 64));
+            e = big > 0.0f && big < INFINITY ? 15 - (int)((__float_as_uint(big) >> 23) & 255) + 126 : 0;
+            zs = ldexpf(zs, -e);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int col = 16 * s + 8 * hh;
+            float x[8];
+            load8(a.q, at + min(col, HD - 8), a.q_type, true, x);
+            uint32_t p[4][NP];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float u = col < HD ? x[2 * i] : 0.0f, v = col < HD ? x[2 * i + 1] : 0.0f;
+                if constexpr (HP && CT == MLLM_F16) { u = ldexpf(u, e); v = ldexpf(v, e); }
+                pa_planes<CT, NP>(u, v, p[i]);
+#pragma unroll
+                for (int n = 1; n < NP; n++) {               // an infinity's rest is 0
+                    if (!(fabsf(u) < INFINITY)) p[i][n] &= 0xFFFF0000u;
+                    if (!(fabsf(v) < INFINITY)) p[i][n] &= 0xFFFFu;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NP; n++) qf[n][s] = make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]);
+        }
+    }
+
+    // ---- staging.  Row x's 16-byte piece y of K lies at piece y ^ kx(x), of V at y ^ vx(x).
+    auto kx = [](int x) { return HDB == 64 ? (x >> 1) & 7 : x & 15; };
+    auto vx = [](int x) { return HDB == 64 ? (x >> 1 & 1) << 2 : (x & 3) << 2; };
+    const long rs = a.kv.row_stride * ES, ps = a.kv.page_stride * ES, hs = a.kv.head_stride * ES * j;
+    const uint8_t *kb = (const uint8_t *)a.kv.k + hs, *vb = (const uint8_t *)a.kv.v + hs;
+    const int lrow = lane / LPR, lpc = lane & (LPR - 1);     // row of a load and piece
+    const bool even = a.kv.page_size % 16 == 0;
+    // Row TK/4 * w + RI * n + lrow of the step at s0: where it is, -1 if it holds nothing; returns which of
+    // the step's rows are on mapped pages, one bit each.
+    struct place { long row[NI], exp[NI]; };
+    auto find = [&](int s0, place &p) __attribute__((always_inline)) {
+        uint64_t on = 0;
+        if (even) {                                          // 16 rows lie in one page, so do the wave's
+            int page = 0, row = -1;
+#pragma unroll
+            for (int n = 0; n < TK / 16; n++) {
+                const int s = s0 + 16 * n, blk = pa_block(a, s);
+                const int pg = pa_table(a, seq, min(blk, a.kv.max_blocks - 1));
+                if (s < len && pg >= 0 && pg < a.kv.n_pages) {
+                    on |= 0xFFFFull << (16 * n);
+                    if (n == TK / 4 * w / 16) { page = pg; row = s - blk * a.kv.page_size; }
+                }
+            }
+            const int mine = TK / 4 * w;
+#pragma unroll
+            for (int n = 0; n < NI; n++) {
+                const int x = RI * n + lrow;
+                const bool in = row >= 0 && s0 + mine + x < len;
+                p.row[n] = in ? page * ps + (row + mine % 16 + x) * rs : -1;
+                if constexpr (E8) p.exp[n] = (page * (long)NKH + j) * a.kv.page_size + row + mine % 16 + x;
+            }
+        } else {
+            const int s = s0 + (lane & (TK - 1)), blk = pa_block(a, s);
+            int pg = -1;
+            if (s < len && blk < a.kv.max_blocks) pg = a.kv.tables[(long)seq * a.kv.table_ld + blk];
+            const bool in = pg >= 0 && pg < a.kv.n_pages;
+            on = __ballot(in);
+            const int row = s - blk * a.kv.page_size;
+            const long at = in ? pg * ps + row * rs : -1, ex = (pg * (long)NKH + j) * a.kv.page_size + row;
+#pragma unroll
+            for (int n = 0; n < NI; n++) {
+                p.row[n] = __shfl(at, TK / 4 * w + RI * n + lrow, 64);
+                if constexpr (E8) p.exp[n] = __shfl(ex, TK / 4 * w + RI * n + lrow, 64);
+            }
+        }
+        return TK == 64 ? on : on & 0xFFFFFFFFull;
+    };
+    uint4 sk[E8 ? NI : 1], sv[E8 ? NI : 1];
+    uint32_t se[2][E8 ? NI : 1];
+    auto fetch = [&](const place &p, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NI; n++) {
+            const int x = TK / 4 * w + RI * n + lrow;        // row in the step
+            const bool in = p.row[n] >= 0;
+            const uint8_t *zero = (const uint8_t *)pa_zeros;
+            if constexpr (E8) {
+                const int col = 16 * lpc < HD ? 16 * lpc : 0;
+                sk[n] = *(const uint4 *)(in ? kb + p.row[n] + col : zero);
+                sv[n] = *(const uint4 *)(in ? vb + p.row[n] + col : zero);
+                se[0][n] = in ? a.kv.k_exp[p.exp[n]] : 127;
+                se[1][n] = in ? a.kv.v_exp[p.exp[n]] : 127;
+            } else {
+                const int ck = 16 * (lpc ^ kx(x)), cv = 16 * (lpc ^ vx(x));
+                const uint8_t *gk = in ? kb + p.row[n] + (ck < 2 * HD ? ck : 0) : zero;
+                const uint8_t *gv = in ? vb + p.row[n] + (cv < 2 * HD ? cv : 0) : zero;
+                const int at = (TK / 4 * w + RI * n) * RB;   // the load's 1 KB
+                __builtin_amdgcn_global_load_lds(gk, (__attribute__((address_space(3))) void *)(kl + at), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds(gv, (__attribute__((address_space(3))) void *)(vl + at), 16, 0, 0);
+            }
+        }
+    };
+    auto store = [&](uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
+        if constexpr (E8) {
+#pragma unroll
+            for (int n = 0; n < NI; n++) {
+                const int x = TK / 4 * w + RI * n + lrow;
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const uint4 u = z ? sv[n] : sk[n];
+                    const float f = pa_exp8(se[z][n]);
+                    uint8_t *row = (z ? vl : kl) + x * RB;
+                    const int y = z ? vx(x) : kx(x);
+                    *(uint4 *)(row + 16 * ((2 * lpc) ^ y)) = make_uint4(pa_cvt8<false>(u.x, f), pa_cvt8<true>(u.x, f), pa_cvt8<false>(u.y, f), pa_cvt8<true>(u.y, f));
+                    *(uint4 *)(row + 16 * ((2 * lpc + 1) ^ y)) = make_uint4(pa_cvt8<false>(u.z, f), pa_cvt8<true>(u.z, f), pa_cvt8<false>(u.w, f), pa_cvt8<true>(u.w, f));
+                }
+            }
+        }
+    };
+
+    float m = kLowest, l = 0.0f;
+    f32x16 o[OB] = {};
+    const int tr = (lane & 15) >> 2;                         // V operand: row of four, 8-byte piece of 32 bytes
+    // K operand: row c (+ 32 n), piece 2 s + hh; V operand: row 4 hh + tr (+ 16 t, + 8), columns 32 x + 16 (lane / 16 % 2) + 4 (lane % 4)
+    const int kbase = c * RB, kxor = kx(c);
+    const int vbase = (4 * hh + tr) * RB + 8 * (lane & 1), vpc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vxor = vx(4 * hh + tr);
+
+    auto work = [&](int s0, uint64_t on, uint8_t *kl, uint8_t *vl, int par) __attribute__((always_inline)) {
+        // of the workgroup: some row is masked somewhere in this step
+        const int top_first = a.window > 0 ? off + last - a.window + 1 : 0;
+        const bool holes = on != (TK == 64 ? ~0ull : 0xFFFFFFFFull);
+        const bool edge = s0 + TK - 1 > off + first || s0 + TK > len || s0 < top_first || holes;
+        uint64_t bad = 0;
+        if (edge) {                                          // the wave looks through its part of V
+            uint32_t mine = 0;
+            constexpr int PCS = RB / 16;                     // pieces per row
+#pragma unroll
+            for (int n = 0; n < TK / 4 * PCS / 64; n++) {
+                const int x = TK / 4 * w + (64 * n + lane) / PCS, y = (64 * n + lane) % PCS;
+                const uint4 u = *(const uint4 *)(vl + x * RB + 16 * y);
+                constexpr uint32_t E = CT == MLLM_F16 ? 0x7C00u : 0x7F80u;
+                auto f = [&](uint32_t q) { return (q & E) == E || (q >> 16 & E) == E; };
+                const uint64_t any = __ballot(f(u.x) || f(u.y) || f(u.z) || f(u.w));
+#pragma unroll
+                for (int z = 0; z < 64 / PCS; z++)
+                    if (any >> (z * PCS) & (PCS == 64 ? ~0ull : (1ull << PCS) - 1)) mine |= 1u << (64 / PCS * n + z);
+            }
+            if (lane == 0) odd[par][w] = mine;
+            __syncthreads();
+#pragma unroll
+            for (int z = 0; z < 4; z++) bad |= (uint64_t)odd[par][z] << (TK / 4 * z);
+            bad = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)bad) | (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
+            if (bad) {
+                __syncthreads();
+                for (int x = 0; x < TK / 4; x++)
+                    if (bad >> (TK / 4 * w + x) & 1)
+                        for (int y = lane; y < RB / 4; y += 64) *(uint32_t *)(vl + (TK / 4 * w + x) * RB + 4 * y) = 0;
+                __syncthreads();
+            }
+        }
+        if (!busy || s0 > pmax || s0 + TK <= lmin) return;   // nothing that the wave's rows see
+        f32x16 s[NB] = {};
+#pragma unroll
+        for (int y = 0; y < KS; y++) {
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const uint4 k = *(const uint4 *)(kl + kbase + 32 * n * RB + 16 * ((2 * y + hh) ^ kxor));
+#pragma unroll
+                for (int x = NP - 1; x >= 0; x--) s[n] = pa_mfma32<CT>(k, qf[x][y], s[n]);
+            }
+        }
+        float top = kLowest;
+        const bool masked = s0 + TK - 1 > pmin || s0 < lmax || s0 + TK > len || holes;
+        if (masked) {
+            const int u = min(pr, len - 1) - s0 - 4 * hh, v = lr - s0 - 4 * hh;
+            const uint64_t bits = on >> (4 * hh);
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int x = 32 * n + 8 * (e >> 2) + (e & 3);
+                    s[n][e] = x <= u && x >= v && (bits >> x & 1) ? s[n][e] * zs : -INFINITY;
+                    top = fmaxf(top, s[n][e]);
+                }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[n][e] *= zs;
+                    top = fmaxf(top, s[n][e]);
+                }
+        }
+        if (__any(top > m + kSlack)) {
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
+            const float f = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int x = 0; x < OB; x++) o[x] *= f;
+        }
+        const float mb = m - kBias<CT>;
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] - mb);
+                l += s[n][e];
+            }
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 *lptr;
+#pragma unroll
+        for (int y = 0; y < TK / 16; y++) {
+            uint32_t p[4][NP];
+#pragma unroll
+            for (int e = 0; e < 4; e++) pa_planes<CT, NP>(s[y >> 1][8 * (y & 1) + 2 * e], s[y >> 1][8 * (y & 1) + 2 * e + 1], p[e]);
+#pragma unroll
+            for (int x = 0; x < OB; x++) {
+                const uint8_t *va = vl + vbase + 16 * y * RB + 16 * ((4 * x + vpc) ^ vxor);
+                const s16x4 f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)va);
+                const s16x4 f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(va + 8 * RB));
+                const uint2 g0 = __builtin_bit_cast(uint2, f0), g1 = __builtin_bit_cast(uint2, f1);
+#pragma unroll
+                for (int n = NP - 1; n >= 0; n--)
+                    o[x] = pa_mfma32<CT>(make_uint4(g0.x, g0.y, g1.x, g1.y), make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]), o[x]);
+            }
+        }
+        while (bad) {                                        // rare: V rows that were cleared
+            const int x = __builtin_ctzll(bad);
+            bad &= bad - 1;
+            const int pos = s0 + x, blk = pa_block(a, pos);
+            const int pg = blk < a.kv.max_blocks ? pa_table(a, seq, blk) : -1;
+            if (pos >= len || pg < 0 || pg >= a.kv.n_pages) continue;
+            float p = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if ((x & ~4) == 32 * n + 8 * (e >> 2) + (e & 3)) p = s[n][e];
+            const float q = __shfl_xor(p, 32, 64);
+            if (hh != (x >> 2 & 1)) p = q;
+            const int row = pos - blk * a.kv.page_size;
+            const uint8_t *vr = vb + pg * ps + row * rs;
+            const float f = E8 ? pa_exp8(a.kv.v_exp[(pg * (long)NKH + j) * a.kv.page_size + row]) : 1.0f;
+            if (pos <= pr && pos >= lr)
+#pragma unroll
+                for (int y = 0; y < OB; y++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int d = 32 * y + 8 * (e >> 2) + 4 * hh + (e & 3);
+                        float z;
+                        if (d >= HD) z = 0.0f;
+                        else if constexpr (E8) z = __builtin_amdgcn_cvt_f32_fp8(vr[d], 0) * f;
+                        else if constexpr (CT == MLLM_BF16) z = (float)((const __bf16 *)vr)[d];
+                        else z = (float)((const _Float16 *)vr)[d];
+                        o[y][e] = fmaf(p, z, o[y][e]);
+                    }
+        }
+    };
+
+    if (begin < end) {
+        place p;
+        uint64_t on0 = find(begin, p), on1 = 0;
+        fetch(p, k0, v0);
+        store(k0, v0);
+        for (int s0 = begin;; s0 += 2 * TK) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): this wave's part is in LDS
+            __syncthreads();
+            bool more = s0 + TK < end;
+            if (more) {
+                on1 = find(s0 + TK, p);
+                fetch(p, k1, v1);
+            }
+            work(s0, on0, k0, v0, 0);
+            if (!more) break;
+            store(k1, v1);
+            __builtin_amdgcn_s_waitcnt(0x0F70);
+            __syncthreads();
+            more = s0 + 2 * TK < end;
+            if (more) {
+                on0 = find(s0 + 2 * TK, p);
+                fetch(p, k0, v0);
+            }
+            work(s0 + TK, on1, k1, v1, 1);
+            if (!more) break;
+            store(k0, v0);
+        }
+    }
+    if (rr >= nrows) return;
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int x = 0; x < OB; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = 32 * x + 8 * e + 4 * hh;
+            if (d >= HD) continue;
+            const float4 y = make_float4(o[x][4 * e], o[x][4 * e + 1], o[x][4 * e + 2], o[x][4 * e + 3]);
+            if (a.splits > 1) *(float4 *)(a.part + (orow * a.splits + sp) * HD + d) = y;
+            else pa_finish(a, h, q0 + tok, d, m, l, y);
+        }
+    if (a.splits > 1 && hh == 0) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(m, l);
+}
+
+template <int CT, bool HP, int HDB> static void pa_prompt_go(const pa_args &a, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(256), 0, st, a);
+}
+template <int CT, bool HP> static void pa_prompt_hd(const pa_args &a, hipStream_t st)
+{
+    const int HD = a.kv.head_dim;
+    HD <= 64 ? pa_prompt_go<CT, HP, 64>(a, st) : HD <= 128 ? pa_prompt_go<CT, HP, 128>(a, st) : pa_prompt_go<CT, HP, 256>(a, st);
+}
+template <int CT> static void pa_prompt(const pa_args &a, bool wide, hipStream_t st)
+{
+    wide ? pa_prompt_hd<CT, true>(a, st) : pa_prompt_hd<CT, false>(a, st);
+}

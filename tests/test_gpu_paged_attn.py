@@ -188,6 +188,52 @@ def test_prompt_unmapped_pages_and_slots(dev, cache, q, head_major):
     prompt(dev, c, [20, 33, 7], 6, q, q, seqs=[3, 1, 3], seed=4)
 
 
+@pytest.mark.parametrize("cache,q", [(BF16, BF16), (E4M3, BF16), (F16, F32)])
+@pytest.mark.parametrize("HD,page,window", [(64, 16, 0), (128, 16, 40), (80, 25, 0), (256, 64, 100)])
+def test_prompt_infinities_and_nan_stay_with_the_queries_that_see_them(dev, cache, q, HD, page, window):
+    """Elements of V that are infinite or NaN, and a row of K that is NaN, at positions in the middle of the prompt:
+    queries before them and, with a window, queries far behind them are as if they were not there."""
+    n, NH, NKH = 200, 6, 2
+    c = Cache(HD, [n], NKH, HD, page, cache)
+    nan, inf = float("nan"), float("inf")
+    marks = [("v", 3, 0, 5, nan), ("v", 90, 1, 0, nan if cache == E4M3 else inf), ("v", 91, 1, 0, nan if cache == E4M3 else -inf),
+             ("v", 150, 0, HD - 1, nan), ("k", 170, 1, 7, nan)]
+    for name, s, h, d, x in marks:
+        (c.k if name == "k" else c.v)[0][s, h, d] = x
+        pool = c.pools[0 if name == "k" else 1]
+        at = int(c.tables[0, s // page]), s % page, h, d
+        if cache == E4M3:
+            pool.view(torch.uint8)[at] = 0x7F
+        else:
+            pool[at] = x
+    query = queries(2, n, NH, HD, q)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    got = dev.paged_attn_prompt(c.view(dev), query.cuda(), i32([0, n]), i32([n]), n, NH, window=window)
+    got = got.double().cpu().view(n, NH, HD)
+    t = torch.arange(n)
+    see = t[None] <= t[:, None]
+    if window:
+        see &= t[None] > t[:, None] - window
+    clean = Cache(HD, [n], NKH, HD, page, cache)
+    for name, s, h, d, _ in marks:
+        (clean.k if name == "k" else clean.v)[0][s, h, d] = 0.0
+    o, mag, za, zq = attend(clean, 0, query.double().view(n, NH, HD), t, HD ** -0.5, window)
+    bound = attend_bound(o, mag, za, zq, n, HD, cache, q, q)
+    wrong = torch.zeros(n, NH, HD, dtype=torch.bool)
+    for name, s, h, d, x in marks:
+        heads = slice(h * NH // NKH, (h + 1) * NH // NKH)
+        if name == "k":
+            wrong[see[:, s], heads] = True
+        else:
+            wrong[:, heads, d] |= see[:, s, None]
+    assert ((got - o).abs() <= bound)[~wrong].all()
+    assert not torch.isfinite(got[wrong]).any()
+    # one query per sequence: the same rows as the last query's
+    last = dev.paged_attn_decode(c.view(dev), query[-1:].cuda(), i32([n]), n, NH, window=window).double().cpu().view(NH, HD)
+    assert torch.equal(torch.isfinite(last), ~wrong[-1])
+    assert ((last - o[-1]).abs() <= bound[-1])[~wrong[-1]].all()
+
+
 def test_prompt_more_queries_than_rows(dev):
     """A length below the number of new tokens: the first queries lie before position 0 and give zeros."""
     c = Cache(6, [40], 2, 64, 16, BF16)
