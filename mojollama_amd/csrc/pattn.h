@@ -17,7 +17,7 @@ struct pa_args {
     unsigned div_mul;              // s / page_size = s * div_mul >> div_sh for 0 <= s < 2^31
     int div_sh;
     int chunk, splits;             // rows per split, splits of a query's range of rows
-    int tiles;                     // tiles of 128 rows at most (prompt)
+    int waves, tiles;              // prompt: waves of 32 rows per tile, tiles at most
     float *part, *stat;            // with splits > 1: sums [T * NH][splits][HD], (maximum, sum) [T * NH][splits]
 };
 

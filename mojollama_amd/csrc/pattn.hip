@@ -67,15 +67,17 @@ __global__ __launch_bounds__(256) void k_pa_join(pa_args a)
 }
 
 constexpr int kMaxSplits = 256, kMinRows = 256;      // rows of a split at least
-constexpr long kTargetWG = 1024;
+// Splits are made until a launch has so many workgroups: then all partial sums together are at most those of
+// kPartRows rows (16 of a workgroup's in decode, 128 in a prompt's) and one of each row.
+constexpr long kPartRows = 65536, kDecodeWG = kPartRows / 16, kPromptWG = kPartRows / 128;
 
 // Rows that a query can see, as far as the host knows.
 long seen(int max_len, int window) { return window > 0 ? std::min<long>(max_len, (long)window + 31) : max_len; }
 
 // Splits of a launch of `wgs` workgroups that each would take all of n rows.
-int pa_splits(long wgs, long n)
+int pa_splits(long wgs, long n, long target)
 {
-    const long want = std::min<long>((kTargetWG + wgs - 1) / wgs, (n + kMinRows - 1) / kMinRows);
+    const long want = std::min<long>((target + wgs - 1) / wgs, (n + kMinRows - 1) / kMinRows);
     return (int)std::max<long>(1, std::min<long>(want, kMaxSplits));
 }
 
@@ -90,7 +92,17 @@ void pa_divisor(pa_args &a)
     a.div_sh = 31 + l;
 }
 
-int pa_launch(const char *who, pa_args &a, void *ws, void *stream)
+// The partial sums' places; false where the workspace does not hold them.
+bool pa_partials(pa_args &a, void *ws, long ws_bytes)
+{
+    if (a.splits == 1) return true;
+    const long n = (long)a.T * a.NH * a.splits, stat = (n * 2 + 3) / 4 * 4;
+    a.stat = (float *)ws;
+    a.part = a.stat + stat;
+    return 4 * (stat + n * a.kv.head_dim) <= ws_bytes;
+}
+
+int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
     pa_divisor(a);
@@ -102,25 +114,26 @@ int pa_launch(const char *who, pa_args &a, void *ws, void *stream)
                              (es == 2 || !(((uintptr_t)a.kv.k_exp | (uintptr_t)a.kv.v_exp) & 3));
         a.groups = (a.rep + 15) / 16;
         const long n = seen(a.max_len, a.window);
-        a.splits = pa_splits((long)a.B * a.kv.n_kv_head * a.groups, n);
+        a.splits = pa_splits((long)a.B * a.kv.n_kv_head * a.groups, n, kDecodeWG);
         a.chunk = (int)std::min<long>(0x7FFFFF80, (n + a.splits - 1) / a.splits / 128 * 128 + 128);
         a.splits = (int)std::max<long>(1, (n + a.chunk - 1) / a.chunk);
-        a.stat = (float *)ws;
-        a.part = a.stat + ((long)a.T * a.NH * a.splits * 2 + 3) / 4 * 4;
+        if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
         if (a.kv.type == MLLM_F16) pa_decode_f16(a, wide, uniform, st);
         else if (a.kv.type == MLLM_BF16) pa_decode_bf16(a, wide, uniform, st);
         else pa_decode_e4m3(a, wide, uniform, st);
-        if (a.splits > 1) hipLaunchKernelGGL(k_pa_join, dim3(a.T, a.NH), dim3(256), 0, st, a);
     } else {
-        a.tiles = (int)((long)a.T * a.rep / 128 + std::min(a.T, a.B));
-        const long n = seen(a.max_len, a.window) + a.T;
-        a.splits = 1;
-        a.chunk = 1 << 30;
+        const long rows = (long)a.T * a.rep, n = a.window > 0 ? std::min<long>(a.window + 320l, a.max_len) : a.max_len;
+        a.waves = !wide && a.kv.head_dim <= 128 && (es == 2 || a.kv.head_dim > 64) && rows / 256 * a.kv.n_kv_head >= 256 ? 8 : 4;
+        a.tiles = (int)(rows / (32 * a.waves) + std::min(a.T, a.B));
+        a.splits = a.waves == 8 ? 1 : pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG);
+        a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + a.splits - 1) / a.splits / 64 * 64 + 64);
+        if (a.splits > 1) a.splits = (int)((n + a.chunk - 1) / a.chunk);
+        if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
         if (a.kv.type == MLLM_F16) pa_prompt_f16(a, wide, st);
         else if (a.kv.type == MLLM_BF16) pa_prompt_bf16(a, wide, st);
         else pa_prompt_e4m3(a, wide, st);
-        (void)n;
     }
+    if (a.splits > 1) hipLaunchKernelGGL(k_pa_join, dim3(a.T, a.NH), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed");
 }
 
@@ -131,11 +144,11 @@ extern "C" {
 MLLM_API long mllm_paged_attn_workspace_size(const mllm_paged_kv *kv, int T, int B, int NH, int max_len, int window)
 {
     if (pk_refusal(kv) || T < 0 || B < 0 || NH <= 0 || NH % kv->n_kv_head || max_len < 0 || window < 0) return -1;
-    // rows (query and head) times splits: each row has at most its range's, all rows together the target
-    // number of workgroups' worth and one each; both grow with every size, so a workspace serves smaller calls
-    const long rows = (long)T * NH, rep = std::min<long>(NH / kv->n_kv_head, 16), n = seen(max_len, window);
+    // rows (query and head) times splits: each row has at most its range's, all rows together kPartRows and
+    // one each; both grow with every size, so a workspace serves smaller calls
+    const long rows = (long)T * NH, n = window > 0 ? std::min<long>(max_len, window + 320l) : max_len;
     const long most = std::max<long>(1, std::min<long>((n + kMinRows - 1) / kMinRows, kMaxSplits));
-    return 4 * (std::min(rows * most, rep * kTargetWG + rows) * (kv->head_dim + 2) + 64);
+    return 4 * (std::min(rows * most, kPartRows + rows) * (kv->head_dim + 2) + 64);
 }
 
 MLLM_API int mllm_paged_attn_decode(const mllm_paged_kv *kv, int q_type, const void *q, long q_ld, const int *seqs,
@@ -151,7 +164,7 @@ MLLM_API int mllm_paged_attn_decode(const mllm_paged_kv *kv, int q_type, const v
         return pk_fail(who, "workspace below mllm_paged_attn_workspace_size");
     if (!B) return 0;
     pa_args a{q, out, q_ld, out_ld, q_type, out_type, *kv, seqs, nullptr, lens, max_len, B, B, NH, window, scale, sinks};
-    return pa_launch(who, a, workspace, stream);
+    return pa_launch(who, a, workspace, ws_bytes, stream);
 }
 
 MLLM_API int mllm_paged_attn_prompt(const mllm_paged_kv *kv, int q_type, const void *q, long q_ld, const int *seqs,
@@ -168,7 +181,7 @@ MLLM_API int mllm_paged_attn_prompt(const mllm_paged_kv *kv, int q_type, const v
         return pk_fail(who, "workspace below mllm_paged_attn_workspace_size");
     if (!T || !B) return 0;
     pa_args a{q, out, q_ld, out_ld, q_type, out_type, *kv, seqs, starts, lens, max_len, T, B, NH, window, scale, sinks};
-    return pa_launch(who, a, workspace, stream);
+    return pa_launch(who, a, workspace, ws_bytes, stream);
 }
 
 } // extern "C"

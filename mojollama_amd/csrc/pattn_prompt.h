@@ -32,26 +32,28 @@ static __device__ const uint4 pa_zeros[1] = {};
 // some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
 // element by element to the queries that do see them.  Rows that no query of the sequence sees (past
 // the length, on unmapped pages) are read as zeros.
-template <int CT, bool HP, int HDB>
-__global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa_prompt(pa_args a)
+template <int CT, bool HP, int HDB, int NW>
+__global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1 : 2) void k_pa_prompt(pa_args a)
 {
     constexpr bool E8 = CT == MLLM_E4M3;
     constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1;
+    constexpr int ROWS = 32 * NW;
     constexpr int TK = HDB > 128 ? 32 : 64, NB = TK / 32;    // rows per step, in blocks of 32
     constexpr int KS = HDB / 16, OB = HDB / 32;
     constexpr int RB = HDB * 2;                              // bytes of a row in LDS
-    constexpr int LPR = HDB * ES / 16, RI = 64 / LPR, NI = TK / (4 * RI);   // lanes per row, rows per load, loads per wave
+    constexpr int LPR = HDB * ES / 16, RI = 64 / LPR, WR = TK / NW, NI = WR / RI;   // lanes per row, rows per load, rows and loads per wave
     __shared__ __attribute__((aligned(1024))) uint8_t k0[TK * RB], v0[TK * RB], k1[TK * RB], v1[TK * RB];
-    __shared__ uint32_t odd[2][4];                           // rows of V that hold infinities or NaN, per wave's part
+    __shared__ uint32_t odd[2][NW], there[2][NW];            // of a wave's rows: V holds an infinity or NaN; on a mapped page
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hh = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int NKH = a.kv.n_kv_head, j = blockIdx.x % NKH, HD = a.kv.head_dim, sp = blockIdx.y, rep = a.rep;
 
+    auto start = [&](int x) { return max(0, min(a.starts[x], a.T)); };
     // which sequence and tile: 64 sequences at a time
     int t = blockIdx.x / NKH, b = -1, tiles = 0;
     for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
         const int bb = b0 + lane;
-        const int n = bb < a.B ? (int)(((long)max(0, a.starts[bb + 1] - a.starts[bb]) * rep + 127) / 128) : 0;
+        const int n = bb < a.B ? (int)(((long)max(0, start(bb + 1) - start(bb)) * rep + ROWS - 1) / ROWS) : 0;
         int sum = n;
         for (int d = 1; d < 64; d <<= 1) {
             const int y = __shfl_up(sum, d, 64);
@@ -70,23 +72,23 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
     if (b < 0) return;
     b = __builtin_amdgcn_readfirstlane(b);
     const int tile = __builtin_amdgcn_readfirstlane(tiles - 1 - t);     // the last rows, which see most, first
-    const int q0 = a.starts[b], nq = a.starts[b + 1] - q0;
+    const int q0 = start(b), nq = start(b + 1) - q0;
     const int seq = a.seqs ? a.seqs[b] : b;
     const int len0 = min(a.lens[b], a.max_len);
     int len = seq >= 0 && seq < a.kv.n_seqs ? len0 : 0;
     len = min(len, (int)min((long)a.kv.max_blocks * a.kv.page_size, 0x7FFFFFFFl));
-    const int nrows = (int)min(128l, (long)nq * rep - tile * 128l);      // of the tile
-    const int first = (int)((long)tile * 128 / rep), last = (int)(((long)tile * 128 + nrows - 1) / rep);   // tokens
+    const int nrows = (int)min((long)ROWS, (long)nq * rep - (long)tile * ROWS);      // of the tile
+    const int first = (int)((long)tile * ROWS / rep), last = (int)(((long)tile * ROWS + nrows - 1) / rep);   // tokens
     // positions of a token's query: len0 - nq + token; it sees (p - window, p]
     const int off = len0 - nq;
     const int lo = a.window > 0 ? max(0, off + first - a.window + 1) : 0, hi = min(len, off + last + 1);
     const int begin = lo / TK * TK + sp * a.chunk, end = min(hi, begin + a.chunk);
     // this lane's row
-    const int rr = 32 * w + c, r = min(rr, nrows - 1), tok = (int)((tile * 128l + r) / rep), h = j * rep + (int)((tile * 128l + r) - (long)tok * rep);
+    const int rr = 32 * w + c, r = min(rr, nrows - 1), tok = (int)(((long)tile * ROWS + r) / rep), h = j * rep + (int)(((long)tile * ROWS + r) - (long)tok * rep);
     const int pr = off + tok, lr = a.window > 0 ? max(0, pr - a.window + 1) : 0;
     const bool busy = 32 * w < nrows;                        // the wave has rows
     // of the wave's rows: the least last position and the largest first one
-    const int wtok0 = (int)((tile * 128l + min(32 * w, nrows - 1)) / rep), wtok1 = (int)((tile * 128l + min(32 * w + 31, nrows - 1)) / rep);
+    const int wtok0 = (int)(((long)tile * ROWS + min(32 * w, nrows - 1)) / rep), wtok1 = (int)(((long)tile * ROWS + min(32 * w + 31, nrows - 1)) / rep);
     const int pmin = off + wtok0, pmax = off + wtok1, lmax = a.window > 0 ? max(0, pmax - a.window + 1) : 0;
     const int lmin = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
     const long orow = (long)(q0 + tok) * a.NH + h;
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
     }
 
     uint4 qf[NP][KS];
-    float zs = a.scale * kLog2e;
+    float zs = fabsf(a.scale) * kLog2e;                      // its sign goes into q: the largest product is the largest score
     {
         const long at = (long)(q0 + tok) * a.q_ld + (long)h * HD;
         int e = 0;
@@ -125,6 +127,7 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
             for (int i = 0; i < 4; i++) {
                 float u = col < HD ? x[2 * i] : 0.0f, v = col < HD ? x[2 * i + 1] : 0.0f;
                 if constexpr (HP && CT == MLLM_F16) { u = ldexpf(u, e); v = ldexpf(v, e); }
+                if (a.scale < 0.0f) { u = -u; v = -v; }
                 pa_planes<CT, NP>(u, v, p[i]);
 #pragma unroll
                 for (int n = 1; n < NP; n++) {               // an infinity's rest is 0
@@ -144,52 +147,45 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
     const uint8_t *kb = (const uint8_t *)a.kv.k + hs, *vb = (const uint8_t *)a.kv.v + hs;
     const int lrow = lane / LPR, lpc = lane & (LPR - 1);     // row of a load and piece
     const bool even = a.kv.page_size % 16 == 0;
-    // Row TK/4 * w + RI * n + lrow of the step at s0: where it is, -1 if it holds nothing; returns which of
-    // the step's rows are on mapped pages, one bit each.
+    // Row WR * w + RI * n + lrow of the step at s0: where it is, -1 if it holds nothing.  Each wave looks up
+    // its own rows and leaves word of which are on mapped pages.
     struct place { long row[NI], exp[NI]; };
-    auto find = [&](int s0, place &p) __attribute__((always_inline)) {
-        uint64_t on = 0;
-        if (even) {                                          // 16 rows lie in one page, so do the wave's
-            int page = 0, row = -1;
-#pragma unroll
-            for (int n = 0; n < TK / 16; n++) {
-                const int s = s0 + 16 * n, blk = pa_block(a, s);
-                const int pg = pa_table(a, seq, min(blk, a.kv.max_blocks - 1));
-                if (s < len && pg >= 0 && pg < a.kv.n_pages) {
-                    on |= 0xFFFFull << (16 * n);
-                    if (n == TK / 4 * w / 16) { page = pg; row = s - blk * a.kv.page_size; }
-                }
-            }
-            const int mine = TK / 4 * w;
+    auto find = [&](int s0, place &p, int par) __attribute__((always_inline)) {
+        uint32_t on;
+        if (even) {                                          // the wave's rows lie in one page
+            const int s = s0 + WR * w, blk = pa_block(a, s);
+            const int pg = pa_table(a, seq, min(blk, a.kv.max_blocks - 1));
+            const bool in = s < len && pg >= 0 && pg < a.kv.n_pages;
+            const long row = s - blk * a.kv.page_size, at = pg * ps + row * rs;
+            on = in ? (1u << WR) - 1 : 0;
 #pragma unroll
             for (int n = 0; n < NI; n++) {
                 const int x = RI * n + lrow;
-                const bool in = row >= 0 && s0 + mine + x < len;
-                p.row[n] = in ? page * ps + (row + mine % 16 + x) * rs : -1;
-                if constexpr (E8) p.exp[n] = (page * (long)NKH + j) * a.kv.page_size + row + mine % 16 + x;
+                p.row[n] = in && s + x < len ? at + x * rs : -1;
+                if constexpr (E8) p.exp[n] = (pg * (long)NKH + j) * a.kv.page_size + row + x;
             }
         } else {
-            const int s = s0 + (lane & (TK - 1)), blk = pa_block(a, s);
+            const int s = s0 + WR * w + (lane & (WR - 1)), blk = pa_block(a, s);
             int pg = -1;
             if (s < len && blk < a.kv.max_blocks) pg = a.kv.tables[(long)seq * a.kv.table_ld + blk];
             const bool in = pg >= 0 && pg < a.kv.n_pages;
-            on = __ballot(in);
+            on = (uint32_t)__ballot(in || s >= len) & ((1u << WR) - 1);
             const int row = s - blk * a.kv.page_size;
             const long at = in ? pg * ps + row * rs : -1, ex = (pg * (long)NKH + j) * a.kv.page_size + row;
 #pragma unroll
             for (int n = 0; n < NI; n++) {
-                p.row[n] = __shfl(at, TK / 4 * w + RI * n + lrow, 64);
-                if constexpr (E8) p.exp[n] = __shfl(ex, TK / 4 * w + RI * n + lrow, 64);
+                p.row[n] = __shfl(at, RI * n + lrow, 64);
+                if constexpr (E8) p.exp[n] = __shfl(ex, RI * n + lrow, 64);
             }
         }
-        return TK == 64 ? on : on & 0xFFFFFFFFull;
+        if (lane == 0) there[par][w] = on;
     };
     uint4 sk[E8 ? NI : 1], sv[E8 ? NI : 1];
     uint32_t se[2][E8 ? NI : 1];
     auto fetch = [&](const place &p, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < NI; n++) {
-            const int x = TK / 4 * w + RI * n + lrow;        // row in the step
+            const int x = WR * w + RI * n + lrow;        // row in the step
             const bool in = p.row[n] >= 0;
             const uint8_t *zero = (const uint8_t *)pa_zeros;
             if constexpr (E8) {
@@ -202,7 +198,7 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
                 const int ck = 16 * (lpc ^ kx(x)), cv = 16 * (lpc ^ vx(x));
                 const uint8_t *gk = in ? kb + p.row[n] + (ck < 2 * HD ? ck : 0) : zero;
                 const uint8_t *gv = in ? vb + p.row[n] + (cv < 2 * HD ? cv : 0) : zero;
-                const int at = (TK / 4 * w + RI * n) * RB;   // the load's 1 KB
+                const int at = (WR * w + RI * n) * RB;   // the load's 1 KB
                 __builtin_amdgcn_global_load_lds(gk, (__attribute__((address_space(3))) void *)(kl + at), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds(gv, (__attribute__((address_space(3))) void *)(vl + at), 16, 0, 0);
             }
@@ -212,7 +208,7 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
         if constexpr (E8) {
 #pragma unroll
             for (int n = 0; n < NI; n++) {
-                const int x = TK / 4 * w + RI * n + lrow;
+                const int x = WR * w + RI * n + lrow;
 #pragma unroll
                 for (int z = 0; z < 2; z++) {
                     const uint4 u = z ? sv[n] : sk[n];
@@ -226,25 +222,28 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
         }
     };
 
-    float m = kLowest, l = 0.0f;
+    float m = kLowest, l0 = 0.0f, l1 = 0.0f;               // the sum in two parts: shorter chains
     f32x16 o[OB] = {};
     const int tr = (lane & 15) >> 2;                         // V operand: row of four, 8-byte piece of 32 bytes
     // K operand: row c (+ 32 n), piece 2 s + hh; V operand: row 4 hh + tr (+ 16 t, + 8), columns 32 x + 16 (lane / 16 % 2) + 4 (lane % 4)
     const int kbase = c * RB, kxor = kx(c);
     const int vbase = (4 * hh + tr) * RB + 8 * (lane & 1), vpc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vxor = vx(4 * hh + tr);
 
-    auto work = [&](int s0, uint64_t on, uint8_t *kl, uint8_t *vl, int par) __attribute__((always_inline)) {
+    auto work = [&](int s0, uint8_t *kl, uint8_t *vl, int par) __attribute__((always_inline)) {
         // of the workgroup: some row is masked somewhere in this step
         const int top_first = a.window > 0 ? off + last - a.window + 1 : 0;
-        const bool holes = on != (TK == 64 ? ~0ull : 0xFFFFFFFFull);
+        uint32_t every = ~0u;
+#pragma unroll
+        for (int z = 0; z < NW; z++) every &= there[par][z];
+        const bool holes = __builtin_amdgcn_readfirstlane(every) != (1u << WR) - 1;
         const bool edge = s0 + TK - 1 > off + first || s0 + TK > len || s0 < top_first || holes;
         uint64_t bad = 0;
         if (edge) {                                          // the wave looks through its part of V
             uint32_t mine = 0;
             constexpr int PCS = RB / 16;                     // pieces per row
 #pragma unroll
-            for (int n = 0; n < TK / 4 * PCS / 64; n++) {
-                const int x = TK / 4 * w + (64 * n + lane) / PCS, y = (64 * n + lane) % PCS;
+            for (int n = 0; n < WR * PCS / 64; n++) {
+                const int x = WR * w + (64 * n + lane) / PCS, y = (64 * n + lane) % PCS;
                 const uint4 u = *(const uint4 *)(vl + x * RB + 16 * y);
                 constexpr uint32_t E = CT == MLLM_F16 ? 0x7C00u : 0x7F80u;
                 auto f = [&](uint32_t q) { return (q & E) == E || (q >> 16 & E) == E; };
@@ -256,82 +255,115 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
             if (lane == 0) odd[par][w] = mine;
             __syncthreads();
 #pragma unroll
-            for (int z = 0; z < 4; z++) bad |= (uint64_t)odd[par][z] << (TK / 4 * z);
+            for (int z = 0; z < NW; z++) bad |= (uint64_t)odd[par][z] << (WR * z);
             bad = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)bad) | (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
             if (bad) {
                 __syncthreads();
-                for (int x = 0; x < TK / 4; x++)
-                    if (bad >> (TK / 4 * w + x) & 1)
-                        for (int y = lane; y < RB / 4; y += 64) *(uint32_t *)(vl + (TK / 4 * w + x) * RB + 4 * y) = 0;
+                for (int x = 0; x < WR; x++)
+                    if (bad >> (WR * w + x) & 1)
+                        for (int y = lane; y < RB / 4; y += 64) *(uint32_t *)(vl + (WR * w + x) * RB + 4 * y) = 0;
                 __syncthreads();
             }
         }
         if (!busy || s0 > pmax || s0 + TK <= lmin) return;   // nothing that the wave's rows see
+        // Operands are read from LDS ahead of the products that take them: K's two products' worth (KD), V's
+        // a group of OB; the scheduler is held to that order, or it reads each right before its use.
+        constexpr int KD = KS < 2 ? 1 : 2;
         f32x16 s[NB] = {};
+        uint4 kf[KD + 1][NB];
+        auto read_k = [&](int y) __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+                kf[y % (KD + 1)][n] = *(const uint4 *)(kl + kbase + 32 * n * RB + 16 * ((2 * y + hh) ^ kxor));
+        };
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 *lptr;
+        uint2 vf[2][OB][2];
+        auto read_v = [&](int y) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 0; x < OB; x++) {
+                const uint8_t *va = vl + vbase + 16 * y * RB + 16 * ((4 * x + vpc) ^ vxor);
+                vf[y & 1][x][0] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)va));
+                vf[y & 1][x][1] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(va + 8 * RB)));
+            }
+        };
+#pragma unroll
+        for (int y = 0; y < KD; y++) read_k(y);
 #pragma unroll
         for (int y = 0; y < KS; y++) {
+            if (y + KD < KS) read_k(y + KD);
+            else if (y + KD == KS) read_v(0);
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                const uint4 k = *(const uint4 *)(kl + kbase + 32 * n * RB + 16 * ((2 * y + hh) ^ kxor));
+            for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int x = NP - 1; x >= 0; x--) s[n] = pa_mfma32<CT>(k, qf[x][y], s[n]);
-            }
+                for (int x = NP - 1; x >= 0; x--) s[n] = pa_mfma32<CT>(kf[y % (KD + 1)][n], qf[x][y], s[n]);
         }
-        float top = kLowest;
-        const bool masked = s0 + TK - 1 > pmin || s0 < lmax || s0 + TK > len || holes;
-        if (masked) {
+        __builtin_amdgcn_sched_group_barrier(0x100, KD * NB, 0);
+#pragma unroll
+        for (int y = 0; y < KS; y++) {
+            if (y + KD < KS) __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
+            if (y + KD == KS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * OB, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, NB * NP, 0);
+        }
+        float top = -INFINITY;
+        if (s0 + TK - 1 > pmin || s0 < lmax || s0 + TK > len || holes) {
+            asm volatile("");                                // a branch: the selects are for the few edges
             const int u = min(pr, len - 1) - s0 - 4 * hh, v = lr - s0 - 4 * hh;
-            const uint64_t bits = on >> (4 * hh);
+            uint64_t bits = 0;
+#pragma unroll
+            for (int z = 0; z < NW; z++) bits |= (uint64_t)there[par][z] << (WR * z);
+            bits >>= 4 * hh;
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int x = 32 * n + 8 * (e >> 2) + (e & 3);
-                    s[n][e] = x <= u && x >= v && (bits >> x & 1) ? s[n][e] * zs : -INFINITY;
-                    top = fmaxf(top, s[n][e]);
-                }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NB; n++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[n][e] *= zs;
-                    top = fmaxf(top, s[n][e]);
+                    if (!(x <= u && x >= v && (bits >> x & 1))) s[n][e] = -INFINITY;
                 }
         }
-        if (__any(top > m + kSlack)) {
-            top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
-            const float f = __builtin_amdgcn_exp2f(m - top);
-            m = top;
-            l *= f;
-#pragma unroll
-            for (int x = 0; x < OB; x++) o[x] *= f;
-        }
-        const float mb = m - kBias<CT>;
 #pragma unroll
         for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                s[n][e] = __builtin_amdgcn_exp2f(s[n][e] - mb);
-                l += s[n][e];
-            }
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s16x4 *lptr;
+            for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(top, s[n][e]), s[n][e + 1]);
+        top = fmaxf(top * zs, kLowest);
+        if (__any(top > m + kSlack)) {
+            asm volatile("");
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
+            const float f = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l0 *= f;
+            l1 *= f;
+#pragma unroll
+            for (int x = 0; x < OB; x++) o[x] *= f;
+        }
+        const float mb = kBias<CT> - m;
 #pragma unroll
         for (int y = 0; y < TK / 16; y++) {
             uint32_t p[4][NP];
 #pragma unroll
-            for (int e = 0; e < 4; e++) pa_planes<CT, NP>(s[y >> 1][8 * (y & 1) + 2 * e], s[y >> 1][8 * (y & 1) + 2 * e + 1], p[e]);
+            for (int e = 0; e < 4; e++) {
+                const int at = 8 * (y & 1) + 2 * e;
+                const float u = __builtin_amdgcn_exp2f(fmaf(s[y >> 1][at], zs, mb));
+                const float v = __builtin_amdgcn_exp2f(fmaf(s[y >> 1][at + 1], zs, mb));
+                s[y >> 1][at] = u;
+                s[y >> 1][at + 1] = v;
+                pa_planes<CT, NP>(u, v, p[e]);
+                float &l = e & 1 ? l1 : l0;
+                l += u + v;
+            }
+            if (y + 1 < TK / 16) read_v(y + 1);
 #pragma unroll
             for (int x = 0; x < OB; x++) {
-                const uint8_t *va = vl + vbase + 16 * y * RB + 16 * ((4 * x + vpc) ^ vxor);
-                const s16x4 f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)va);
-                const s16x4 f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(va + 8 * RB));
-                const uint2 g0 = __builtin_bit_cast(uint2, f0), g1 = __builtin_bit_cast(uint2, f1);
+                const uint2 f0 = vf[y & 1][x][0], f1 = vf[y & 1][x][1];
 #pragma unroll
                 for (int n = NP - 1; n >= 0; n--)
-                    o[x] = pa_mfma32<CT>(make_uint4(g0.x, g0.y, g1.x, g1.y), make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]), o[x]);
+                    o[x] = pa_mfma32<CT>(make_uint4(f0.x, f0.y, f1.x, f1.y), make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]), o[x]);
             }
+        }
+#pragma unroll
+        for (int y = 0; y < TK / 16; y++) {
+            if (y + 1 < TK / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2 * OB, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, OB * NP, 0);
         }
         while (bad) {                                        // rare: V rows that were cleared
             const int x = __builtin_ctzll(bad);
@@ -368,7 +400,7 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
 
     if (begin < end) {
         place p;
-        uint64_t on0 = find(begin, p), on1 = 0;
+        find(begin, p, 0);
         fetch(p, k0, v0);
         store(k0, v0);
         for (int s0 = begin;; s0 += 2 * TK) {
@@ -376,25 +408,26 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
             __syncthreads();
             bool more = s0 + TK < end;
             if (more) {
-                on1 = find(s0 + TK, p);
+                find(s0 + TK, p, 1);
                 fetch(p, k1, v1);
             }
-            work(s0, on0, k0, v0, 0);
+            work(s0, k0, v0, 0);
             if (!more) break;
             store(k1, v1);
             __builtin_amdgcn_s_waitcnt(0x0F70);
             __syncthreads();
             more = s0 + 2 * TK < end;
             if (more) {
-                on0 = find(s0 + 2 * TK, p);
+                find(s0 + 2 * TK, p, 0);
                 fetch(p, k0, v0);
             }
-            work(s0 + TK, on1, k1, v1, 1);
+            work(s0 + TK, k1, v1, 1);
             if (!more) break;
             store(k0, v0);
         }
     }
     if (rr >= nrows) return;
+    float l = l0 + l1;
     l += __shfl_xor(l, 32, 64);
 #pragma unroll
     for (int x = 0; x < OB; x++)
@@ -409,16 +442,17 @@ __global__ __launch_bounds__(256, HP && HDB > 64 || HDB > 128 ? 1 : 2) void k_pa
     if (a.splits > 1 && hh == 0) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(m, l);
 }
 
-template <int CT, bool HP, int HDB> static void pa_prompt_go(const pa_args &a, hipStream_t st)
+template <int CT, bool HP, int HDB, int NW> static void pa_prompt_go(const pa_args &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(256), 0, st, a);
-}
-template <int CT, bool HP> static void pa_prompt_hd(const pa_args &a, hipStream_t st)
-{
-    const int HD = a.kv.head_dim;
-    HD <= 64 ? pa_prompt_go<CT, HP, 64>(a, st) : HD <= 128 ? pa_prompt_go<CT, HP, 128>(a, st) : pa_prompt_go<CT, HP, 256>(a, st);
+    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB, NW>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(64 * NW), 0, st, a);
 }
 template <int CT> static void pa_prompt(const pa_args &a, bool wide, hipStream_t st)
 {
-    wide ? pa_prompt_hd<CT, true>(a, st) : pa_prompt_hd<CT, false>(a, st);
+    const int HD = a.kv.head_dim;
+    if (wide)
+        HD <= 64 ? pa_prompt_go<CT, true, 64, 4>(a, st) : HD <= 128 ? pa_prompt_go<CT, true, 128, 4>(a, st) : pa_prompt_go<CT, true, 256, 4>(a, st);
+    else if (a.waves == 8)
+        HD <= 64 ? pa_prompt_go<CT, false, 64, CT == MLLM_E4M3 ? 4 : 8>(a, st) : pa_prompt_go<CT, false, 128, 8>(a, st);
+    else
+        HD <= 64 ? pa_prompt_go<CT, false, 64, 4>(a, st) : HD <= 128 ? pa_prompt_go<CT, false, 128, 4>(a, st) : pa_prompt_go<CT, false, 256, 4>(a, st);
 }
