@@ -101,6 +101,6 @@ __device__ __forceinline__ void pa_finish(const pa_args &a, int h, int t, int d,
 void pa_decode_bf16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_f16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_e4m3(const pa_args &a, bool wide, bool uniform, hipStream_t st);
-void pa_prompt_bf16(const pa_args &a, bool wide, hipStream_t st);
-void pa_prompt_f16(const pa_args &a, bool wide, hipStream_t st);
-void pa_prompt_e4m3(const pa_args &a, bool wide, hipStream_t st);
+void pa_prompt_bf16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
+void pa_prompt_f16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
+void pa_prompt_e4m3(const pa_args &a, bool wide, bool uniform, hipStream_t st);

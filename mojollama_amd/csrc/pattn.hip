@@ -23,9 +23,9 @@ const char *pa_refusal(const mllm_paged_kv *kv, int q_type, const void *q, long 
     return nullptr;
 }
 
-// The splits of a query's rows joined: their sums under one maximum.  One row (query and head) per
-// workgroup; HD / 4 threads cover a split's sums, the groups of so many threads take every
-// (256 / (HD / 4))-th split.
+// The splits of a query's rows joined: their sums under one maximum.  One row (query and head) and up
+// to 64 columns per workgroup: 16 threads cover the columns, the 16 groups of so many take every 16th
+// split, four loads in flight each.
 __global__ __launch_bounds__(256) void k_pa_join(pa_args a)
 {
     __shared__ float wt[256], red[2][4];
@@ -33,35 +33,45 @@ __global__ __launch_bounds__(256) void k_pa_join(pa_args a)
     const int h = blockIdx.y, t = blockIdx.x, tid = threadIdx.x, HD = a.kv.head_dim;
     if (a.starts && (t < a.starts[0] || t >= a.starts[a.B])) return;
     const long row = (long)t * a.NH + h;
+    const int gi = tid >> 4, d = 64 * blockIdx.z + 4 * (tid & 15), dc = min(d, HD - 4);
+    const float *part = a.part + row * a.splits * HD + dc;
     float2 ml = make_float2(kLowest, 0.0f);
     if (tid < a.splits) ml = *(const float2 *)(a.stat + (row * a.splits + tid) * 2);
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) x[u] = *(const float4 *)(part + (long)min(gi + 16 * u, a.splits - 1) * HD);
     float m = ml.x;
-    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
     if (!(tid & 63)) red[0][tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     const float f = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
     wt[tid] = f;
     float l = f * ml.y;
-    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d, 64);
+    for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k, 64);
     if (!(tid & 63)) red[1][tid >> 6] = l;
     __syncthreads();
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const int n = HD / 4, ng = 256 / n, gi = tid / n, d = 4 * (tid - gi * n);
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (gi < ng)
-        for (int s = gi; s < a.splits; s += ng) {
-            const float u = wt[s];
-            if (u == 0.0f) continue;                 // an empty split's sums are not written
-            const float4 x = *(const float4 *)(a.part + (row * a.splits + s) * HD + d);
-            y.x = fmaf(u, x.x, y.x); y.y = fmaf(u, x.y, y.y); y.z = fmaf(u, x.z, y.z); y.w = fmaf(u, x.w, y.w);
+    for (int s = gi; s < a.splits; s += 64) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float c = s + 16 * u < a.splits ? wt[s + 16 * u] : 0.0f;
+            if (c != 0.0f) {                         // an empty split's sums are not written (NaN's are: c is NaN)
+                y.x = fmaf(c, x[u].x, y.x); y.y = fmaf(c, x[u].y, y.y); y.z = fmaf(c, x[u].z, y.z); y.w = fmaf(c, x[u].w, y.w);
+            }
         }
+        if (s + 64 < a.splits)
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = *(const float4 *)(part + (long)min(s + 64 + 16 * u, a.splits - 1) * HD);
+    }
     *(float4 *)(acc + 4 * tid) = y;
     __syncthreads();
-    if (gi) return;
-    for (int s = 1; s < ng; s++) {
-        const float4 x = *(const float4 *)(acc + 4 * (tid + s * n));
-        y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+    if (gi || d >= HD) return;
+#pragma unroll
+    for (int s = 1; s < 16; s++) {
+        const float4 z = *(const float4 *)(acc + 4 * (tid + 16 * s));
+        y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
     }
     pa_finish(a, h, t, d, m, l, y);
 }
@@ -109,9 +119,10 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
     a.rep = a.NH / a.kv.n_kv_head;
     const bool wide = a.q_type == MLLM_F32 || a.out_type == MLLM_F32;
     const int es = pk_size(a.kv.type);
+    // pages of a multiple of 16 rows: a tile's rows lie in one page (and four exponents in a word)
+    const bool uniform = a.kv.page_size % 16 == 0 && a.kv.row_stride * 16 * es < 0x7FFFFFFF &&
+                         (es == 2 || !(((uintptr_t)a.kv.k_exp | (uintptr_t)a.kv.v_exp) & 3));
     if (!a.starts) {
-        const bool uniform = a.kv.page_size % 16 == 0 && a.kv.row_stride * 16 * es < 0x7FFFFFFF &&
-                             (es == 2 || !(((uintptr_t)a.kv.k_exp | (uintptr_t)a.kv.v_exp) & 3));
         a.groups = (a.rep + 15) / 16;
         const long n = seen(a.max_len, a.window);
         a.splits = pa_splits((long)a.B * a.kv.n_kv_head * a.groups, n, kDecodeWG);
@@ -123,17 +134,22 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         else pa_decode_e4m3(a, wide, uniform, st);
     } else {
         const long rows = (long)a.T * a.rep, n = a.window > 0 ? std::min<long>(a.window + 320l, a.max_len) : a.max_len;
-        a.waves = !wide && a.kv.head_dim <= 128 && (es == 2 || a.kv.head_dim > 64) && rows / 256 * a.kv.n_kv_head >= 256 ? 8 : 4;
+        a.waves = uniform && a.kv.page_size % 64 == 0 && !wide && a.kv.head_dim <= 128 && (es == 2 || a.kv.head_dim > 64) && rows / 256 * a.kv.n_kv_head >= 256 ? 8 : 4;
         a.tiles = (int)(rows / (32 * a.waves) + std::min(a.T, a.B));
-        a.splits = a.waves == 8 ? 1 : pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG);
+        // no more than keep the partial sums, written and read again, below the rows of K and V that they save
+        // time on: prompts of 1 to 1100 tokens over up to 2600 rows, window 512, 16/4 heads of 96, in three
+        // splits / whole 52.7 / 32.2 us; 3 to 5 tokens over 1500 to 4000 rows, 64/8 heads of 64, seven / whole
+        // 29 / 123 us
+        const long most = n * a.B * a.kv.n_kv_head * es / (4l * a.T * a.NH);
+        a.splits = a.waves == 8 ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG)));
         a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + a.splits - 1) / a.splits / 64 * 64 + 64);
         if (a.splits > 1) a.splits = (int)((n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
-        if (a.kv.type == MLLM_F16) pa_prompt_f16(a, wide, st);
-        else if (a.kv.type == MLLM_BF16) pa_prompt_bf16(a, wide, st);
-        else pa_prompt_e4m3(a, wide, st);
+        if (a.kv.type == MLLM_F16) pa_prompt_f16(a, wide, uniform, st);
+        else if (a.kv.type == MLLM_BF16) pa_prompt_bf16(a, wide, uniform, st);
+        else pa_prompt_e4m3(a, wide, uniform, st);
     }
-    if (a.splits > 1) hipLaunchKernelGGL(k_pa_join, dim3(a.T, a.NH), dim3(256), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL(k_pa_join, dim3(a.T, a.NH, (a.kv.head_dim + 63) / 64), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed");
 }
 

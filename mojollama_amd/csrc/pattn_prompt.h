@@ -1,5 +1,8 @@
 // pattn_prompt.h — the tiled prompt kernel over a paged cache, instantiated per cache type.
 #pragma once
+#ifndef PA_NBUF
+#define PA_NBUF 2
+#endif
 #include <math.h>
 #include <type_traits>
 #include "pattn.h"
@@ -11,9 +14,6 @@ template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, 
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
 }
-
-// Rows that hold nothing are read from here.
-static __device__ const uint4 pa_zeros[1] = {};
 
 // 128 rows of queries against the rows of one kv head, 64 of these at a time (32 at head sizes
 // above 128).  A row is a (token, head) pair of the heads that share the kv head, tokens outer, so a
@@ -32,7 +32,7 @@ static __device__ const uint4 pa_zeros[1] = {};
 // some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
 // element by element to the queries that do see them.  Rows that no query of the sequence sees (past
 // the length, on unmapped pages) are read as zeros.
-template <int CT, bool HP, int HDB, int NW>
+template <int CT, bool HP, int HDB, int NW, int EV>
 __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1 : 2) void k_pa_prompt(pa_args a)
 {
     constexpr bool E8 = CT == MLLM_E4M3;
@@ -42,8 +42,11 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     constexpr int KS = HDB / 16, OB = HDB / 32;
     constexpr int RB = HDB * 2;                              // bytes of a row in LDS
     constexpr int LPR = HDB * ES / 16, RI = 64 / LPR, WR = TK / NW, NI = WR / RI;   // lanes per row, rows per load, rows and loads per wave
+    constexpr int NBUF = E8 ? 2 : PA_NBUF;                   // buffers: steps in flight and the one at work
     __shared__ __attribute__((aligned(1024))) uint8_t k0[TK * RB], v0[TK * RB], k1[TK * RB], v1[TK * RB];
-    __shared__ uint32_t odd[2][NW], there[2][NW];            // of a wave's rows: V holds an infinity or NaN; on a mapped page
+    __shared__ __attribute__((aligned(1024))) uint8_t k2[NBUF > 2 ? TK * RB : 16], v2[NBUF > 2 ? TK * RB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t k3[NBUF > 3 ? TK * RB : 16], v3[NBUF > 3 ? TK * RB : 16];
+    __shared__ uint32_t odd[2][NW];                          // of a wave's rows of V: those that hold an infinity or a NaN
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hh = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int NKH = a.kv.n_kv_head, j = blockIdx.x % NKH, HD = a.kv.head_dim, sp = blockIdx.y, rep = a.rep;
@@ -86,11 +89,12 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     // this lane's row
     const int rr = 32 * w + c, r = min(rr, nrows - 1), tok = (int)(((long)tile * ROWS + r) / rep), h = j * rep + (int)(((long)tile * ROWS + r) - (long)tok * rep);
     const int pr = off + tok, lr = a.window > 0 ? max(0, pr - a.window + 1) : 0;
-    const bool busy = 32 * w < nrows;                        // the wave has rows
-    // of the wave's rows: the least last position and the largest first one
+    // The rows that all of the workgroup's queries see, [full_begin, full_end); of the wave's: those that some
+    // sees, [lmin, pmax], and that all see, [lmax, wave_end)
+    const int full_begin = a.window > 0 ? off + last - a.window + 1 : 0, full_end = min(off + first + 1, len);
     const int wtok0 = (int)(((long)tile * ROWS + min(32 * w, nrows - 1)) / rep), wtok1 = (int)(((long)tile * ROWS + min(32 * w + 31, nrows - 1)) / rep);
-    const int pmin = off + wtok0, pmax = off + wtok1, lmax = a.window > 0 ? max(0, pmax - a.window + 1) : 0;
-    const int lmin = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
+    const int pmax = 32 * w < nrows ? off + wtok1 : -1, lmax = a.window > 0 ? max(0, off + wtok1 - a.window + 1) : 0;
+    const int lmin = a.window > 0 ? max(0, off + wtok0 - a.window + 1) : 0, wave_end = min(off + wtok0 + 1, len);
     const long orow = (long)(q0 + tok) * a.NH + h;
 
     if (begin >= end && a.splits > 1) {
@@ -146,61 +150,103 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     const long rs = a.kv.row_stride * ES, ps = a.kv.page_stride * ES, hs = a.kv.head_stride * ES * j;
     const uint8_t *kb = (const uint8_t *)a.kv.k + hs, *vb = (const uint8_t *)a.kv.v + hs;
     const int lrow = lane / LPR, lpc = lane & (LPR - 1);     // row of a load and piece
-    const bool even = a.kv.page_size % 16 == 0;
-    // Row WR * w + RI * n + lrow of the step at s0: where it is, -1 if it holds nothing.  Each wave looks up
-    // its own rows and leaves word of which are on mapped pages.
-    struct place { long row[NI], exp[NI]; };
-    auto find = [&](int s0, place &p, int par) __attribute__((always_inline)) {
-        uint32_t on;
-        if (even) {                                          // the wave's rows lie in one page
-            const int s = s0 + WR * w, blk = pa_block(a, s);
-            const int pg = pa_table(a, seq, min(blk, a.kv.max_blocks - 1));
-            const bool in = s < len && pg >= 0 && pg < a.kv.n_pages;
-            const long row = s - blk * a.kv.page_size, at = pg * ps + row * rs;
-            on = in ? (1u << WR) - 1 : 0;
-#pragma unroll
-            for (int n = 0; n < NI; n++) {
-                const int x = RI * n + lrow;
-                p.row[n] = in && s + x < len ? at + x * rs : -1;
-                if constexpr (E8) p.exp[n] = (pg * (long)NKH + j) * a.kv.page_size + row + x;
-            }
+    // The pages of a step's rows, looked up a step before they are used.
+    //   EV 2: a step lies in one page (p0; block and row are counted on from step to step)
+    //   EV 1: every 16 rows do, and so do a wave's; 0: p0 is the page of row s0 + lane.
+    struct pages { int p0, p1, p2, p3; };
+    // all ones for the 16 rows that the wave brings
+    const int own0 = WR * w / 16 == 0 ? -1 : 0, own1 = WR * w / 16 == 1 ? -1 : 0, own2 = WR * w / 16 == 2 ? -1 : 0,
+              own3 = WR * w / 16 == 3 ? -1 : 0;
+    const int blk0 = EV == 2 && begin < end ? pa_block(a, begin) : 0;
+    int nblk = blk0, nrow = begin - blk0 * a.kv.page_size, row0 = nrow;   // EV 2: of the looked-up step; row0: in p0
+    auto look = [&](int s0) __attribute__((always_inline)) {
+        pages g{};
+        if constexpr (EV == 2) {
+            g.p0 = pa_table(a, seq, nblk);
+        } else if constexpr (EV == 1) {
+            auto page = [&](int s) { return pa_table(a, seq, min(pa_block(a, s), a.kv.max_blocks - 1)); };
+            g.p0 = page(s0);
+            g.p1 = page(s0 + 16);
+            if constexpr (TK == 64) { g.p2 = page(s0 + 32); g.p3 = page(s0 + 48); }
         } else {
-            const int s = s0 + WR * w + (lane & (WR - 1)), blk = pa_block(a, s);
-            int pg = -1;
-            if (s < len && blk < a.kv.max_blocks) pg = a.kv.tables[(long)seq * a.kv.table_ld + blk];
-            const bool in = pg >= 0 && pg < a.kv.n_pages;
-            on = (uint32_t)__ballot(in || s >= len) & ((1u << WR) - 1);
-            const int row = s - blk * a.kv.page_size;
-            const long at = in ? pg * ps + row * rs : -1, ex = (pg * (long)NKH + j) * a.kv.page_size + row;
-#pragma unroll
-            for (int n = 0; n < NI; n++) {
-                p.row[n] = __shfl(at, RI * n + lrow, 64);
-                if constexpr (E8) p.exp[n] = __shfl(ex, RI * n + lrow, 64);
-            }
+            const int s = s0 + (lane & (TK - 1)), blk = pa_block(a, s);
+            g.p0 = s < len && blk < a.kv.max_blocks ? a.kv.tables[(long)seq * a.kv.table_ld + blk] : -1;
         }
-        if (lane == 0) there[par][w] = on;
+        return g;
     };
+    // Bits: rows of the step on mapped pages (those past the length count as mapped).
+    constexpr uint64_t ALL = TK == 64 ? ~0ull : 0xFFFFFFFFull;
+    auto mapped = [&](int s0, const pages &g) __attribute__((always_inline)) {
+        uint64_t on = 0;
+        auto is = [&](int s, int p) { return s >= len || (unsigned)p < (unsigned)a.kv.n_pages; };
+        if constexpr (EV == 2) {
+            if (is(s0, g.p0)) on = ALL;
+        } else if constexpr (EV == 1) {
+            if (is(s0, g.p0)) on |= 0xFFFFull;
+            if (is(s0 + 16, g.p1)) on |= 0xFFFFull << 16;
+            if (is(s0 + 32, g.p2)) on |= 0xFFFFull << 32;
+            if (is(s0 + 48, g.p3)) on |= 0xFFFFull << 48;
+        } else {
+            on = __ballot(is(s0 + (lane & (TK - 1)), g.p0));
+        }
+        return on & ALL;
+    };
+    // this lane's pieces of its rows: bytes from the wave's first row (EV) or in the row; columns past head_dim
+    // read the row's start
+    unsigned pk_[NI], pv_[NI];
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+        const int x = WR * w + RI * n + lrow;
+        const int ck = 16 * (E8 ? lpc : lpc ^ kx(x)), cv = 16 * (E8 ? lpc : lpc ^ vx(x));
+        const unsigned o = EV ? (RI * n + lrow) * (unsigned)rs : 0;
+        pk_[n] = o + (ck < HD * ES ? ck : 0);
+        pv_[n] = o + (cv < HD * ES ? cv : 0);
+    }
     uint4 sk[E8 ? NI : 1], sv[E8 ? NI : 1];
     uint32_t se[2][E8 ? NI : 1];
-    auto fetch = [&](const place &p, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
+    // The wave's part of the step at s0, always 2 NI loads.  Rows past the length read what their page holds (with
+    // EV 0 the pool's first row), rows on no page the pool's first: it is masked, and looked through like every edge.
+    auto fetch = [&](int s0, const pages &g, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
+        const int mine = s0 + WR * w;
+        long at = 0, ex = 0;
+        if constexpr (EV) {
+            const int pg = EV == 2 ? g.p0 : (g.p0 & own0) | (g.p1 & own1) | (g.p2 & own2) | (g.p3 & own3);
+            const int row = EV == 2 ? row0 + WR * w : mine - pa_block(a, mine) * a.kv.page_size;
+            if (mine < len && (unsigned)pg < (unsigned)a.kv.n_pages) {
+                at = pg * ps + row * rs;
+                ex = (pg * (long)NKH + j) * a.kv.page_size + row;
+            }
+        } else {
+            const int s = s0 + (lane & (TK - 1)), row = s - pa_block(a, s) * a.kv.page_size;
+            if (s < len && (unsigned)g.p0 < (unsigned)a.kv.n_pages) {
+                at = g.p0 * ps + row * rs;
+                ex = (g.p0 * (long)NKH + j) * a.kv.page_size + row;
+            }
+        }
+        const uint8_t *bk = kb + at, *bv = vb + at;
 #pragma unroll
         for (int n = 0; n < NI; n++) {
-            const int x = WR * w + RI * n + lrow;        // row in the step
-            const bool in = p.row[n] >= 0;
-            const uint8_t *zero = (const uint8_t *)pa_zeros;
-            if constexpr (E8) {
-                const int col = 16 * lpc < HD ? 16 * lpc : 0;
-                sk[n] = *(const uint4 *)(in ? kb + p.row[n] + col : zero);
-                sv[n] = *(const uint4 *)(in ? vb + p.row[n] + col : zero);
-                se[0][n] = in ? a.kv.k_exp[p.exp[n]] : 127;
-                se[1][n] = in ? a.kv.v_exp[p.exp[n]] : 127;
+            const int x = RI * n + lrow;
+            const uint8_t *gk, *gv;
+            long e = ex + x;
+            if constexpr (EV) {
+                gk = bk + pk_[n];
+                gv = bv + pv_[n];
             } else {
-                const int ck = 16 * (lpc ^ kx(x)), cv = 16 * (lpc ^ vx(x));
-                const uint8_t *gk = in ? kb + p.row[n] + (ck < 2 * HD ? ck : 0) : zero;
-                const uint8_t *gv = in ? vb + p.row[n] + (cv < 2 * HD ? cv : 0) : zero;
-                const int at = (WR * w + RI * n) * RB;   // the load's 1 KB
-                __builtin_amdgcn_global_load_lds(gk, (__attribute__((address_space(3))) void *)(kl + at), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds(gv, (__attribute__((address_space(3))) void *)(vl + at), 16, 0, 0);
+                const long r = __shfl(at, WR * w + x, 64);
+                gk = kb + r + pk_[n];
+                gv = vb + r + pv_[n];
+                e = __shfl(ex, WR * w + x, 64);
+            }
+            if constexpr (E8) {
+                sk[n] = *(const uint4 *)gk;
+                sv[n] = *(const uint4 *)gv;
+                se[0][n] = a.kv.k_exp[e];
+                se[1][n] = a.kv.v_exp[e];
+            } else {
+                const int to = (WR * w + RI * n) * RB;       // the load's 1 KB
+                __builtin_amdgcn_global_load_lds(gk, (__attribute__((address_space(3))) void *)(kl + to), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds(gv, (__attribute__((address_space(3))) void *)(vl + to), 16, 0, 0);
             }
         }
     };
@@ -229,14 +275,10 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     const int kbase = c * RB, kxor = kx(c);
     const int vbase = (4 * hh + tr) * RB + 8 * (lane & 1), vpc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vxor = vx(4 * hh + tr);
 
-    auto work = [&](int s0, uint8_t *kl, uint8_t *vl, int par) __attribute__((always_inline)) {
-        // of the workgroup: some row is masked somewhere in this step
-        const int top_first = a.window > 0 ? off + last - a.window + 1 : 0;
-        uint32_t every = ~0u;
-#pragma unroll
-        for (int z = 0; z < NW; z++) every &= there[par][z];
-        const bool holes = __builtin_amdgcn_readfirstlane(every) != (1u << WR) - 1;
-        const bool edge = s0 + TK - 1 > off + first || s0 + TK > len || s0 < top_first || holes;
+    auto work = [&](int s0, bool holes, uint8_t *kl, uint8_t *vl, int par) __attribute__((always_inline)) {
+        // some row of the workgroup's is masked somewhere in this step
+        if (EV == 2 && holes) return;                        // none of the step's rows is there
+        const bool edge = s0 + TK > full_end || s0 < full_begin || (EV < 2 && holes);
         uint64_t bad = 0;
         if (edge) {                                          // the wave looks through its part of V
             uint32_t mine = 0;
@@ -265,7 +307,7 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
                 __syncthreads();
             }
         }
-        if (!busy || s0 > pmax || s0 + TK <= lmin) return;   // nothing that the wave's rows see
+        if (s0 > pmax || s0 + TK <= lmin) return;            // nothing that the wave's rows see
         // Operands are read from LDS ahead of the products that take them: K's two products' worth (KD), V's
         // a group of OB; the scheduler is held to that order, or it reads each right before its use.
         constexpr int KD = KS < 2 ? 1 : 2;
@@ -306,12 +348,11 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
             __builtin_amdgcn_sched_group_barrier(0x8, NB * NP, 0);
         }
         float top = -INFINITY;
-        if (s0 + TK - 1 > pmin || s0 < lmax || s0 + TK > len || holes) {
+        if (s0 + TK > wave_end || s0 < lmax || (EV < 2 && holes)) {
             asm volatile("");                                // a branch: the selects are for the few edges
             const int u = min(pr, len - 1) - s0 - 4 * hh, v = lr - s0 - 4 * hh;
-            uint64_t bits = 0;
-#pragma unroll
-            for (int z = 0; z < NW; z++) bits |= (uint64_t)there[par][z] << (WR * z);
+            uint64_t bits = ~0ull;
+            if (EV < 2 && holes) bits = mapped(s0, look(s0));
             bits >>= 4 * hh;
 #pragma unroll
             for (int n = 0; n < NB; n++)
@@ -399,32 +440,57 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     };
 
     if (begin < end) {
-        place p;
-        find(begin, p, 0);
-        fetch(p, k0, v0);
+        // Before its barrier a wave waits until its loads of the step have landed and its reads of the buffer
+        // that is filled next have returned.  Its younger loads, those of the steps in flight, may stay out: the
+        // count holds as every fetch issues 2 NI loads; any other load in between makes the wait stricter.
+        constexpr int D = NBUF - 1, YOUNG = E8 ? 0 : 2 * NI * (D - 1);
+        static_assert(YOUNG < 64, "vmcnt is six bits");
+        uint32_t holes = 0;                                  // per buffer: some row is on no page
+        pages g = look(begin);
+        auto bring = [&](int s0, uint8_t *kl, uint8_t *vl, int buf) __attribute__((always_inline)) {
+            fetch(s0, g, kl, vl);
+            const bool hole = EV == 2 ? s0 < len && (unsigned)g.p0 >= (unsigned)a.kv.n_pages : mapped(s0, g) != ALL;
+            holes = (holes & ~(1u << buf)) | (uint32_t)hole << buf;
+            if (s0 + TK < end) {
+                if constexpr (EV == 2) {
+                    nrow += TK;
+                    if (nrow == a.kv.page_size) { nrow = 0; nblk++; }
+                    row0 = nrow;
+                }
+                g = look(s0 + TK);
+            }
+        };
+        auto step = [&](int s0, uint8_t *kl, uint8_t *vl, int buf, uint8_t *kn, uint8_t *vn, int next) __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt((YOUNG & 15) | ((YOUNG >> 4) << 14) | 0x0070);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            bring(s0 + D * TK, kn, vn, next);
+            work(s0, holes >> buf & 1, kl, vl, buf & 1);
+            store(kn, vn);
+            return s0 + TK < end;
+        };
+        bring(begin, k0, v0, 0);
         store(k0, v0);
-        for (int s0 = begin;; s0 += 2 * TK) {
-            __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0): this wave's part is in LDS
-            __syncthreads();
-            bool more = s0 + TK < end;
-            if (more) {
-                find(s0 + TK, p, 1);
-                fetch(p, k1, v1);
+        if constexpr (NBUF > 2) bring(begin + TK, k1, v1, 1);
+        if constexpr (NBUF > 3) bring(begin + 2 * TK, k2, v2, 2);
+        for (int s0 = begin;; s0 += NBUF * TK) {
+            if constexpr (NBUF == 2) {
+                if (!step(s0, k0, v0, 0, k1, v1, 1)) break;
+                if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
+            } else if constexpr (NBUF == 3) {
+                if (!step(s0, k0, v0, 0, k2, v2, 2)) break;
+                if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
+                if (!step(s0 + 2 * TK, k2, v2, 2, k1, v1, 1)) break;
+            } else {
+                if (!step(s0, k0, v0, 0, k3, v3, 3)) break;
+                if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
+                if (!step(s0 + 2 * TK, k2, v2, 2, k1, v1, 1)) break;
+                if (!step(s0 + 3 * TK, k3, v3, 3, k2, v2, 2)) break;
             }
-            work(s0, k0, v0, 0);
-            if (!more) break;
-            store(k1, v1);
-            __builtin_amdgcn_s_waitcnt(0x0F70);
-            __syncthreads();
-            more = s0 + 2 * TK < end;
-            if (more) {
-                find(s0 + 2 * TK, p, 0);
-                fetch(p, k0, v0);
-            }
-            work(s0 + TK, k1, v1, 1);
-            if (!more) break;
-            store(k0, v0);
         }
+        __builtin_amdgcn_s_waitcnt(0x0F70);                  // no load may still be on its way into LDS at the end
     }
     if (rr >= nrows) return;
     float l = l0 + l1;
@@ -442,17 +508,25 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     if (a.splits > 1 && hh == 0) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(m, l);
 }
 
-template <int CT, bool HP, int HDB, int NW> static void pa_prompt_go(const pa_args &a, hipStream_t st)
+template <int CT, bool HP, int HDB, int NW, int EV> static void pa_prompt_ev(const pa_args &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB, NW>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB, NW, EV>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(64 * NW), 0, st, a);
 }
-template <int CT> static void pa_prompt(const pa_args &a, bool wide, hipStream_t st)
+template <int CT, bool HP, int HDB> static void pa_prompt_go(const pa_args &a, bool uniform, hipStream_t st)
+{
+    if constexpr (!HP && (HDB == 128 || HDB == 64 && CT != MLLM_E4M3))
+        if (a.waves == 8) return pa_prompt_ev<CT, HP, HDB, 8, 2>(a, st);
+    if (!uniform) pa_prompt_ev<CT, HP, HDB, 4, 0>(a, st);
+    else if (a.kv.page_size % 64) pa_prompt_ev<CT, HP, HDB, 4, 1>(a, st);
+    else pa_prompt_ev<CT, HP, HDB, 4, 2>(a, st);
+}
+template <int CT, bool HP> static void pa_prompt_hd(const pa_args &a, bool uniform, hipStream_t st)
 {
     const int HD = a.kv.head_dim;
-    if (wide)
-        HD <= 64 ? pa_prompt_go<CT, true, 64, 4>(a, st) : HD <= 128 ? pa_prompt_go<CT, true, 128, 4>(a, st) : pa_prompt_go<CT, true, 256, 4>(a, st);
-    else if (a.waves == 8)
-        HD <= 64 ? pa_prompt_go<CT, false, 64, CT == MLLM_E4M3 ? 4 : 8>(a, st) : pa_prompt_go<CT, false, 128, 8>(a, st);
-    else
-        HD <= 64 ? pa_prompt_go<CT, false, 64, 4>(a, st) : HD <= 128 ? pa_prompt_go<CT, false, 128, 4>(a, st) : pa_prompt_go<CT, false, 256, 4>(a, st);
+    HD <= 64 ? pa_prompt_go<CT, HP, 64>(a, uniform, st) : HD <= 128 ? pa_prompt_go<CT, HP, 128>(a, uniform, st)
+                                                                    : pa_prompt_go<CT, HP, 256>(a, uniform, st);
+}
+template <int CT> static void pa_prompt(const pa_args &a, bool wide, bool uniform, hipStream_t st)
+{
+    wide ? pa_prompt_hd<CT, true>(a, uniform, st) : pa_prompt_hd<CT, false>(a, uniform, st);
 }

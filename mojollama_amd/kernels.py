@@ -318,6 +318,7 @@ class DeviceOps:
         import torch
         self.torch = torch
         self.so = so or load_kernels()
+        self._types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}
 
     def _stream(self):
         return ctypes.c_void_p(self.torch.cuda.current_stream().cuda_stream)
@@ -451,27 +452,32 @@ class DeviceOps:
         return buf
 
     # ------------------------------------------- paged 16- or 8-bit KV cache
-    def _type(self, t, what):
-        """mllm type of a tensor on the current GPU whose last dimension is dense."""
-        torch = self.torch
-        code = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}.get(
-            t.dtype)
+    def _cur(self):
+        return self.torch.cuda.current_device()
+
+    def _raw_stream(self, cur):
+        return self.torch._C._cuda_getCurrentRawStream(cur)
+
+    def _type(self, t, what, cur):
+        """mllm type of a tensor on the current GPU (cur) whose last dimension is dense."""
+        code = self._types.get(t.dtype)
         if code is None:
             raise TypeError(f"{what}: {t.dtype} is not served")
-        self._here(t, what)
+        if t.get_device() != cur:
+            self._elsewhere(t, what)
         if t.stride(-1) != 1 and t.shape[-1] > 1:
             raise ValueError(f"{what}: the last dimension is not dense")
         return code
 
-    def _here(self, t, what):
-        if t.device.type != "cuda" or t.device.index != self.torch.cuda.current_device():
-            raise ValueError(f"{what}: a tensor on {t.device}, not on the current GPU")
+    def _elsewhere(self, t, what):
+        raise ValueError(f"{what}: a tensor on {t.device}, not on the current GPU")
 
-    def _ints(self, t, what, n=None):
+    def _ints(self, t, what, cur, n=None):
         """Address of a dense int32 tensor on the current GPU (None: a null pointer)."""
         if t is None:
             return None
-        self._here(t, what)
+        if t.get_device() != cur:
+            self._elsewhere(t, what)
         if t.dtype != self.torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
             raise ValueError(f"{what}: a dense int32 tensor{'' if n is None else ' of %d' % n} is needed")
         return t.data_ptr()
@@ -481,11 +487,12 @@ class DeviceOps:
         float8_e4m3fn; any strides, the last dimension dense, so a [page][head][row] pool is passed permuted) and
         tables int32 [n_seqs, max_blocks]; float8 pools with their exponents uint8 [n_pages, n_kv_head, page_size].
         The view keeps the tensors alive."""
-        torch = self.torch
-        code = self._type(k, "k")
-        if code != self._type(v, "v") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4:
+        torch, cur = self.torch, self._cur()
+        code = self._type(k, "k", cur)
+        if code != self._type(v, "v", cur) or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4:
             raise ValueError("k and v: two pools [page, row, head, element] of one type, shape and strides")
-        self._here(tables, "tables")
+        if tables.get_device() != cur:
+            self._elsewhere(tables, "tables")
         if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1:
             raise ValueError("tables: int32 [n_seqs, max_blocks], rows dense")
         n_pages, page, heads, hd = k.shape
@@ -493,7 +500,8 @@ class DeviceOps:
             if (e is None) != (code != T_E4M3):
                 raise ValueError("k_exp and v_exp belong to float8 pools")
             if e is not None:
-                self._here(e, "exponents")
+                if e.get_device() != cur:
+                    self._elsewhere(e, "exponents")
                 if e.dtype != torch.uint8 or tuple(e.shape) != (n_pages, heads, page) or not e.is_contiguous():
                     raise ValueError("exponents: dense uint8 [n_pages, n_kv_head, page_size]")
         p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
@@ -517,27 +525,30 @@ class DeviceOps:
         """mllm_rotary_append: q [T, NH*HD], k, v [T, NKH*HD] (parts of a fused buffer may be passed as slices; q, or k
         and v, may be None), pos int32 [T]; k and v go to rows `rows` (None: pos) of sequences `seqs` (None: 0, 1, ...)
         of kv, the turned q to q_out and k to k_out.  Heads and head size come from kv where it is given."""
-        T = self._ints(pos, "pos") and pos.numel()
+        cur = self._cur()
+        pp, T = self._ints(pos, "pos", cur), pos.numel()
         if kv is not None:
             NKH, HD = kv.n_kv_head, kv.head_dim
-        parts = []
-        for t, n, what in ((q, NH * HD, "q"), (k, NKH * HD, "k"), (v, NKH * HD, "v"), (q_out, NH * HD, "q_out"),
-                           (k_out, NKH * HD, "k_out")):
-            if t is None:
-                parts += [None, None, 0]
-                continue
-            code = self._type(t, what)
-            if t.dim() != 2 or t.shape[0] != T or t.shape[1] != n:
-                raise ValueError(f"{what}: [{T}, {n}] is needed, got {list(t.shape)}")
-            parts += [code, t.data_ptr(), t.stride(0) if T > 1 else max(t.stride(0), n)]
-        ins, outs = {c for c in parts[0:9:3] if c is not None}, {c for c in parts[9::3] if c is not None}
-        if len(ins) > 1 or len(outs) > 1:
-            raise TypeError("q, k and v have one type, and q_out and k_out")
+        it, qp, ql = self._rows(q, "q", T, NH * HD, cur, None)
+        it, kp, kl = self._rows(k, "k", T, NKH * HD, cur, it)
+        it, vp, vl = self._rows(v, "v", T, NKH * HD, cur, it)
+        ot, qop, qol = self._rows(q_out, "q_out", T, NH * HD, cur, None)
+        ot, kop, kol = self._rows(k_out, "k_out", T, NKH * HD, cur, ot)
         self._check(self.so.mllm_rotary_append(
-            rot, ins.pop() if ins else T_F32, parts[1], parts[2], parts[4], parts[5], parts[7], parts[8], pos.data_ptr(),
-            T, NH, NKH, HD, outs.pop() if outs else T_F32, parts[10], parts[11], parts[13], parts[14], kv,
-            self._ints(seqs, "seqs", T), self._ints(rows, "rows", T), self.torch.cuda.current_stream().cuda_stream),
+            rot, it or T_F32, qp, ql, kp, kl, vp, vl, pp, T, NH, NKH, HD, ot or T_F32, qop, qol, kop, kol, kv,
+            self._ints(seqs, "seqs", cur, T), self._ints(rows, "rows", cur, T), self._raw_stream(cur)),
             "mllm_rotary_append")
+
+    def _rows(self, t, what, T, n, cur, code):
+        """(type, address, row stride) of a [T, n] tensor of type `code` (None: any); nothing for None."""
+        if t is None:
+            return code, None, 0
+        c = self._type(t, what, cur)
+        if t.dim() != 2 or t.shape[0] != T or t.shape[1] != n:
+            raise ValueError(f"{what}: [{T}, {n}] is needed, got {list(t.shape)}")
+        if code is not None and c != code:
+            raise TypeError("q, k and v have one type, and q_out and k_out")
+        return c, t.data_ptr(), t.stride(0) if T > 1 else max(t.stride(0), n)
 
     def paged_attn_workspace(self, kv, T, B, NH, max_len, window=0):
         """A workspace for paged_attn_decode (T = B) and paged_attn_prompt calls up to these sizes."""
@@ -546,57 +557,57 @@ class DeviceOps:
             raise ValueError("paged_attn_workspace: sizes that are not served")
         return self.torch.empty(n, dtype=self.torch.uint8, device="cuda")
 
-    def _attn(self, kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws):
-        if q.dim() != 2 or q.shape[1] != NH * kv.head_dim:
-            raise ValueError(f"q: [tokens, {NH * kv.head_dim}] is needed, got {list(q.shape)}")
-        qt = self._type(q, "q")
+    def _attn(self, kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws, cur):
+        n = NH * kv.head_dim
+        qt, qp, ql = self._rows(q, "q", T, n, cur, None)
         if out is None:
-            out = self.torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-        elif out.shape != q.shape:
-            raise ValueError("out: the shape of q is needed")
+            out = self.torch.empty((T, n), dtype=out_dtype or q.dtype, device=q.device)
+        ot, op, ol = self._rows(out, "out", T, n, cur, None)
+        sk = None
         if sinks is not None:
-            self._here(sinks, "sinks")
+            if sinks.get_device() != cur:
+                self._elsewhere(sinks, "sinks")
             if sinks.dtype != self.torch.float32 or sinks.numel() != NH or not sinks.is_contiguous():
                 raise ValueError("sinks: dense float32 [NH]")
+            sk = sinks.data_ptr()
         if ws is None:
             ws = self.paged_attn_workspace(kv, T, B, NH, max_len, window)
-        else:
-            self._here(ws, "workspace")
-        n = q.shape[1]
-        return (qt, q.data_ptr(), q.stride(0) if T > 1 else max(q.stride(0), n), out, self._type(out, "out"),
-                out.data_ptr(), out.stride(0) if T > 1 else max(out.stride(0), n), ws,
-                sinks.data_ptr() if sinks is not None else None)
+        elif ws.get_device() != cur:
+            self._elsewhere(ws, "workspace")
+        return qt, qp, ql, out, ot, op, ol, ws, sk
 
     def paged_attn_decode(self, kv, q, lens, max_len, NH, scale=None, window=0, sinks=None, seqs=None, out=None,
                           out_dtype=None, ws=None):
         """mllm_paged_attn_decode: q [B, NH*HD], lens int32 [B] (cached rows, the new one among them, at most max_len);
         scale None: 1/sqrt(HD); out in out_dtype (None: q's)."""
-        B = q.shape[0]
-        qt, qp, ql, out, ot, op, ol, ws, sk = self._attn(kv, q, B, B, NH, max_len, window, sinks, out, out_dtype, ws)
+        B, cur = q.shape[0], self._cur()
+        qt, qp, ql, out, ot, op, ol, ws, sk = self._attn(kv, q, B, B, NH, max_len, window, sinks, out, out_dtype, ws, cur)
         self._check(self.so.mllm_paged_attn_decode(
-            kv, qt, qp, ql, self._ints(seqs, "seqs", B), self._ints(lens, "lens", B), max_len, B, NH,
-            kv.head_dim ** -0.5 if scale is None else scale, window, sk, ot, op, ol, ws.data_ptr(),
-            ws.numel() * ws.element_size(), self.torch.cuda.current_stream().cuda_stream), "mllm_paged_attn_decode")
+            kv, qt, qp, ql, self._ints(seqs, "seqs", cur, B), self._ints(lens, "lens", cur, B), max_len, B, NH,
+            kv.head_dim ** -0.5 if scale is None else scale, window, sk, ot, op, ol, ws.data_ptr(), ws.nbytes,
+            self._raw_stream(cur)), "mllm_paged_attn_decode")
         return out
 
     def paged_attn_prompt(self, kv, q, starts, lens, max_len, NH, scale=None, window=0, sinks=None, seqs=None, out=None,
                           out_dtype=None, ws=None):
         """mllm_paged_attn_prompt: q [T, NH*HD] holds the new tokens of B sequences, starts int32 [B + 1], lens int32
         [B] (cached rows, the new ones among them, at most max_len)."""
-        T, B = q.shape[0], lens.numel()
-        qt, qp, ql, out, ot, op, ol, ws, sk = self._attn(kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws)
+        T, B, cur = q.shape[0], lens.numel(), self._cur()
+        qt, qp, ql, out, ot, op, ol, ws, sk = self._attn(kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws, cur)
         self._check(self.so.mllm_paged_attn_prompt(
-            kv, qt, qp, ql, self._ints(seqs, "seqs", B), self._ints(starts, "starts", B + 1), self._ints(lens, "lens", B),
-            max_len, T, B, NH, kv.head_dim ** -0.5 if scale is None else scale, window, sk, ot, op, ol, ws.data_ptr(),
-            ws.numel() * ws.element_size(), self.torch.cuda.current_stream().cuda_stream), "mllm_paged_attn_prompt")
+            kv, qt, qp, ql, self._ints(seqs, "seqs", cur, B), self._ints(starts, "starts", cur, B + 1),
+            self._ints(lens, "lens", cur, B), max_len, T, B, NH, kv.head_dim ** -0.5 if scale is None else scale, window,
+            sk, ot, op, ol, ws.data_ptr(), ws.nbytes, self._raw_stream(cur)), "mllm_paged_attn_prompt")
         return out
 
     def page_map(self, tables, refs, page_size):
         """An mllm_page_map over tables int32 [n_seqs, max_blocks] (-1 unmapped) and refs int32 [n_pages]."""
-        self._here(tables, "tables")
+        cur = self._cur()
+        if tables.get_device() != cur:
+            self._elsewhere(tables, "tables")
         if tables.dtype != self.torch.int32 or tables.dim() != 2 or tables.stride(1) != 1:
             raise ValueError("tables: int32 [n_seqs, max_blocks], rows dense")
-        m = PageMap(tables.data_ptr(), tables.shape[0], tables.shape[1], tables.stride(0), self._ints(refs, "refs"),
+        m = PageMap(tables.data_ptr(), tables.shape[0], tables.shape[1], tables.stride(0), self._ints(refs, "refs", cur),
                     refs.numel(), page_size)
         m._tensors = (tables, refs)
         return m
@@ -606,7 +617,8 @@ class DeviceOps:
         of float8 pools)."""
         planes = (PagePlane * len(pools))()
         for p, t in zip(planes, pools):
-            self._here(t, "pool")
+            if t.get_device() != self._cur():
+                self._elsewhere(t, "pool")
             if t.dim() < 2 or not t[0].is_contiguous():
                 raise ValueError("pools: [n_layers, n_pages, ...], each layer dense")
             p.base, p.n_layers = t.data_ptr(), t.shape[0]
@@ -618,14 +630,15 @@ class DeviceOps:
         """A workspace for pages_reserve and pages_fork calls of up to n requests, and pages_compact."""
         return self.torch.empty(self.so.mllm_pages_workspace_size(m, n), dtype=self.torch.uint8, device="cuda")
 
-    def _pages_args(self, m, n, status, ws):
+    def _pages_args(self, m, n, status, ws, cur):
         torch = self.torch
         if status is None:
             status = torch.empty(1, dtype=torch.int32, device="cuda")
         if ws is None:
             ws = self.pages_workspace(m, n)
-        self._here(ws, "workspace")
-        return status, self._ints(status, "status"), ws
+        elif ws.get_device() != cur:
+            self._elsewhere(ws, "workspace")
+        return status, self._ints(status, "status", cur, 1), ws
 
     @staticmethod
     def _pages_in(planes, n_pages):
@@ -635,44 +648,45 @@ class DeviceOps:
     def pages_reserve(self, m, seqs, lens, status=None, ws=None):
         """mllm_pages_reserve: pages for rows below lens[i] of sequences seqs[i]; returns status (a device int32, 0 when
         every request was met)."""
-        n = seqs.numel()
-        status, sp, ws = self._pages_args(m, n, status, ws)
-        self._check(self.so.mllm_pages_reserve(m, n, self._ints(seqs, "seqs"), self._ints(lens, "lens", n), sp,
-                                               ws.data_ptr(), ws.numel() * ws.element_size(), self._stream()),
+        n, cur = seqs.numel(), self._cur()
+        status, sp, ws = self._pages_args(m, n, status, ws, cur)
+        self._check(self.so.mllm_pages_reserve(m, n, self._ints(seqs, "seqs", cur), self._ints(lens, "lens", cur, n), sp,
+                                               ws.data_ptr(), ws.nbytes, self._raw_stream(cur)),
                     "mllm_pages_reserve")
         return status
 
     def pages_free(self, m, seqs, lens=None):
         """mllm_pages_free: sequences seqs[i] give back their pages past the first lens[i] rows (None: all)."""
-        n = seqs.numel()
-        self._check(self.so.mllm_pages_free(m, n, self._ints(seqs, "seqs"), self._ints(lens, "lens", n), self._stream()),
+        n, cur = seqs.numel(), self._cur()
+        self._check(self.so.mllm_pages_free(m, n, self._ints(seqs, "seqs", cur), self._ints(lens, "lens", cur, n), self._raw_stream(cur)),
                     "mllm_pages_free")
 
     def pages_fork(self, m, planes, parents, children, lens, status=None, ws=None):
         """mllm_pages_fork: children[i] takes over the first lens[i] rows of parents[i], all at once; returns status."""
-        n = parents.numel()
+        n, cur = parents.numel(), self._cur()
         self._pages_in(planes, m.n_pages)
-        status, sp, ws = self._pages_args(m, n, status, ws)
-        self._check(self.so.mllm_pages_fork(m, planes, len(planes), n, self._ints(parents, "parents"),
-                                            self._ints(children, "children", n), self._ints(lens, "lens", n), sp,
-                                            ws.data_ptr(), ws.numel() * ws.element_size(), self._stream()),
+        status, sp, ws = self._pages_args(m, n, status, ws, cur)
+        self._check(self.so.mllm_pages_fork(m, planes, len(planes), n, self._ints(parents, "parents", cur),
+                                            self._ints(children, "children", cur, n), self._ints(lens, "lens", cur, n), sp,
+                                            ws.data_ptr(), ws.nbytes, self._raw_stream(cur)),
                     "mllm_pages_fork")
         return status
 
     def pages_compact(self, m, planes, status=None, ws=None):
         """mllm_pages_compact: the live pages move to the front; returns their number (a device int32)."""
+        cur = self._cur()
         self._pages_in(planes, m.n_pages)
-        status, sp, ws = self._pages_args(m, 0, status, ws)
+        status, sp, ws = self._pages_args(m, 0, status, ws, cur)
         self._check(self.so.mllm_pages_compact(m, planes, len(planes), sp, ws.data_ptr(),
-                                               ws.numel() * ws.element_size(), self._stream()), "mllm_pages_compact")
+                                               ws.nbytes, self._raw_stream(cur)), "mllm_pages_compact")
         return status
 
     def pages_copy(self, planes, n_pages, src, dst):
         """mllm_pages_copy: page dst[i] := page src[i] in every plane."""
-        n = src.numel()
+        n, cur = src.numel(), self._cur()
         self._pages_in(planes, n_pages)
-        self._check(self.so.mllm_pages_copy(planes, len(planes), n_pages, n, self._ints(src, "src"),
-                                            self._ints(dst, "dst", n), self._stream()), "mllm_pages_copy")
+        self._check(self.so.mllm_pages_copy(planes, len(planes), n_pages, n, self._ints(src, "src", cur),
+                                            self._ints(dst, "dst", cur, n), self._raw_stream(cur)), "mllm_pages_copy")
 
     def moe_prepare(self, qts, N, M, E, K, gates, ups, downs, router, renorm):
         """gates/ups/downs: per-expert raw GGUF uint8 tensors (GPU) in the
