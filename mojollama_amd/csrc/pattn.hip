@@ -126,7 +126,7 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         a.groups = (a.rep + 15) / 16;
         const long n = seen(a.max_len, a.window);
         a.splits = pa_splits((long)a.B * a.kv.n_kv_head * a.groups, n, kDecodeWG);
-        a.chunk = (int)std::min<long>(0x7FFFFF80, (n + a.splits - 1) / a.splits / 128 * 128 + 128);
+        a.chunk = (int)(std::max<long>(1, (n + 128l * a.splits - 1) / (128l * a.splits)) * 128);
         a.splits = (int)std::max<long>(1, (n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
         if (a.kv.type == MLLM_F16) pa_decode_f16(a, wide, uniform, st);
@@ -142,7 +142,7 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         // 29 / 123 us
         const long most = n * a.B * a.kv.n_kv_head * es / (4l * a.T * a.NH);
         a.splits = a.waves == 8 ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG)));
-        a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + a.splits - 1) / a.splits / 64 * 64 + 64);
+        a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + 64l * a.splits - 1) / (64l * a.splits) * 64);
         if (a.splits > 1) a.splits = (int)((n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
         if (a.kv.type == MLLM_F16) pa_prompt_f16(a, wide, uniform, st);
