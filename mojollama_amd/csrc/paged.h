@@ -97,13 +97,22 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type)
     return __builtin_bit_cast(uint32_t, (f16x2){(_Float16)a, (_Float16)b});
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <bool PAST> __device__ __forceinline__ void put16(void *p, u32x4 v)
+{
+    if constexpr (PAST) __builtin_nontemporal_store(v, (u32x4 *)p);
+    else *(u32x4 *)p = v;
+}
+
+// PAST: past the caches (rows that are multiples of 16 bytes).
+template <bool PAST = false>
 __device__ __forceinline__ void store8(void *p, long at, int type, bool wide, const float (&x)[8])
 {
     if (type == MLLM_F32) {
         float *f = (float *)p + at;
         if (wide) {
-            ((float4 *)f)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            ((float4 *)f)[1] = make_float4(x[4], x[5], x[6], x[7]);
+            put16<PAST>(f, __builtin_bit_cast(u32x4, (f32x4){x[0], x[1], x[2], x[3]}));
+            put16<PAST>(f + 4, __builtin_bit_cast(u32x4, (f32x4){x[4], x[5], x[6], x[7]}));
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) f[i] = x[i];
@@ -115,7 +124,7 @@ __device__ __forceinline__ void store8(void *p, long at, int type, bool wide, co
     for (int i = 0; i < 4; i++) w[i] = pack16(x[2 * i], x[2 * i + 1], type);
     uint16_t *h = (uint16_t *)p + at;
     if (wide) {
-        *(uint4 *)h = make_uint4(w[0], w[1], w[2], w[3]);
+        put16<PAST>(h, (u32x4){w[0], w[1], w[2], w[3]});
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) { h[2 * i] = (uint16_t)w[i]; h[2 * i + 1] = (uint16_t)(w[i] >> 16); }

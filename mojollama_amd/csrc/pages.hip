@@ -240,7 +240,6 @@ __global__ __launch_bounds__(kWG) void k_fork_plan(mllm_page_map m, int n, const
 // that are 16 KB together.  The pages are not read again soon and pass the caches by: 17 copies of 3.1 MB
 // pages 28.9 -> 20.2 us, 134 of 0.5 MB 56.5 -> 37.5 us (stores that stay in L2 evict what is read; loads
 // past the caches as well 44 us).
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void copy_unit(const copy_args &c, int unit, int src, int dst)
 {
     int i = 0;

@@ -84,11 +84,24 @@ constexpr long kPartRows = 65536, kDecodeWG = kPartRows / 16, kPromptWG = kPartR
 // Rows that a query can see, as far as the host knows.
 long seen(int max_len, int window) { return window > 0 ? std::min<long>(max_len, (long)window + 31) : max_len; }
 
-// Splits of a launch of `wgs` workgroups that each would take all of n rows.
-int pa_splits(long wgs, long n, long target)
+long up(long a, long b) { return (a + b - 1) / b; }
+
+// Splits of a launch of `wgs` workgroups that would each take all of n rows: until there are kPromptWG.
+int pa_splits(long wgs, long n)
 {
-    const long want = std::min<long>((target + wgs - 1) / wgs, (n + kMinRows - 1) / kMinRows);
-    return (int)std::max<long>(1, std::min<long>(want, kMaxSplits));
+    return (int)std::max<long>(1, std::min({up(kPromptWG, wgs), up(n, kMinRows), (long)kMaxSplits}));
+}
+
+// In decode, of 1024 rows where the launch is large (unequal lengths then share the GPU evenly, and the sums
+// stay small), down to 256 until every CU has a workgroup; up to 640 rows whole, which saves the join.
+// 256 / 512 / 1024 rows: one sequence of 2000 rows, 4 kv heads, 8.2 / 9.6 / 12.4 us, of 131072 60.8 / 60.6 /
+// 58.7, eight of 2048 to 4096, 8 kv heads, 18.3 / 19.2 / 16.5, 48 of up to 9000 42.0 / 42.5 / 43.1; one of 300
+// rows whole / split 5.8 / 8.1, of 500 6.7 / 8.2, of 700 8.0 / 8.2.
+int pa_splits_decode(long wgs, long n)
+{
+    if (n <= 640) return 1;
+    const long fill = std::min(up(n, kMinRows), up(256, wgs));
+    return (int)std::min({std::max(std::min(up(n, 1024), up(kDecodeWG, wgs)), fill), (long)kMaxSplits});
 }
 
 void pa_divisor(pa_args &a)
@@ -125,7 +138,7 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
     if (!a.starts) {
         a.groups = (a.rep + 15) / 16;
         const long n = seen(a.max_len, a.window);
-        a.splits = pa_splits((long)a.B * a.kv.n_kv_head * a.groups, n, kDecodeWG);
+        a.splits = pa_splits_decode((long)a.B * a.kv.n_kv_head * a.groups, n);
         a.chunk = (int)(std::max<long>(1, (n + 128l * a.splits - 1) / (128l * a.splits)) * 128);
         a.splits = (int)std::max<long>(1, (n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
@@ -141,7 +154,7 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         // splits / whole 52.7 / 32.2 us; 3 to 5 tokens over 1500 to 4000 rows, 64/8 heads of 64, seven / whole
         // 29 / 123 us
         const long most = n * a.B * a.kv.n_kv_head * es / (4l * a.T * a.NH);
-        a.splits = a.waves == 8 ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG)));
+        a.splits = a.waves == 8 ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n)));
         a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + 64l * a.splits - 1) / (64l * a.splits) * 64);
         if (a.splits > 1) a.splits = (int)((n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
