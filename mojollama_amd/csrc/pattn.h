@@ -13,11 +13,11 @@ struct pa_args {
     float scale;
     const float *sinks;
     // set by the launcher
-    int rep, groups;               // query heads per kv head, in groups of 16 (decode)
+    int rep, groups;               // query heads per kv head; of 16 (decode), or 32 rows of a tile (prompt)
     unsigned div_mul;              // s / page_size = s * div_mul >> div_sh for 0 <= s < 2^31
     int div_sh;
     int chunk, splits;             // rows per split, splits of a query's range of rows
-    int waves, tiles;              // prompt: waves of 32 rows per tile, tiles at most
+    int tiles;                     // prompt: tiles at most
     float *part, *stat;            // with splits > 1: sums [T * NH][splits][HD], (maximum, sum) [T * NH][splits]
 };
 
@@ -97,6 +97,13 @@ __device__ __forceinline__ void pa_finish(const pa_args &a, int h, int t, int d,
     else
         *(uint2 *)((uint16_t *)a.out + at) = make_uint2(pack16(y.x * f, y.y * f, a.out_type), pack16(y.z * f, y.w * f, a.out_type));
 }
+
+// The prompt kernel's tile: groups of 32 rows, and whether two waves share each, one half of every step's
+// rows of K and V for each.
+constexpr int pa_row_groups(int type, bool wide, int hdb) { return wide ? 2 : 4; }
+// ... or, at head sizes above 128, the columns of the output: the registers of a wave hold half of them.
+constexpr int pa_parts(int hdb) { return hdb > 128 ? 2 : 1; }
+constexpr int pa_halves(int type, bool wide, int hdb) { return hdb > 128 || (!wide && type == MLLM_E4M3 && hdb == 64) ? 1 : 2; }
 
 void pa_decode_bf16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_f16(const pa_args &a, bool wide, bool uniform, hipStream_t st);

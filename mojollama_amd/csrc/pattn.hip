@@ -86,10 +86,10 @@ long seen(int max_len, int window) { return window > 0 ? std::min<long>(max_len,
 
 long up(long a, long b) { return (a + b - 1) / b; }
 
-// Splits of a launch of `wgs` workgroups that would each take all of n rows: until there are kPromptWG.
-int pa_splits(long wgs, long n)
+// Splits of a launch of `wgs` workgroups that would each take all of n rows: until there are `target`.
+int pa_splits(long wgs, long n, long target)
 {
-    return (int)std::max<long>(1, std::min({up(kPromptWG, wgs), up(n, kMinRows), (long)kMaxSplits}));
+    return (int)std::max<long>(1, std::min({up(target, wgs), up(n, kMinRows), (long)kMaxSplits}));
 }
 
 // In decode, of 1024 rows where the launch is large (unequal lengths then share the GPU evenly, and the sums
@@ -147,14 +147,19 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         else pa_decode_e4m3(a, wide, uniform, st);
     } else {
         const long rows = (long)a.T * a.rep, n = a.window > 0 ? std::min<long>(a.window + 320l, a.max_len) : a.max_len;
-        a.waves = uniform && a.kv.page_size % 64 == 0 && !wide && a.kv.head_dim <= 128 && (es == 2 || a.kv.head_dim > 64) && rows / 256 * a.kv.n_kv_head >= 256 ? 8 : 4;
-        a.tiles = (int)(rows / (32 * a.waves) + std::min(a.T, a.B));
+        const int hdb = a.kv.head_dim <= 64 ? 64 : a.kv.head_dim <= 128 ? 128 : 256;
+        a.groups = pa_row_groups(a.kv.type, wide, hdb);
+        // tiles of 256 rows, half the traffic from L2, where they fill the GPU
+        const bool large = a.groups == 4 && pa_halves(a.kv.type, wide, hdb) == 2 && uniform && a.kv.page_size % 64 == 0 &&
+                           rows / 256 * a.kv.n_kv_head >= 256;
+        if (large) a.groups = 8;
+        a.tiles = (int)(rows / (32 * a.groups) + std::min(a.T, a.B));
         // no more than keep the partial sums, written and read again, below the rows of K and V that they save
         // time on: prompts of 1 to 1100 tokens over up to 2600 rows, window 512, 16/4 heads of 96, in three
         // splits / whole 52.7 / 32.2 us; 3 to 5 tokens over 1500 to 4000 rows, 64/8 heads of 64, seven / whole
         // 29 / 123 us
         const long most = n * a.B * a.kv.n_kv_head * es / (4l * a.T * a.NH);
-        a.splits = a.waves == 8 ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n)));
+        a.splits = large ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG)));
         a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + 64l * a.splits - 1) / (64l * a.splits) * 64);
         if (a.splits > 1) a.splits = (int)((n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");

@@ -19,14 +19,15 @@
 // maximum per head and moves it rarely (kSlack), and each lane its own part of the sum, so the loop has
 // no exchange between lanes.  The four waves of a workgroup take every fourth tile pair and join in LDS.
 //
-// HP: q and the weights in planes that hold fp32's precision (each product once per plane); the
-// loop stays bound by memory.  PU: pages of a multiple of 16 rows: a tile lies in one page, whose
+// HP: q and the weights in planes that hold fp32's precision (each product once per plane); else q is
+// 16 bits as it is, and the weights take two planes all the same: the loop stays bound by memory, and
+// one plane's rounding is as large as the output's own.  PU: pages of a multiple of 16 rows: a tile lies in one page, whose
 // number comes through the scalar cache two steps ahead; else every lane looks its row up.
 template <int CT, bool HP, int HDB, bool PU>
 __global__ __launch_bounds__(256, HDB == 256 || (HP && HDB == 128) ? 1 : 2) void k_pa_decode(pa_args a)
 {
     constexpr bool E8 = CT == MLLM_E4M3;
-    constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1;
+    constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1, NW = HP ? kPlanes<CT> : 2;   // planes of q, of the weights
     constexpr int KS = HDB / 32;                     // 16x16x32 products per tile of scores
     constexpr int KW = E8 ? KS / 2 : KS;             // 16-byte loads per K row and lane
     constexpr int NM = HDB / 16;                     // columns per lane of V
@@ -249,14 +250,14 @@ __global__ __launch_bounds__(256, HDB == 256 || (HP && HDB == 128) ? 1 : 2) void
 #pragma unroll
                 for (int x = 0; x < NM; x++) o[x] *= f;
             }
-            uint32_t pw[4][NP];
+            uint32_t pw[4][NW];
 #pragma unroll
             for (int r = 0; r < 8; r++) {
                 z[r] = __builtin_amdgcn_exp2f(z[r] - (m - kBias<CT>));
                 l += z[r];
             }
 #pragma unroll
-            for (int x = 0; x < 4; x++) pa_planes<CT, NP>(z[2 * x], z[2 * x + 1], pw[x]);
+            for (int x = 0; x < 4; x++) pa_planes<CT, NW>(z[2 * x], z[2 * x + 1], pw[x]);
             if (!all) {                              // what lies in rows that are not the query's may be NaN
 #pragma unroll
                 for (int r = 0; r < 8; r++)
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(256, HDB == 256 || (HP && HDB == 128) ? 1 : 2) void
 #pragma unroll
                     for (int r = 0; r < 4; r++) f[r] = __builtin_amdgcn_perm(v[2 * r + 1], v[2 * r], hi ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; n--)
+                    for (int n = NW - 1; n >= 0; n--)
                         o[2 * x + hi] = pa_mfma16<CT>(make_uint4(f[0], f[1], f[2], f[3]),
                                                       make_uint4(pw[0][n], pw[1][n], pw[2][n], pw[3][n]), o[2 * x + hi]);
                 }

@@ -32,14 +32,15 @@ template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, 
 // some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
 // element by element to the queries that do see them.  Rows that no query of the sequence sees (past
 // the length, on unmapped pages) are read as zeros.
-template <int CT, bool HP, int HDB, int NW, int EV>
-__global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1 : 2) void k_pa_prompt(pa_args a)
+template <int CT, bool HP, int HDB, int RG, int KH, int EV>
+__global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG * KH * pa_parts(HDB) == 8 ? 1 : 2) void k_pa_prompt(pa_args a)
 {
     constexpr bool E8 = CT == MLLM_E4M3;
     constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1;
-    constexpr int ROWS = 32 * NW;
-    constexpr int TK = HDB > 128 ? 32 : 64, NB = TK / 32;    // rows per step, in blocks of 32
-    constexpr int KS = HDB / 16, OB = HDB / 32;
+    constexpr int DH = pa_parts(HDB), NW = RG * KH * DH, ROWS = 32 * RG;
+    static_assert(KH == 1 || DH == 1, "a row group has at most two waves");
+    constexpr int TK = HDB > 128 ? 32 : 64, TW = TK / KH, NB = TW / 32;   // rows per step, and of them a wave's, in blocks of 32
+    constexpr int KS = HDB / 16, OB = HDB / 32 / DH;         // K's operands per row, V's (of a wave's columns)
     constexpr int RB = HDB * 2;                              // bytes of a row in LDS
     constexpr int LPR = HDB * ES / 16, RI = 64 / LPR, WR = TK / NW, NI = WR / RI;   // lanes per row, rows per load, rows and loads per wave
     constexpr int NBUF = E8 ? 2 : PA_NBUF;                   // buffers: steps in flight and the one at work
@@ -48,7 +49,7 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     __shared__ __attribute__((aligned(1024))) uint8_t k3[NBUF > 3 ? TK * RB : 16], v3[NBUF > 3 ? TK * RB : 16];
     __shared__ uint32_t odd[2][NW];                          // of a wave's rows of V: those that hold an infinity or a NaN
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hh = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), rg = w % RG, kh = KH > 1 ? w / RG : 0, dh = DH > 1 ? w / RG : 0;
     const int NKH = a.kv.n_kv_head, j = blockIdx.x % NKH, HD = a.kv.head_dim, sp = blockIdx.y, rep = a.rep;
 
     auto start = [&](int x) { return max(0, min(a.starts[x], a.T)); };
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     int t = blockIdx.x / NKH, b = -1, tiles = 0;
     for (int b0 = 0; b0 < a.B && b < 0; b0 += 64) {
         const int bb = b0 + lane;
-        const int n = bb < a.B ? (int)(((long)max(0, start(bb + 1) - start(bb)) * rep + ROWS - 1) / ROWS) : 0;
+        const int n = bb < a.B ? (max(0, start(bb + 1) - start(bb)) * rep + ROWS - 1) / ROWS : 0;
         int sum = n;
         for (int d = 1; d < 64; d <<= 1) {
             const int y = __shfl_up(sum, d, 64);
@@ -80,25 +81,25 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     const int len0 = min(a.lens[b], a.max_len);
     int len = seq >= 0 && seq < a.kv.n_seqs ? len0 : 0;
     len = min(len, (int)min((long)a.kv.max_blocks * a.kv.page_size, 0x7FFFFFFFl));
-    const int nrows = (int)min((long)ROWS, (long)nq * rep - (long)tile * ROWS);      // of the tile
-    const int first = (int)((long)tile * ROWS / rep), last = (int)(((long)tile * ROWS + nrows - 1) / rep);   // tokens
+    const int nrows = min(ROWS, nq * rep - tile * ROWS);     // of the tile (queries times heads are below 2^30)
+    const int first = (unsigned)(tile * ROWS) / (unsigned)rep, last = (unsigned)(tile * ROWS + nrows - 1) / (unsigned)rep;   // tokens
     // positions of a token's query: len0 - nq + token; it sees (p - window, p]
     const int off = len0 - nq;
     const int lo = a.window > 0 ? max(0, off + first - a.window + 1) : 0, hi = min(len, off + last + 1);
     const int begin = lo / TK * TK + sp * a.chunk, end = min(hi, begin + a.chunk);
     // this lane's row
-    const int rr = 32 * w + c, r = min(rr, nrows - 1), tok = (int)(((long)tile * ROWS + r) / rep), h = j * rep + (int)(((long)tile * ROWS + r) - (long)tok * rep);
+    const int rr = 32 * rg + c, r = min(rr, nrows - 1), tok = (int)((unsigned)(tile * ROWS + r) / (unsigned)rep), h = j * rep + (int)((tile * ROWS + r) - tok * rep);
     const int pr = off + tok, lr = a.window > 0 ? max(0, pr - a.window + 1) : 0;
     // The rows that all of the workgroup's queries see, [full_begin, full_end); of the wave's: those that some
     // sees, [lmin, pmax], and that all see, [lmax, wave_end)
     const int full_begin = a.window > 0 ? off + last - a.window + 1 : 0, full_end = min(off + first + 1, len);
-    const int wtok0 = (int)(((long)tile * ROWS + min(32 * w, nrows - 1)) / rep), wtok1 = (int)(((long)tile * ROWS + min(32 * w + 31, nrows - 1)) / rep);
-    const int pmax = 32 * w < nrows ? off + wtok1 : -1, lmax = a.window > 0 ? max(0, off + wtok1 - a.window + 1) : 0;
+    const int wtok0 = (int)((unsigned)(tile * ROWS + min(32 * rg, nrows - 1)) / (unsigned)rep), wtok1 = (int)((unsigned)(tile * ROWS + min(32 * rg + 31, nrows - 1)) / (unsigned)rep);
+    const int pmax = 32 * rg < nrows ? off + wtok1 : -1, lmax = a.window > 0 ? max(0, off + wtok1 - a.window + 1) : 0;
     const int lmin = a.window > 0 ? max(0, off + wtok0 - a.window + 1) : 0, wave_end = min(off + wtok0 + 1, len);
     const long orow = (long)(q0 + tok) * a.NH + h;
 
     if (begin >= end && a.splits > 1) {
-        if (hh == 0 && rr < nrows) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(kLowest, 0.0f);
+        if (hh == 0 && kh == 0 && dh == 0 && rr < nrows) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(kLowest, 0.0f);
         return;
     }
 
@@ -272,8 +273,8 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
     f32x16 o[OB] = {};
     const int tr = (lane & 15) >> 2;                         // V operand: row of four, 8-byte piece of 32 bytes
     // K operand: row c (+ 32 n), piece 2 s + hh; V operand: row 4 hh + tr (+ 16 t, + 8), columns 32 x + 16 (lane / 16 % 2) + 4 (lane % 4)
-    const int kbase = c * RB, kxor = kx(c);
-    const int vbase = (4 * hh + tr) * RB + 8 * (lane & 1), vpc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vxor = vx(4 * hh + tr);
+    const int kbase = (TW * kh + c) * RB, kxor = kx(c);
+    const int vbase = (TW * kh + 4 * hh + tr) * RB + 8 * (lane & 1), vpc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vxor = vx(4 * hh + tr);
 
     auto work = [&](int s0, bool holes, uint8_t *kl, uint8_t *vl, int par) __attribute__((always_inline)) {
         // some row of the workgroup's is masked somewhere in this step
@@ -307,9 +308,10 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
                 __syncthreads();
             }
         }
-        if (s0 > pmax || s0 + TK <= lmin) return;            // nothing that the wave's rows see
+        const int sw = s0 + TW * kh;                         // the wave's rows of K and V
+        if (sw > pmax || sw + TW <= lmin) return;            // nothing that the wave's queries see
         // Operands are read from LDS ahead of the products that take them: K's two products' worth (KD), V's
-        // a group of OB; the scheduler is held to that order, or it reads each right before its use.
+        // a group of VG; the scheduler is held to that order, or it reads each right before its use.
         constexpr int KD = KS < 2 ? 1 : 2;
         f32x16 s[NB] = {};
         uint4 kf[KD + 1][NB];
@@ -320,13 +322,14 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
         };
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4 *lptr;
-        uint2 vf[2][OB][2];
-        auto read_v = [&](int y) __attribute__((always_inline)) {
+        constexpr int VG = OB < 4 ? OB : 4, VS = OB / VG;    // V's operands per group, groups per 16 rows
+        uint2 vf[2][VG][2];
+        auto read_v = [&](int z) __attribute__((always_inline)) {
 #pragma unroll
-            for (int x = 0; x < OB; x++) {
-                const uint8_t *va = vl + vbase + 16 * y * RB + 16 * ((4 * x + vpc) ^ vxor);
-                vf[y & 1][x][0] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)va));
-                vf[y & 1][x][1] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(va + 8 * RB)));
+            for (int x = 0; x < VG; x++) {
+                const uint8_t *va = vl + vbase + 16 * (z / VS) * RB + 16 * ((4 * (OB * dh + VG * (z % VS) + x) + vpc) ^ vxor);
+                vf[z & 1][x][0] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)va));
+                vf[z & 1][x][1] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(va + 8 * RB)));
             }
         };
 #pragma unroll
@@ -344,16 +347,16 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
 #pragma unroll
         for (int y = 0; y < KS; y++) {
             if (y + KD < KS) __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
-            if (y + KD == KS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * OB, 0);
+            if (y + KD == KS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * VG, 0);
             __builtin_amdgcn_sched_group_barrier(0x8, NB * NP, 0);
         }
         float top = -INFINITY;
-        if (s0 + TK > wave_end || s0 < lmax || (EV < 2 && holes)) {
+        if (sw + TW > wave_end || sw < lmax || (EV < 2 && holes)) {
             asm volatile("");                                // a branch: the selects are for the few edges
-            const int u = min(pr, len - 1) - s0 - 4 * hh, v = lr - s0 - 4 * hh;
+            const int u = min(pr, len - 1) - sw - 4 * hh, v = lr - sw - 4 * hh;
             uint64_t bits = ~0ull;
             if (EV < 2 && holes) bits = mapped(s0, look(s0));
-            bits >>= 4 * hh;
+            bits >>= TW * kh + 4 * hh;
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
@@ -379,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
         }
         const float mb = kBias<CT> - m;
 #pragma unroll
-        for (int y = 0; y < TK / 16; y++) {
+        for (int y = 0; y < TW / 16; y++) {
             uint32_t p[4][NP];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -392,24 +395,29 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
                 float &l = e & 1 ? l1 : l0;
                 l += u + v;
             }
-            if (y + 1 < TK / 16) read_v(y + 1);
 #pragma unroll
-            for (int x = 0; x < OB; x++) {
-                const uint2 f0 = vf[y & 1][x][0], f1 = vf[y & 1][x][1];
+            for (int g = 0; g < VS; g++) {
+                const int z = VS * y + g;
+                if (z + 1 < VS * TW / 16) read_v(z + 1);
 #pragma unroll
-                for (int n = NP - 1; n >= 0; n--)
-                    o[x] = pa_mfma32<CT>(make_uint4(f0.x, f0.y, f1.x, f1.y), make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]), o[x]);
+                for (int x = 0; x < VG; x++) {
+                    const uint2 f0 = vf[z & 1][x][0], f1 = vf[z & 1][x][1];
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; n--)
+                        o[VG * g + x] = pa_mfma32<CT>(make_uint4(f0.x, f0.y, f1.x, f1.y), make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]), o[VG * g + x]);
+                }
             }
         }
 #pragma unroll
-        for (int y = 0; y < TK / 16; y++) {
-            if (y + 1 < TK / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2 * OB, 0);
-            __builtin_amdgcn_sched_group_barrier(0x8, OB * NP, 0);
+        for (int z = 0; z < VS * TW / 16; z++) {
+            if (z + 1 < VS * TW / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2 * VG, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, VG * NP, 0);
         }
+        if constexpr (KH > 1) bad = bad >> (TW * kh) & 0xFFFFFFFFull;
         while (bad) {                                        // rare: V rows that were cleared
             const int x = __builtin_ctzll(bad);
             bad &= bad - 1;
-            const int pos = s0 + x, blk = pa_block(a, pos);
+            const int pos = sw + x, blk = pa_block(a, pos);
             const int pg = blk < a.kv.max_blocks ? pa_table(a, seq, blk) : -1;
             if (pos >= len || pg < 0 || pg >= a.kv.n_pages) continue;
             float p = 0.0f;
@@ -428,7 +436,7 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
                 for (int y = 0; y < OB; y++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const int d = 32 * y + 8 * (e >> 2) + 4 * hh + (e & 3);
+                        const int d = 32 * (OB * dh + y) + 8 * (e >> 2) + 4 * hh + (e & 3);
                         float z;
                         if (d >= HD) z = 0.0f;
                         else if constexpr (E8) z = __builtin_amdgcn_cvt_f32_fp8(vr[d], 0) * f;
@@ -492,33 +500,61 @@ __global__ __launch_bounds__(64 * NW, HP && HDB > 64 || HDB > 128 || NW == 8 ? 1
         }
         __builtin_amdgcn_s_waitcnt(0x0F70);                  // no load may still be on its way into LDS at the end
     }
-    if (rr >= nrows) return;
     float l = l0 + l1;
+    if constexpr (KH == 2) {
+        // the two halves of the rows of K and V: the second waves' sums through the buffers of the steps
+        __shared__ float hm[RG][64], hl[RG][64];
+        __syncthreads();
+        f32x4 *to = (f32x4 *)(rg == 0 ? k0 : rg == 1 ? v0 : rg == 2 ? k1 : v1);
+        if (kh) {
+            hm[rg][lane] = m;
+            hl[rg][lane] = l;
+#pragma unroll
+            for (int x = 0; x < OB; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) to[(4 * x + e) * 64 + lane] = f32x4{o[x][4 * e], o[x][4 * e + 1], o[x][4 * e + 2], o[x][4 * e + 3]};
+        }
+        __syncthreads();
+        if (kh) return;
+        const float n = hm[rg][lane], top = fmaxf(m, n), f = __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(n - top);
+        m = top;
+        l = l * f + hl[rg][lane] * g;
+#pragma unroll
+        for (int x = 0; x < OB; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const f32x4 y = to[(4 * x + e) * 64 + lane];
+#pragma unroll
+                for (int z = 0; z < 4; z++) o[x][4 * e + z] = o[x][4 * e + z] * f + y[z] * g;
+            }
+    }
+    if (rr >= nrows) return;
     l += __shfl_xor(l, 32, 64);
 #pragma unroll
     for (int x = 0; x < OB; x++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int d = 32 * x + 8 * e + 4 * hh;
+            const int d = 32 * (OB * dh + x) + 8 * e + 4 * hh;
             if (d >= HD) continue;
             const float4 y = make_float4(o[x][4 * e], o[x][4 * e + 1], o[x][4 * e + 2], o[x][4 * e + 3]);
             if (a.splits > 1) *(float4 *)(a.part + (orow * a.splits + sp) * HD + d) = y;
             else pa_finish(a, h, q0 + tok, d, m, l, y);
         }
-    if (a.splits > 1 && hh == 0) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(m, l);
+    if (a.splits > 1 && hh == 0 && dh == 0) *(float2 *)(a.stat + (orow * a.splits + sp) * 2) = make_float2(m, l);
 }
 
-template <int CT, bool HP, int HDB, int NW, int EV> static void pa_prompt_ev(const pa_args &a, hipStream_t st)
+template <int CT, bool HP, int HDB, int RG, int KH, int EV> static void pa_prompt_ev(const pa_args &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB, NW, EV>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((k_pa_prompt<CT, HP, HDB, RG, KH, EV>), dim3(a.tiles * a.kv.n_kv_head, a.splits), dim3(64 * RG * KH * pa_parts(HDB)), 0, st, a);
 }
 template <int CT, bool HP, int HDB> static void pa_prompt_go(const pa_args &a, bool uniform, hipStream_t st)
 {
-    if constexpr (!HP && (HDB == 128 || HDB == 64 && CT != MLLM_E4M3))
-        if (a.waves == 8) return pa_prompt_ev<CT, HP, HDB, 8, 2>(a, st);
-    if (!uniform) pa_prompt_ev<CT, HP, HDB, 4, 0>(a, st);
-    else if (a.kv.page_size % 64) pa_prompt_ev<CT, HP, HDB, 4, 1>(a, st);
-    else pa_prompt_ev<CT, HP, HDB, 4, 2>(a, st);
+    constexpr int RG = pa_row_groups(CT, HP, HDB), KH = pa_halves(CT, HP, HDB);
+    if constexpr (KH == 2 && RG == 4)
+        if (a.groups == 8) return pa_prompt_ev<CT, HP, HDB, 8, 1, 2>(a, st);
+    if (!uniform) pa_prompt_ev<CT, HP, HDB, RG, KH, 0>(a, st);
+    else if (a.kv.page_size % 64) pa_prompt_ev<CT, HP, HDB, RG, KH, 1>(a, st);
+    else pa_prompt_ev<CT, HP, HDB, RG, KH, 2>(a, st);
 }
 template <int CT, bool HP> static void pa_prompt_hd(const pa_args &a, bool uniform, hipStream_t st)
 {
