@@ -108,6 +108,9 @@ constexpr int pa_halves(int type, bool wide, int hdb) { return hdb > 128 || (!wi
 void pa_decode_bf16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_f16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
 void pa_decode_e4m3(const pa_args &a, bool wide, bool uniform, hipStream_t st);
-void pa_prompt_bf16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
-void pa_prompt_f16(const pa_args &a, bool wide, bool uniform, hipStream_t st);
-void pa_prompt_e4m3(const pa_args &a, bool wide, bool uniform, hipStream_t st);
+void pa_prompt_bf16(const pa_args &a, bool uniform, hipStream_t st);
+void pa_prompt_f16(const pa_args &a, bool uniform, hipStream_t st);
+void pa_prompt_e4m3(const pa_args &a, bool uniform, hipStream_t st);
+void pa_prompt_wide_bf16(const pa_args &a, bool uniform, hipStream_t st);
+void pa_prompt_wide_f16(const pa_args &a, bool uniform, hipStream_t st);
+void pa_prompt_wide_e4m3(const pa_args &a, bool uniform, hipStream_t st);

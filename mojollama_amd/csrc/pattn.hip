@@ -163,9 +163,10 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         a.chunk = a.splits == 1 ? 1 << 30 : (int)((n + 64l * a.splits - 1) / (64l * a.splits) * 64);
         if (a.splits > 1) a.splits = (int)((n + a.chunk - 1) / a.chunk);
         if (!pa_partials(a, ws, ws_bytes)) return pk_fail(who, "workspace below what the splits take");
-        if (a.kv.type == MLLM_F16) pa_prompt_f16(a, wide, uniform, st);
-        else if (a.kv.type == MLLM_BF16) pa_prompt_bf16(a, wide, uniform, st);
-        else pa_prompt_e4m3(a, wide, uniform, st);
+        auto go = a.kv.type == MLLM_F16 ? wide ? pa_prompt_wide_f16 : pa_prompt_f16
+                : a.kv.type == MLLM_BF16 ? wide ? pa_prompt_wide_bf16 : pa_prompt_bf16
+                                         : wide ? pa_prompt_wide_e4m3 : pa_prompt_e4m3;
+        go(a, uniform, st);
     }
     if (a.splits > 1) hipLaunchKernelGGL(k_pa_join, dim3(a.T, a.NH, (a.kv.head_dim + 63) / 64), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed");

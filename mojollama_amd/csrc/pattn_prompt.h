@@ -1,8 +1,5 @@
 // pattn_prompt.h — the tiled prompt kernel over a paged cache, instantiated per cache type.
 #pragma once
-#ifndef PA_NBUF
-#define PA_NBUF 2
-#endif
 #include <math.h>
 #include <type_traits>
 #include "pattn.h"
@@ -43,10 +40,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
     constexpr int KS = HDB / 16, OB = HDB / 32 / DH;         // K's operands per row, V's (of a wave's columns)
     constexpr int RB = HDB * 2;                              // bytes of a row in LDS
     constexpr int LPR = HDB * ES / 16, RI = 64 / LPR, WR = TK / NW, NI = WR / RI;   // lanes per row, rows per load, rows and loads per wave
-    constexpr int NBUF = E8 ? 2 : PA_NBUF;                   // buffers: steps in flight and the one at work
     __shared__ __attribute__((aligned(1024))) uint8_t k0[TK * RB], v0[TK * RB], k1[TK * RB], v1[TK * RB];
-    __shared__ __attribute__((aligned(1024))) uint8_t k2[NBUF > 2 ? TK * RB : 16], v2[NBUF > 2 ? TK * RB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t k3[NBUF > 3 ? TK * RB : 16], v3[NBUF > 3 ? TK * RB : 16];
     __shared__ uint32_t odd[2][NW];                          // of a wave's rows of V: those that hold an infinity or a NaN
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hh = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), rg = w % RG, kh = KH > 1 ? w / RG : 0, dh = DH > 1 ? w / RG : 0;
@@ -448,11 +442,8 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
     };
 
     if (begin < end) {
-        // Before its barrier a wave waits until its loads of the step have landed and its reads of the buffer
-        // that is filled next have returned.  Its younger loads, those of the steps in flight, may stay out: the
-        // count holds as every fetch issues 2 NI loads; any other load in between makes the wait stricter.
-        constexpr int D = NBUF - 1, YOUNG = E8 ? 0 : 2 * NI * (D - 1);
-        static_assert(YOUNG < 64, "vmcnt is six bits");
+        // Before its barrier a wave waits until its loads of the step have landed and its reads of the buffer that
+        // is filled next have returned.
         uint32_t holes = 0;                                  // per buffer: some row is on no page
         pages g = look(begin);
         auto bring = [&](int s0, uint8_t *kl, uint8_t *vl, int buf) __attribute__((always_inline)) {
@@ -469,34 +460,21 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
             }
         };
         auto step = [&](int s0, uint8_t *kl, uint8_t *vl, int buf, uint8_t *kn, uint8_t *vn, int next) __attribute__((always_inline)) {
-            __builtin_amdgcn_s_waitcnt((YOUNG & 15) | ((YOUNG >> 4) << 14) | 0x0070);
+            __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0), lgkmcnt(0)
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
-            bring(s0 + D * TK, kn, vn, next);
+            bring(s0 + TK, kn, vn, next);
             work(s0, holes >> buf & 1, kl, vl, buf & 1);
             store(kn, vn);
             return s0 + TK < end;
         };
         bring(begin, k0, v0, 0);
         store(k0, v0);
-        if constexpr (NBUF > 2) bring(begin + TK, k1, v1, 1);
-        if constexpr (NBUF > 3) bring(begin + 2 * TK, k2, v2, 2);
-        for (int s0 = begin;; s0 += NBUF * TK) {
-            if constexpr (NBUF == 2) {
-                if (!step(s0, k0, v0, 0, k1, v1, 1)) break;
-                if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
-            } else if constexpr (NBUF == 3) {
-                if (!step(s0, k0, v0, 0, k2, v2, 2)) break;
-                if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
-                if (!step(s0 + 2 * TK, k2, v2, 2, k1, v1, 1)) break;
-            } else {
-                if (!step(s0, k0, v0, 0, k3, v3, 3)) break;
-                if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
-                if (!step(s0 + 2 * TK, k2, v2, 2, k1, v1, 1)) break;
-                if (!step(s0 + 3 * TK, k3, v3, 3, k2, v2, 2)) break;
-            }
+        for (int s0 = begin;; s0 += 2 * TK) {
+            if (!step(s0, k0, v0, 0, k1, v1, 1)) break;
+            if (!step(s0 + TK, k1, v1, 1, k0, v0, 0)) break;
         }
         __builtin_amdgcn_s_waitcnt(0x0F70);                  // no load may still be on its way into LDS at the end
     }
@@ -556,13 +534,9 @@ template <int CT, bool HP, int HDB> static void pa_prompt_go(const pa_args &a, b
     else if (a.kv.page_size % 64) pa_prompt_ev<CT, HP, HDB, RG, KH, 1>(a, st);
     else pa_prompt_ev<CT, HP, HDB, RG, KH, 2>(a, st);
 }
-template <int CT, bool HP> static void pa_prompt_hd(const pa_args &a, bool uniform, hipStream_t st)
+template <int CT, bool HP> static void pa_prompt(const pa_args &a, bool uniform, hipStream_t st)
 {
     const int HD = a.kv.head_dim;
     HD <= 64 ? pa_prompt_go<CT, HP, 64>(a, uniform, st) : HD <= 128 ? pa_prompt_go<CT, HP, 128>(a, uniform, st)
                                                                     : pa_prompt_go<CT, HP, 256>(a, uniform, st);
-}
-template <int CT> static void pa_prompt(const pa_args &a, bool wide, bool uniform, hipStream_t st)
-{
-    wide ? pa_prompt_hd<CT, true>(a, uniform, st) : pa_prompt_hd<CT, false>(a, uniform, st);
 }
