@@ -511,7 +511,7 @@ MLLM_API int mllm_rotary_freqs(int scaling, int rope_dim, double base, double fa
  * the types and strides are the same; other overlaps are not supported.  A
  * token with pos < 0 is left out (its outputs keep their contents); one whose
  * sequence or row is outside the tables, or on an unmapped page, is not
- * stored.  in_type and out_type: MLLM_F32, _F16, _BF16.  To an MLLM_E4M3 cache
+ * stored; no two tokens of a call go to one row.  in_type and out_type: MLLM_F32, _F16, _BF16.  To an MLLM_E4M3 cache
  * a row is rounded once, from 64 bits, under the least 2^e, -100 <= e <= 100,
  * that brings its largest element to 448 or below (e = 0 for a row of zeros; a
  * row that holds an infinity or a NaN takes e = 0, those elements become NaN
@@ -526,7 +526,8 @@ MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void 
  *   out = sum_s exp(z_s) v_s / (sum_s exp(z_s) + exp(sinks[h])), z_s = scale * q . k_s,
  * over the mapped rows s <= p that the query at position p sees, with window
  * w > 0 only those of s > p - w (the sink's term only where sinks is given,
- * fp32 [NH]).  A query that sees no row gives zeros.  lens[i] (device) is the
+ * fp32 [NH]).  A query that sees no row gives zeros; what rows hold that a query
+ * does not see, NaN too, has no part in its result.  scale is finite.  lens[i] (device) is the
  * number of cached rows of the i-th sequence, the new tokens' own among them;
  * it is taken as at most max_len.  The i-th sequence reads table row seqs[i]
  * (NULL: i); one outside the tables has no rows.

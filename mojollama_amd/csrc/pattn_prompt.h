@@ -12,9 +12,11 @@ template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, 
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
 }
 
-// 128 rows of queries against the rows of one kv head, 64 of these at a time (32 at head sizes
-// above 128).  A row is a (token, head) pair of the heads that share the kv head, tokens outer, so a
-// tile of K and V serves all of them and a few drafted tokens fill a wave; each of four waves owns 32.
+// A tile of 64, 128 or 256 rows of queries against the rows of one kv head, 64 of these at a time (32 at
+// head sizes above 128).  A row is a (token, head) pair of the heads that share the kv head, tokens outer,
+// so a tile of K and V serves all of them and a few drafted tokens fill a wave.  RG groups of 32 rows; a
+// group is one wave's, or two waves share it: KH, each takes half of every step's rows of K and V, and
+// they join at the end; above head size 128, each takes half of the output's columns.
 //   S^T = K Q^T   (32x32x16): q stays in registers as the second operand; a lane holds half of the
 //                 scores of one row (lane % 32), so maximum and sum are the lane's own
 //   O^T += V^T P  the scores' registers are this product's second operand as they stand: slot
@@ -25,10 +27,23 @@ template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, 
 // lanes (K: 16 rows; V: 4 rows of 64 bytes) fall on distinct banks.  8-bit caches pass through
 // registers, where they become bf16.
 //
-// A weight of 0 times an infinity or a NaN that a masked row of V holds is NaN, so in the tiles where
+// HP (fp32 q or out): q and the weights in planes that hold fp32's precision, three products for one (two
+// in fp16).  Else both are 16 bits: a weight's rounding is as large as the output's own (the error against
+// 64 bits is 1.4 times that of the output rounded alone), and a second plane would add half of the
+// matrix instructions to a kernel that they bound.
+//
+// A weight of 0 times an infinity or a NaN that a masked row of V holds is NaN, so in the steps where
 // some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
-// element by element to the queries that do see them.  Rows that no query of the sequence sees (past
-// the length, on unmapped pages) are read as zeros.
+// element by element to the queries that do see them.
+//
+// One prompt of 6011 tokens, 32/8 heads of 128, bf16: 323 us, 916 TFLOP/s (a bf16 product of 8192^3 reaches
+// 1288 on this card).  Per step of 32 x 64 scores a wave issues 32 matrix instructions (1024 cycles) and about
+// 190 others (32 exponentials among them, at a quarter of the rate), and the two do not overlap on a SIMD
+// (matrix cores busy 34 to 38 % of the time, the vector unit as much): 4300 cycles for the two waves of a SIMD of
+// 4900 measured; prologue and epilogue are 11 %.  Three or four buffers instead of two 1 to 2 % slower (the loads
+// are hidden by then), 32-row steps 6 %, the sum of the weights by v_dot2 16 % (it issues slowly), scores two
+// waves a SIMD without the order of LDS reads fixed below 10 %, the page looked up by a vector load 5 %, matrix
+// instructions at a higher wave priority 1 % faster or slower.
 template <int CT, bool HP, int HDB, int RG, int KH, int EV>
 __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG * KH * pa_parts(HDB) == 8 ? 1 : 2) void k_pa_prompt(pa_args a)
 {
@@ -116,6 +131,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
             e = big > 0.0f && big < INFINITY ? 15 - (int)((__float_as_uint(big) >> 23) & 255) + 126 : 0;
             zs = ldexpf(zs, -e);
         }
+        zs = fmaxf(zs, 1e-37f);                              // masked scores, -inf, times it stay -inf
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const int col = 16 * s + 8 * hh;

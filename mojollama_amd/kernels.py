@@ -472,6 +472,12 @@ class DeviceOps:
     def _elsewhere(self, t, what):
         raise ValueError(f"{what}: a tensor on {t.device}, not on the current GPU")
 
+    @staticmethod
+    def _made_here(cur, *handles):
+        for h in handles:
+            if h is not None and h._device != cur:
+                raise ValueError(f"a {type(h).__name__} of GPU {h._device}, not of the current one")
+
     def _ints(self, t, what, cur, n=None):
         """Address of a dense int32 tensor on the current GPU (None: a null pointer)."""
         if t is None:
@@ -507,7 +513,7 @@ class DeviceOps:
         p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         view = PagedKV(code, heads, hd, n_pages, page, p(k), p(v), p(k_exp), p(v_exp), k.stride(0), k.stride(1),
                        k.stride(2), p(tables), tables.shape[0], tables.shape[1], tables.stride(0))
-        view._tensors = (k, v, tables, k_exp, v_exp)
+        view._tensors, view._device = (k, v, tables, k_exp, v_exp), cur
         return view
 
     def rotary(self, rope_dim, layout=ROPE_HALF, base=10000.0, scaling=ROPE_NONE, factor=1.0, ctx=0.0, beta_fast=0.0,
@@ -518,7 +524,7 @@ class DeviceOps:
                                               ctypes.byref(m)), "mllm_rotary_freqs")
         freqs = self.torch.tensor(list(f), dtype=self.torch.float64).cuda()
         rot = Rotary(layout, rope_dim, freqs.data_ptr(), m.value)
-        rot._tensors = (freqs,)
+        rot._tensors, rot._device = (freqs,), self._cur()
         return rot
 
     def rotary_append(self, rot, q, k, v, pos, NH=0, NKH=0, HD=0, kv=None, seqs=None, rows=None, q_out=None, k_out=None):
@@ -526,6 +532,7 @@ class DeviceOps:
         and v, may be None), pos int32 [T]; k and v go to rows `rows` (None: pos) of sequences `seqs` (None: 0, 1, ...)
         of kv, the turned q to q_out and k to k_out.  Heads and head size come from kv where it is given."""
         cur = self._cur()
+        self._made_here(cur, rot, kv)
         pp, T = self._ints(pos, "pos", cur), pos.numel()
         if kv is not None:
             NKH, HD = kv.n_kv_head, kv.head_dim
@@ -558,6 +565,7 @@ class DeviceOps:
         return self.torch.empty(n, dtype=self.torch.uint8, device="cuda")
 
     def _attn(self, kv, q, T, B, NH, max_len, window, sinks, out, out_dtype, ws, cur):
+        self._made_here(cur, kv)
         n = NH * kv.head_dim
         qt, qp, ql = self._rows(q, "q", T, n, cur, None)
         if out is None:
@@ -609,7 +617,7 @@ class DeviceOps:
             raise ValueError("tables: int32 [n_seqs, max_blocks], rows dense")
         m = PageMap(tables.data_ptr(), tables.shape[0], tables.shape[1], tables.stride(0), self._ints(refs, "refs", cur),
                     refs.numel(), page_size)
-        m._tensors = (tables, refs)
+        m._tensors, m._device = (tables, refs), cur
         return m
 
     def page_planes(self, pools):
@@ -624,6 +632,7 @@ class DeviceOps:
             p.base, p.n_layers = t.data_ptr(), t.shape[0]
             p.page_bytes, p.layer_bytes = t.stride(1) * t.element_size(), t.stride(0) * t.element_size()
         planes._tensors, planes._n_pages = tuple(pools), min((t.shape[1] for t in pools), default=None)
+        planes._device = self._cur()
         return planes
 
     def pages_workspace(self, m, n):
@@ -632,6 +641,7 @@ class DeviceOps:
 
     def _pages_args(self, m, n, status, ws, cur):
         torch = self.torch
+        self._made_here(cur, m)
         if status is None:
             status = torch.empty(1, dtype=torch.int32, device="cuda")
         if ws is None:
@@ -640,8 +650,8 @@ class DeviceOps:
             self._elsewhere(ws, "workspace")
         return status, self._ints(status, "status", cur, 1), ws
 
-    @staticmethod
-    def _pages_in(planes, n_pages):
+    def _pages_in(self, planes, n_pages, cur):
+        self._made_here(cur, planes)
         if planes._n_pages is not None and planes._n_pages < n_pages:
             raise ValueError(f"a pool holds {planes._n_pages} pages, not {n_pages}")
 
@@ -658,13 +668,14 @@ class DeviceOps:
     def pages_free(self, m, seqs, lens=None):
         """mllm_pages_free: sequences seqs[i] give back their pages past the first lens[i] rows (None: all)."""
         n, cur = seqs.numel(), self._cur()
-        self._check(self.so.mllm_pages_free(m, n, self._ints(seqs, "seqs", cur), self._ints(lens, "lens", cur, n), self._raw_stream(cur)),
-                    "mllm_pages_free")
+        self._made_here(cur, m)
+        self._check(self.so.mllm_pages_free(m, n, self._ints(seqs, "seqs", cur), self._ints(lens, "lens", cur, n),
+                                            self._raw_stream(cur)), "mllm_pages_free")
 
     def pages_fork(self, m, planes, parents, children, lens, status=None, ws=None):
         """mllm_pages_fork: children[i] takes over the first lens[i] rows of parents[i], all at once; returns status."""
         n, cur = parents.numel(), self._cur()
-        self._pages_in(planes, m.n_pages)
+        self._pages_in(planes, m.n_pages, cur)
         status, sp, ws = self._pages_args(m, n, status, ws, cur)
         self._check(self.so.mllm_pages_fork(m, planes, len(planes), n, self._ints(parents, "parents", cur),
                                             self._ints(children, "children", cur, n), self._ints(lens, "lens", cur, n), sp,
@@ -675,7 +686,7 @@ class DeviceOps:
     def pages_compact(self, m, planes, status=None, ws=None):
         """mllm_pages_compact: the live pages move to the front; returns their number (a device int32)."""
         cur = self._cur()
-        self._pages_in(planes, m.n_pages)
+        self._pages_in(planes, m.n_pages, cur)
         status, sp, ws = self._pages_args(m, 0, status, ws, cur)
         self._check(self.so.mllm_pages_compact(m, planes, len(planes), sp, ws.data_ptr(),
                                                ws.nbytes, self._raw_stream(cur)), "mllm_pages_compact")
@@ -684,7 +695,7 @@ class DeviceOps:
     def pages_copy(self, planes, n_pages, src, dst):
         """mllm_pages_copy: page dst[i] := page src[i] in every plane."""
         n, cur = src.numel(), self._cur()
-        self._pages_in(planes, n_pages)
+        self._pages_in(planes, n_pages, cur)
         self._check(self.so.mllm_pages_copy(planes, len(planes), n_pages, n, self._ints(src, "src", cur),
                                             self._ints(dst, "dst", cur, n), self._raw_stream(cur)), "mllm_pages_copy")
 

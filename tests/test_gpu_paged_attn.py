@@ -129,7 +129,8 @@ def test_decode_extreme_scores(dev):
 
 
 # ------------------------------------------------------------------ prompt
-def prompt(dev, cache, new, NH, q_dtype, out_dtype, window=0, sinks=None, seqs=None, behind=0, lens=None, seed=0):
+def prompt(dev, cache, new, NH, q_dtype, out_dtype, window=0, sinks=None, seqs=None, behind=0, lens=None, scale=None,
+           shrink=1.0, seed=0):
     """Sequence i's last new[i] rows are its new tokens; `behind` rows of q and out behind the last sequence."""
     HD, B = cache.HD, len(new)
     slots = list(range(B)) if seqs is None else seqs
@@ -138,18 +139,19 @@ def prompt(dev, cache, new, NH, q_dtype, out_dtype, window=0, sinks=None, seqs=N
     for n in new:
         starts.append(starts[-1] + n)
     T = starts[-1] + behind
-    q = queries(seed, T, NH, HD, q_dtype)
+    q = (queries(seed, T, NH, HD, F32) * shrink).to(q_dtype)
+    scale = HD ** -0.5 if scale is None else scale
     if sinks is not None:
         sinks = torch.randn(NH, generator=torch.Generator().manual_seed(seed + 1)) * 3
     i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
     out = torch.full((T, NH * HD), 7.0, dtype=out_dtype, device="cuda")
-    dev.paged_attn_prompt(cache.view(dev), q.cuda(), i32(starts), i32(lens), max(lens + [0]), NH, window=window,
+    dev.paged_attn_prompt(cache.view(dev), q.cuda(), i32(starts), i32(lens), max(lens + [0]), NH, scale=scale, window=window,
                           sinks=None if sinks is None else sinks.cuda(), seqs=None if seqs is None else i32(seqs), out=out)
     assert (out[starts[-1]:] == 7).all()
     for i, n in enumerate(new):
         if n:
             pos = torch.arange(n) + lens[i] - n
-            check(out[starts[i]:starts[i] + n], cache, slots[i], q[starts[i]:starts[i] + n], pos, HD ** -0.5, window,
+            check(out[starts[i]:starts[i] + n], cache, slots[i], q[starts[i]:starts[i] + n], pos, scale, window,
                   sinks, q_dtype, out_dtype, NH)
 
 
@@ -246,6 +248,29 @@ def test_prompt_long(dev, cache, q):
     prompt(dev, Cache(6, [2100, 4100], 1, 128, 64, cache), [2100, 6], 4, q, q, seed=1)
 
 
+@pytest.mark.parametrize("cache,q", [(BF16, BF16), (F16, F32), (E4M3, F32)])
+@pytest.mark.parametrize("scale,shrink", [(0.0, 1.0), (-0.2, 1.0), (0.125, 1e-30), (0.125, 0.0)])
+def test_scales_and_tiny_queries(dev, cache, q, scale, shrink):
+    """A scale of zero (the mean of the rows), a negative one, queries next to nothing and of zeros."""
+    c = Cache(3, [130, 70], 2, 64, 16, cache)
+    prompt(dev, c, [100, 3], 4, q, q, scale=scale, shrink=shrink, window=90, seed=5)
+    if shrink == 1.0:
+        decode(dev, c, [130, 70], 4, q, q, scale=scale, seed=5)
+
+
+def test_tables_inside_a_wider_tensor(dev):
+    c = Cache(5, [200, 33], 2, 64, 16, BF16)
+    wide = torch.full((2, c.tables.shape[1] + 7), 9999, dtype=torch.int32)
+    wide[:, 3:3 + c.tables.shape[1]] = c.tables
+    t = wide.cuda()[:, 3:3 + c.tables.shape[1]]
+    q = queries(4, 2, 8, 64, BF16)
+    kv = c.view(dev)
+    n = torch.tensor(c.rows, dtype=torch.int32).cuda()
+    a = dev.paged_attn_decode(kv, q.cuda(), n, 200, 8)
+    b = dev.paged_attn_decode(dev.paged_kv(kv._tensors[0], kv._tensors[1], t), q.cuda(), n, 200, 8)
+    assert torch.equal(a, b)
+
+
 def test_decode_is_the_prompt_of_one_token(dev):
     lens = [65, 300, 1]
     c = Cache(1, lens, 2, 64, 64, F16)
@@ -305,5 +330,9 @@ def test_wrapper_refusals(dev):
             dev.paged_attn_decode(kv, **a)
     with pytest.raises(ValueError):
         dev.paged_kv(kv._tensors[0], kv._tensors[1][:, :16], kv._tensors[2])
+    other = c.view(dev)
+    other._device = 1                             # as a view made while another GPU was the current one
+    with pytest.raises(ValueError):
+        dev.paged_attn_decode(other, q, n, 70, 8)
     with pytest.raises(TypeError):
         dev.paged_kv(kv._tensors[0].double(), kv._tensors[1].double(), kv._tensors[2])

@@ -31,17 +31,17 @@ BAD_KV = [dict(type=K.T_F32), dict(type=7), dict(type=K.T_E4M3), dict(head_dim=7
 
 
 def decode(so, v, **c):
-    a = dict(q_type=K.T_BF16, q=P, q_ld=512, seqs=None, lens=P, max_len=60, B=3, NH=8, window=0, out_type=K.T_BF16, out=P,
+    a = dict(q_type=K.T_BF16, q=P, q_ld=512, seqs=None, lens=P, max_len=60, B=3, NH=8, scale=0.1, window=0, out_type=K.T_BF16, out=P,
              out_ld=512, ws=P, n=1 << 40) | c
     return so.mllm_paged_attn_decode(v, a["q_type"], a["q"], a["q_ld"], a["seqs"], a["lens"], a["max_len"], a["B"], a["NH"],
-                                     0.1, a["window"], None, a["out_type"], a["out"], a["out_ld"], a["ws"], a["n"], None)
+                                     a["scale"], a["window"], None, a["out_type"], a["out"], a["out_ld"], a["ws"], a["n"], None)
 
 
 def prompt(so, v, **c):
-    a = dict(q_type=K.T_BF16, q=P, q_ld=512, seqs=None, starts=P, lens=P, max_len=60, T=9, B=3, NH=8, window=0,
+    a = dict(q_type=K.T_BF16, q=P, q_ld=512, seqs=None, starts=P, lens=P, max_len=60, T=9, B=3, NH=8, scale=0.1, window=0,
              out_type=K.T_BF16, out=P, out_ld=512, ws=P, n=1 << 40) | c
     return so.mllm_paged_attn_prompt(v, a["q_type"], a["q"], a["q_ld"], a["seqs"], a["starts"], a["lens"], a["max_len"],
-                                     a["T"], a["B"], a["NH"], 0.1, a["window"], None, a["out_type"], a["out"], a["out_ld"],
+                                     a["T"], a["B"], a["NH"], a["scale"], a["window"], None, a["out_type"], a["out"], a["out_ld"],
                                      a["ws"], a["n"], None)
 
 
@@ -58,7 +58,9 @@ def test_views(so, change):
 
 @pytest.mark.parametrize("c", [dict(q_type=K.T_F16), dict(out_type=K.T_F16), dict(q_type=K.T_E4M3), dict(q=None),
                                dict(out=None), dict(lens=None), dict(q=P + 2), dict(q_ld=504), dict(q_ld=516), dict(out_ld=500),
-                               dict(NH=9), dict(NH=0), dict(B=-1), dict(B=4), dict(max_len=-1), dict(window=-1), dict(ws=None),
+                               dict(NH=9), dict(NH=0), dict(B=-1), dict(B=4), dict(max_len=-1),
+                               dict(max_len=(1 << 30) + 1), dict(window=-1), dict(scale=float("nan")),
+                               dict(scale=float("inf")), dict(ws=None),
                                dict(n=0)])
 def test_attention(so, c):
     assert decode(so, kv(), **c) == -1 and so.mllm_last_error().startswith(b"mllm_paged_attn_decode")
