@@ -511,11 +511,11 @@ MLLM_API int mllm_rotary_freqs(int scaling, int rope_dim, double base, double fa
  * the types and strides are the same; other overlaps are not supported.  A
  * token with pos < 0 is left out (its outputs keep their contents); one whose
  * sequence or row is outside the tables, or on an unmapped page, is not
- * stored; no two tokens of a call go to one row.  in_type and out_type: MLLM_F32, _F16, _BF16.  To an MLLM_E4M3 cache
- * a row is rounded once, from 64 bits, under the least 2^e, -100 <= e <= 100,
- * that brings its largest element to 448 or below (e = 0 for a row of zeros; a
- * row that holds an infinity or a NaN takes e = 0, those elements become NaN
- * and the others saturate). */
+ * stored; no two tokens of a call go to one row.  in_type and out_type:
+ * MLLM_F32, _F16, _BF16.  To an MLLM_E4M3 cache a row is rounded once, from 64
+ * bits, under the least 2^e, -100 <= e <= 100, that brings its largest element
+ * to 448 or below (e = 0 for a row of zeros; a row that holds an infinity or a
+ * NaN takes e = 0, those elements become NaN and the others saturate). */
 MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void *q, long q_ld, const void *k, long k_ld,
                                 const void *v, long v_ld, const int *pos, int T, int NH, int NKH, int HD, int out_type,
                                 void *q_out, long q_out_ld, void *k_out, long k_out_ld, const mllm_paged_kv *kv,
@@ -527,9 +527,9 @@ MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void 
  * over the mapped rows s <= p that the query at position p sees, with window
  * w > 0 only those of s > p - w (the sink's term only where sinks is given,
  * fp32 [NH]).  A query that sees no row gives zeros; what rows hold that a query
- * does not see, NaN too, has no part in its result.  scale is finite.  lens[i] (device) is the
- * number of cached rows of the i-th sequence, the new tokens' own among them;
- * it is taken as at most max_len.  The i-th sequence reads table row seqs[i]
+ * does not see, NaN too, has no part in its result.  scale is finite.  lens[i]
+ * (device) is the number of cached rows of the i-th sequence, the new tokens'
+ * own among them; it is taken as at most max_len.  The i-th sequence reads table row seqs[i]
  * (NULL: i); one outside the tables has no rows.
  *   decode: one query per sequence, at position lens[i] - 1
  *   prompt: sequence i has the queries starts[i] .. starts[i + 1] - 1 (device,
@@ -537,9 +537,10 @@ MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void 
  *           rows of out behind starts[B] are left as they were
  * q [.][NH * HD] with row stride q_ld, out likewise, in q_type and out_type:
  * MLLM_F32 or the cache's own type (MLLM_BF16 for MLLM_E4M3), 16-byte aligned
- * rows.  Scores, softmax and sums are fp32; with 16-bit q and out the weights
- * are rounded to 16 bits for the product with V, with fp32 in either place q
- * and the weights keep fp32's precision.  NH / n_kv_head is not limited.
+ * rows.  Scores, softmax and sums are fp32.  With 16-bit q and out prompt rounds
+ * the weights to 16 bits for the product with V (decode keeps 16 bits of
+ * mantissa and more); with fp32 in either place q and the weights keep fp32's
+ * precision in both.  NH / n_kv_head is not limited.
  * Workspace: mllm_paged_attn_workspace_size bytes (tokens T, for decode B);
  * one for a T, B and max_len serves every smaller one, and calls that overlap
  * need one each.  Results are the same from call to call. */
@@ -579,7 +580,11 @@ MLLM_API long mllm_pages_workspace_size(const mllm_page_map *map, int n);
 /* Sequence seqs[i] gets pages for its unmapped blocks below lens[i] rows. */
 MLLM_API int mllm_pages_reserve(const mllm_page_map *map, int n, const int *seqs, const int *lens, int *status,
                                 void *workspace, long ws_bytes, void *stream);
-/* Sequence seqs[i] gives back its blocks past the first lens[i] rows (lens NULL: all). */
+/* Sequence seqs[i] gives back its blocks past the first lens[i] rows (lens NULL:
+ * all).  The page that row lens[i] - 1 lies in stays as it is: if another
+ * sequence holds it too, what is stored there next is stored for both, so a
+ * sequence cut back into a shared page goes on as a fork of itself (in another
+ * slot), which copies that page. */
 MLLM_API int mllm_pages_free(const mllm_page_map *map, int n, const int *seqs, const int *lens, void *stream);
 /* children[i] takes over the first lens[i] rows of parents[i]: whole pages are
  * shared, a part-filled last one is copied (all planes) to a page of its own,
