@@ -537,10 +537,10 @@ MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void 
  *           rows of out behind starts[B] are left as they were
  * q [.][NH * HD] with row stride q_ld, out likewise, in q_type and out_type:
  * MLLM_F32 or the cache's own type (MLLM_BF16 for MLLM_E4M3), 16-byte aligned
- * rows.  Scores, softmax and sums are fp32.  With 16-bit q and out prompt rounds
- * the weights to 16 bits for the product with V (decode keeps 16 bits of
- * mantissa and more); with fp32 in either place q and the weights keep fp32's
- * precision in both.  NH / n_kv_head is not limited.
+ * rows.  Scores, softmax and sums are fp32.  With 16-bit q and out the weights
+ * keep 16 bits of mantissa (F16 caches: 22) for the product with V; with fp32 in
+ * either place q and the weights keep fp32's precision.  NH / n_kv_head is not
+ * limited.
  * Workspace: mllm_paged_attn_workspace_size bytes (tokens T, for decode B);
  * one for a T, B and max_len serves every smaller one, and calls that overlap
  * need one each.  Results are the same from call to call. */

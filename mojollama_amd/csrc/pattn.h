@@ -99,8 +99,8 @@ __device__ __forceinline__ void pa_finish(const pa_args &a, int h, int t, int d,
 }
 
 // The prompt kernel's tile: groups of 32 rows, and whether two waves share each, one half of every step's
-// rows of K and V for each (two waves a SIMD in small launches: prompts of 1 to 1100 tokens, window 512, 32.2 ->
-// 29.0 us; drafts in fp32 on 64 rows instead of 128, whose waves were half idle, 29.6 -> 26.7).
+// rows of K and V for each (two waves a SIMD in small launches: prompts of 1 to 1100 tokens, window 512, 36.4 ->
+// 33.4 us; drafts in fp32 on 64 rows instead of 128, whose waves were half idle, 29.6 -> 26.7).
 constexpr int pa_row_groups(int type, bool wide, int hdb) { return wide ? 2 : 4; }
 // ... or, at head sizes above 128, the columns of the output: the registers of a wave hold half of them (fp32,
 // fp16 cache, head size 256, 2789 tokens: 403 -> 180 us; the whole of them spilled).

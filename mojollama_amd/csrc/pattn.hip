@@ -152,14 +152,14 @@ int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream
         const int hdb = a.kv.head_dim <= 64 ? 64 : a.kv.head_dim <= 128 ? 128 : 256;
         a.groups = pa_row_groups(a.kv.type, wide, hdb);
         // tiles of 256 rows, half the traffic from L2, where they fill the GPU (6011 tokens, 32/8 heads of 128:
-        // 349 us, of 128 rows 361; below a workgroup per CU they leave CUs without work)
+        // 418 us, of 128 rows 452; below a workgroup per CU they leave CUs without work)
         const bool large = a.groups == 4 && pa_halves(a.kv.type, wide, hdb) == 2 && uniform && a.kv.page_size % 64 == 0 &&
                            rows / 256 * a.kv.n_kv_head >= 256;
         if (large) a.groups = 8;
         a.tiles = (int)(rows / (32 * a.groups) + std::min(a.T, a.B));
         // no more than keep the partial sums, written and read again, below the rows of K and V that they save
-        // time on: prompts of 1 to 1100 tokens over up to 2600 rows, window 512, 16/4 heads of 96, in three
-        // splits / whole 52.7 / 32.2 us; 3 to 5 tokens over 1500 to 4000 rows, 64/8 heads of 64, seven / whole
+        // time on: prompts of 1 to 1100 tokens over up to 2600 rows, window 512, 16/4 heads of 96, split
+        // to fill the GPU / whole 99 / 33 us; 3 to 5 tokens over 1500 to 4000 rows, 64/8 heads of 64, seven / whole
         // 29 / 123 us
         const long most = n * a.B * a.kv.n_kv_head * es / (4l * a.T * a.NH);
         a.splits = large ? 1 : (int)std::max<long>(1, std::min<long>(most, pa_splits((long)a.tiles * a.kv.n_kv_head, n, kPromptWG)));

@@ -28,27 +28,28 @@ template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, 
 // registers, where they become bf16.
 //
 // HP (fp32 q or out): q and the weights in planes that hold fp32's precision, three products for one (two
-// in fp16).  Else both are 16 bits: a weight's rounding is as large as the output's own (the error against
-// 64 bits is 1.4 times that of the output rounded alone), and a second plane would add half of the
-// matrix instructions to a kernel that they bound.
+// in fp16).  Else q is 16 bits as it is, and the weights take two planes, as in decode: rounded to one they
+// raise the error against 64 bits to 1.3 times that of the output rounded alone (6011 tokens, bf16, 2.16e-3
+// for 1.64e-3, 326 us for 418; prompts of 1 to 1100 tokens, fp16, 2.9e-4 for 2.1e-4, 30 us for 33).
 //
 // A weight of 0 times an infinity or a NaN that a masked row of V holds is NaN, so in the steps where
 // some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
 // element by element to the queries that do see them.
 //
-// One prompt of 6011 tokens, 32/8 heads of 128, bf16: 323 us, 916 TFLOP/s (a bf16 product of 8192^3 reaches
-// 1288 on this card).  Per step of 32 x 64 scores a wave issues 32 matrix instructions (1024 cycles) and about
-// 190 others (32 exponentials among them, at a quarter of the rate), and the two do not overlap on a SIMD
-// (matrix cores busy 34 to 38 % of the time, the vector unit as much): 4300 cycles for the two waves of a SIMD of
-// 4900 measured; prologue and epilogue are 11 %.  Three or four buffers instead of two 1 to 2 % slower (the loads
-// are hidden by then), 32-row steps 6 %, the sum of the weights by v_dot2 16 % (it issues slowly), scores two
-// waves a SIMD without the order of LDS reads fixed below 10 %, the page looked up by a vector load 5 %, matrix
-// instructions at a higher wave priority 1 % faster or slower.
+// One prompt of 6011 tokens, 32/8 heads of 128, bf16: 418 us, 709 TFLOP/s of the operator's operations, 1063 with
+// the weights' second plane (a bf16 product of 8192^3 reaches 1288 on this card).  Per step of 32 x 64 scores a wave
+// issues 48 matrix instructions (1536 cycles) and about 275 vector ones (32 exponentials among them, at a quarter of
+// the rate), and the two do not overlap on a SIMD: some 6000 cycles for its two waves (matrix cores busy 41 % of the
+// kernel).  The operand reads are issued ahead, but the waits, five a step, are for all of them at once: a part of
+// that lead is lost.  Tried, with one plane of weights (a step 4300 cycles of 4900 measured): three or four buffers
+// instead of two 1 to 2 % slower (the loads are hidden by then), 32-row steps 6 %, the sum of the weights by v_dot2
+// 16 % (it issues slowly), scores two waves a SIMD without the order of LDS reads fixed below 10 %, the page looked up
+// by a vector load 5 %, matrix instructions at a higher wave priority 1 % faster or slower.
 template <int CT, bool HP, int HDB, int RG, int KH, int EV>
 __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG * KH * pa_parts(HDB) == 8 ? 1 : 2) void k_pa_prompt(pa_args a)
 {
     constexpr bool E8 = CT == MLLM_E4M3;
-    constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1;
+    constexpr int ES = E8 ? 1 : 2, NP = HP ? kPlanes<CT> : 1, PW = HP ? kPlanes<CT> : 2;   // planes of q, of the weights
     constexpr int DH = pa_parts(HDB), NW = RG * KH * DH, ROWS = 32 * RG;
     static_assert(KH == 1 || DH == 1, "a row group has at most two waves");
     constexpr int TK = HDB > 128 ? 32 : 64, TW = TK / KH, NB = TW / 32;   // rows per step, and of them a wave's, in blocks of 32
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
         const int sw = s0 + TW * kh;                         // the wave's rows of K and V
         if (sw > pmax || sw + TW <= lmin) return;            // nothing that the wave's queries see
         // Operands are read from LDS ahead of the products that take them: K's two products' worth (KD), V's
-        // a group of VG; the scheduler is held to that order, or it reads each right before its use.
+        // a group of VG; the scheduler is held to that order, or it issues each read right before its use.
         constexpr int KD = KS < 2 ? 1 : 2;
         f32x16 s[NB] = {};
         uint4 kf[KD + 1][NB];
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
         const float mb = kBias<CT> - m;
 #pragma unroll
         for (int y = 0; y < TW / 16; y++) {
-            uint32_t p[4][NP];
+            uint32_t p[4][PW];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int at = 8 * (y & 1) + 2 * e;
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
                 const float v = __builtin_amdgcn_exp2f(fmaf(s[y >> 1][at + 1], zs, mb));
                 s[y >> 1][at] = u;
                 s[y >> 1][at + 1] = v;
-                pa_planes<CT, NP>(u, v, p[e]);
+                pa_planes<CT, PW>(u, v, p[e]);
                 float &l = e & 1 ? l1 : l0;
                 l += u + v;
             }
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
                 for (int x = 0; x < VG; x++) {
                     const uint2 f0 = vf[z & 1][x][0], f1 = vf[z & 1][x][1];
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; n--)
+                    for (int n = PW - 1; n >= 0; n--)
                         o[VG * g + x] = pa_mfma32<CT>(make_uint4(f0.x, f0.y, f1.x, f1.y), make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]), o[VG * g + x]);
                 }
             }
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
 #pragma unroll
         for (int z = 0; z < VS * TW / 16; z++) {
             if (z + 1 < VS * TW / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2 * VG, 0);
-            __builtin_amdgcn_sched_group_barrier(0x8, VG * NP, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, VG * PW, 0);
         }
         if constexpr (KH > 1) bad = bad >> (TW * kh) & 0xFFFFFFFFull;
         while (bad) {                                        // rare: V rows that were cleared
