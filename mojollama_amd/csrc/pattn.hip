@@ -130,6 +130,8 @@ bool pa_partials(pa_args &a, void *ws, long ws_bytes)
 int pa_launch(const char *who, pa_args &a, void *ws, long ws_bytes, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
+    // every position is below max_len: such a window masks nothing, and the kernels' sums with it stay in 32 bits
+    if (a.window >= a.max_len) a.window = 0;
     pa_divisor(a);
     a.rep = a.NH / a.kv.n_kv_head;
     const bool wide = a.q_type == MLLM_F32 || a.out_type == MLLM_F32;

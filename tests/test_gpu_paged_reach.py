@@ -197,6 +197,21 @@ def test_unmapped_pages_of_every_size(dev, page, cache, q, window):
         check(out[b:b + 1], c, b, x[b:b + 1], torch.tensor([n - 1]), NH, window, None, q)
 
 
+# ------------------------------------------------------------------ windows
+@pytest.mark.parametrize("window", [40, 41, (1 << 30) + 1, (1 << 31) - 50, (1 << 31) - 1])
+@pytest.mark.parametrize("cache,q", [(BF16, BF16), (F16, F32)])
+def test_windows_without_an_end(dev, window, cache, q):
+    """A window at or past the longest length is none, also where the first queries lie before position 0."""
+    c = Cache(6, [40, 33], 2, 64, 16, cache)
+    x, kv = queries(1, 83, 4, 64, q), c.view(dev)
+    got = dev.paged_attn_prompt(kv, x.cuda(), i32([0, 50, 83]), i32([40, 33]), 40, 4, window=window)
+    check(got[:50], c, 0, x[:50], torch.arange(-10, 40), 4, 0, None, q)
+    check(got[50:], c, 1, x[50:], torch.arange(33), 4, 0, None, q)
+    assert torch.equal(got, dev.paged_attn_prompt(kv, x.cuda(), i32([0, 50, 83]), i32([40, 33]), 40, 4))
+    got = dev.paged_attn_decode(kv, x[:2].cuda(), i32([40, 33]), 40, 4, window=window)
+    assert torch.equal(got, dev.paged_attn_decode(kv, x[:2].cuda(), i32([40, 33]), 40, 4))
+
+
 # ------------------------------------------------------------------ how split calls are made
 @pytest.fixture(scope="module")
 def long(dev):
