@@ -113,9 +113,9 @@ __device__ __forceinline__ void store_e4m3(uint8_t *dst, uint8_t *exp, const dou
         float y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float f = to_odd(x[4 * h + i] * inv);
+            const float f = to_odd(x[4 * h + i] * inv);         // infinite where x leaves fp32's range
             const float g = f > 448.0f ? 448.0f : f < -448.0f ? -448.0f : f;
-            y[i] = f - f == 0.0f ? g : NAN;     // infinities and NaN
+            y[i] = fabs(x[4 * h + i]) < INFINITY ? g : NAN;
         }
         int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
         w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);

@@ -1,5 +1,7 @@
 """mllm_rotary_append where its stores go past the caches (more than 32 MB of
-output)."""
+output), and rows for an 8-bit cache whose rotation leaves fp32's range."""
+import math
+
 import pytest
 import torch
 
@@ -49,3 +51,21 @@ def test_stores_past_the_caches(dev, layout, r, act, cache, odd):
     on = ~keep & (pos < torch.where(seqs == 0, 87 * 16, 88 * 16))        # 87 and 88 pages are mapped
     assert int((~on & ~keep).sum()) > 0
     stored(kv, c, seqs[on].tolist(), pos[on].tolist(), want[on][:, NH:], x[on][:, NH + NKH:], x[on][:, NH:NH + NKH], 1.0)
+
+
+def test_e4m3_beyond_fp32(dev):
+    """Elements that the rotation takes past fp32's largest number saturate, at the largest scale in a row of finite
+    ones, at 448 in a row that holds an infinity."""
+    NKH, HD, big = 1, 16, 3e38
+    c = Cache(3, [2], NKH, HD, 16, E4M3)
+    kv = c.view(dev)
+    x = torch.zeros(2, HD)
+    x[:, 0] = x[:, 8] = big                      # 3e38 (cos 1 - sin 1), 3e38 (cos 1 + sin 1)
+    x[1, 3] = math.inf                           # and of its pair's other element, 0, infinity times sin
+    dev.rotary_append(dev.rotary(16), None, x.cuda(), x.cuda(), i32([1, 1]), kv=kv, seqs=i32([0, 0]), rows=i32([0, 1]))
+    p = int(c.tables[0, 0])
+    code = kv._tensors[0][p, :2, 0].cpu().double()
+    assert kv._tensors[3][p, 0, :2].tolist() == [227, 127]                # 2^100, the largest scale, and 2^0
+    assert code[0, [0, 8]].tolist() == [-448.0, 448.0]
+    assert code[1, [0, 8]].tolist() == [-448.0, 448.0]
+    assert torch.isnan(code[1, [3, 11]]).all() and not torch.isnan(code[1, [1, 2, 4, 9, 15]]).any()
