@@ -482,11 +482,15 @@ typedef struct {
  *   NTK     with base * factor^(r / (r - 2))
  *   YARN    divided by factor for the pairs that turn less than beta_slow times
  *           in ctx positions, as they are above beta_fast times, a linear ramp
- *           over the pairs between; mscale 0.1 ln(factor) + 1 (factor > 1)
+ *           over the pairs j between: from floor(p(beta_fast)) to
+ *           ceil(p(beta_slow)), p(b) = r ln(ctx / (2 pi b)) / (2 ln base), at
+ *           least 0 and at most r - 1; mscale 0.1 ln(factor) + 1 (factor > 1)
  *   BANDS   the same by wavelength: divided by factor where ctx holds fewer than
  *           beta_slow turns, as they are above beta_fast, blended by the number
  *           of turns between
- * beta_fast / beta_slow <= 0 take 32 / 1 (YARN) and 4 / 1 (BANDS). */
+ * beta_fast / beta_slow <= 0 take 32 / 1 (YARN) and 4 / 1 (BANDS).  Any other
+ * frequencies and mscale serve as well: a model whose ramp ends between two
+ * pairs forms its own. */
 #define MLLM_ROPE_HALF 0
 #define MLLM_ROPE_PAIRS 1
 #define MLLM_ROPE_NONE 0

@@ -12,6 +12,7 @@ There is no CPU fallback: if the library is missing or cannot be loaded,
 ``load_kernels()`` raises.
 """
 import ctypes
+import math
 import os
 import subprocess
 
@@ -517,13 +518,25 @@ class DeviceOps:
         return view
 
     def rotary(self, rope_dim, layout=ROPE_HALF, base=10000.0, scaling=ROPE_NONE, factor=1.0, ctx=0.0, beta_fast=0.0,
-               beta_slow=0.0):
-        """An mllm_rotary with its frequencies on the current GPU (mllm_rotary_freqs)."""
-        f, m = (ctypes.c_double * max(rope_dim // 2, 1))(), ctypes.c_float()
-        self._check(self.so.mllm_rotary_freqs(scaling, rope_dim, base, factor, ctx, beta_fast, beta_slow, f,
-                                              ctypes.byref(m)), "mllm_rotary_freqs")
-        freqs = self.torch.tensor(list(f), dtype=self.torch.float64).cuda()
-        rot = Rotary(layout, rope_dim, freqs.data_ptr(), m.value)
+               beta_slow=0.0, freqs=None, mscale=None):
+        """An mllm_rotary with its frequencies on the current GPU: those of mllm_rotary_freqs, or the caller's own
+        rope_dim / 2 (freqs, radians per position, in place of a scaling).  mscale None: the scaling's factor."""
+        torch = self.torch
+        if freqs is None:
+            f, m = (ctypes.c_double * max(rope_dim // 2, 1))(), ctypes.c_float()
+            self._check(self.so.mllm_rotary_freqs(scaling, rope_dim, base, factor, ctx, beta_fast, beta_slow, f,
+                                                  ctypes.byref(m)), "mllm_rotary_freqs")
+            freqs, scale = torch.tensor(list(f), dtype=torch.float64), m.value
+        else:
+            freqs, scale = torch.as_tensor(freqs, dtype=torch.float64, device="cpu"), 1.0
+            if scaling != ROPE_NONE or rope_dim % 2 or tuple(freqs.shape) != (rope_dim // 2,) or not freqs.isfinite().all():
+                raise ValueError("freqs: rope_dim / 2 finite frequencies, in place of a scaling")
+        if mscale is not None:
+            scale = float(mscale)
+            if not math.isfinite(scale):
+                raise ValueError("mscale is finite")
+        freqs = freqs.cuda()
+        rot = Rotary(layout, rope_dim, freqs.data_ptr(), scale)
         rot._tensors, rot._device = (freqs,), self._cur()
         return rot
 

@@ -1,5 +1,6 @@
 """mllm_rotary_append where its stores go past the caches (more than 32 MB of
-output), and rows for an 8-bit cache whose rotation leaves fp32's range."""
+output), rows for an 8-bit cache whose rotation leaves fp32's range, and
+frequencies of the caller's own."""
 import math
 
 import pytest
@@ -69,3 +70,32 @@ def test_e4m3_beyond_fp32(dev):
     assert code[0, [0, 8]].tolist() == [-448.0, 448.0]
     assert code[1, [0, 8]].tolist() == [-448.0, 448.0]
     assert torch.isnan(code[1, [3, 11]]).all() and not torch.isnan(code[1, [1, 2, 4, 9, 15]]).any()
+
+
+@pytest.mark.parametrize("layout", [K.ROPE_HALF, K.ROPE_PAIRS])
+def test_own_frequencies(dev, layout):
+    """Frequencies and a factor of the caller's own: here a ramp whose ends are not rounded to whole pairs."""
+    r, base, f, ctx, pos = 64, 150000.0, 32.0, 4096.0, torch.tensor([0, 1, 77, 4095, 131071], dtype=torch.int32)
+    j = torch.arange(r // 2, dtype=torch.float64)
+    w = base ** (-2 * j / r)
+    lo, hi = (r * math.log(ctx / (b * 2 * math.pi)) / (2 * math.log(base)) for b in (32.0, 1.0))
+    ramp = ((j - lo) / (hi - lo)).clamp(0, 1)
+    own = w / f * ramp + w * (1 - ramp)
+    x = torch.randn(len(pos), 2, r, generator=torch.Generator().manual_seed(1))
+    for freqs in (own, own.cuda(), own.tolist()):
+        rot = dev.rotary(r, layout=layout, freqs=freqs, mscale=1.25)
+        assert torch.equal(rot._tensors[0].cpu(), own) and rot.mscale == 1.25
+        out = torch.empty(len(pos), 2 * r, device="cuda")
+        dev.rotary_append(rot, x.view(len(pos), -1).cuda(), None, None, pos.cuda(), NH=2, HD=r, q_out=out)
+        near(out, turn(x.double(), pos, rot, layout), x.double(), F32, 1.25)
+    assert dev.rotary(r, freqs=own).mscale == 1.0
+    assert dev.rotary(r, scaling=K.ROPE_YARN, factor=f, ctx=ctx, mscale=2.0).mscale == 2.0
+    for bad in (own[:-1], own[None], [0.0] * 33, torch.full_like(own, math.nan)):
+        with pytest.raises(ValueError):
+            dev.rotary(r, freqs=bad)
+    with pytest.raises(ValueError):
+        dev.rotary(r, freqs=own, scaling=K.ROPE_YARN, factor=f, ctx=ctx)
+    with pytest.raises(ValueError):
+        dev.rotary(r, mscale=math.nan)
+    with pytest.raises(ValueError):
+        dev.rotary(63, freqs=[1.0] * 31)
