@@ -531,7 +531,10 @@ MLLM_API int mllm_rotary_append(const mllm_rotary *rot, int in_type, const void 
  * over the mapped rows s <= p that the query at position p sees, with window
  * w > 0 only those of s > p - w (the sink's term only where sinks is given,
  * fp32 [NH]).  A query that sees no row gives zeros; what rows hold that a query
- * does not see, NaN too, has no part in its result.  scale is finite.  lens[i]
+ * does not see, NaN too, has no part in its result; of a row that it sees, an
+ * infinity in V makes that column infinite (NaN where the row's weight is too
+ * small for its type, or with one of the other sign), an infinity or NaN in K
+ * may make all of it NaN.  scale is finite.  lens[i]
  * (device) is the number of cached rows of the i-th sequence, the new tokens'
  * own among them; it is taken as at most max_len.  The i-th sequence reads table row seqs[i]
  * (NULL: i); one outside the tables has no rows.

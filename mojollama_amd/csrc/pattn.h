@@ -52,23 +52,27 @@ constexpr float kLowest = -3e38f;   // below every score: exp2(-inf - kLowest) i
 constexpr float kSlack = 8.0f;
 template <int CT> constexpr float kBias = CT == MLLM_F16 ? 7.0f : 0.0f;
 
-// a and b as planes of 16-bit values, one word each: bf16 takes three (8 + 8 + 8 bits), fp16 two
-// (11 + 11); NP == 1 rounds.
-template <int CT, int NP> __device__ __forceinline__ void pa_planes(float x, float y, uint32_t (&w)[NP])
+// x and y as planes of 16-bit values, one word each: bf16 takes three (8 + 8 + 8 bits), fp16 two
+// (11 + 11); NP == 1 rounds.  W: weights, x and y >= 0.  No plane of theirs is then negative, and none 0 beside
+// one that is not (they sum to x (1 + 2^-23); in fp16 as far as its subnormals reach): an infinity of V times
+// them is infinite, where a plane of 0 or below would make it NaN.
+template <int CT, int NP, bool W = false> __device__ __forceinline__ void pa_planes(float x, float y, uint32_t (&w)[NP])
 {
+    constexpr float E = W ? 1.00000011920928955078125f : 1.0f;
     if constexpr (NP == 1) {
         w[0] = pack16(x, y, CT == MLLM_F16 ? MLLM_F16 : MLLM_BF16);
     } else if constexpr (CT == MLLM_F16) {
-        const f16x2 h = {(_Float16)x, (_Float16)y};
+        f16x2 h = {(_Float16)x, (_Float16)y};
+        if constexpr (W) h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
         w[0] = __builtin_bit_cast(uint32_t, h);
-        w[1] = __builtin_bit_cast(uint32_t, (f16x2){(_Float16)(x - (float)h.x), (_Float16)(y - (float)h.y)});
+        w[1] = __builtin_bit_cast(uint32_t, (f16x2){(_Float16)fmaf(x, E, -(float)h.x), (_Float16)fmaf(y, E, -(float)h.y)});
     } else {
 #pragma unroll
         for (int p = 0; p < NP; p++) {
             const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
             w[p] = __builtin_amdgcn_perm(b, a, 0x07060302);
-            x -= __uint_as_float(a & 0xFFFF0000u);
-            y -= __uint_as_float(b & 0xFFFF0000u);
+            x = fmaf(x, E, -__uint_as_float(a & 0xFFFF0000u));
+            y = fmaf(y, E, -__uint_as_float(b & 0xFFFF0000u));
         }
     }
 }

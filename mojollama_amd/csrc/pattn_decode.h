@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, HDB == 256 || (HP && HDB == 128) ? 1 : 2) void
                 l += z[r];
             }
 #pragma unroll
-            for (int x = 0; x < 4; x++) pa_planes<CT, NW>(z[2 * x], z[2 * x + 1], pw[x]);
+            for (int x = 0; x < 4; x++) pa_planes<CT, NW, true>(z[2 * x], z[2 * x + 1], pw[x]);
             if (!all) {                              // what lies in rows that are not the query's may be NaN
 #pragma unroll
                 for (int r = 0; r < 8; r++)

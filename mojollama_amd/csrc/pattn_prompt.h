@@ -402,7 +402,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
                 const float v = __builtin_amdgcn_exp2f(fmaf(s[y >> 1][at + 1], zs, mb));
                 s[y >> 1][at] = u;
                 s[y >> 1][at + 1] = v;
-                pa_planes<CT, PW>(u, v, p[e]);
+                pa_planes<CT, PW, true>(u, v, p[e]);
                 float &l = e & 1 ? l1 : l0;
                 l += u + v;
             }

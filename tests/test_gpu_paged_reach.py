@@ -211,6 +211,28 @@ def test_windows_without_an_end(dev, window, cache, q):
     got = dev.paged_attn_decode(kv, x[:2].cuda(), i32([40, 33]), 40, 4, window=window)
     assert torch.equal(got, dev.paged_attn_decode(kv, x[:2].cuda(), i32([40, 33]), 40, 4))
 
+# ------------------------------------------------------------------ infinities in V
+@pytest.mark.parametrize("cache,q", [(BF16, BF16), (F16, F16), (BF16, F32), (F16, F32)])
+@pytest.mark.parametrize("HD,page", [(64, 16), (128, 64), (80, 25), (256, 64)])
+def test_infinities_of_one_sign_stay_infinite(dev, cache, q, HD, page):
+    """An infinity of V in a row that a query sees makes that column infinite, not NaN: in a row of its own (weight 1), in
+    rows that all queries of a tile see, and in steps where some do not; a column of both signs is NaN."""
+    n, NH, NKH = 300, 4, 2
+    c = Cache(HD, [n, 1], NKH, HD, page, cache)
+    marks = [(0, 0, 0, 3, INF), (0, 40, 0, 7, -INF), (0, 250, 1, 1, INF), (0, 60, 1, 9, INF), (0, 61, 1, 9, -INF),
+             (1, 0, 0, 2, -INF)]
+    for b, s, h, d, x in marks:
+        c.pools[1][int(c.tables[b, s // page]), s % page, h, d] = x
+    kv, x = c.view(dev), queries(HD, n + 1, NH, HD, q) / 4                # no weight is so small that fp16 holds none of it
+    got = dev.paged_attn_prompt(kv, x.cuda(), i32([0, n, n + 1]), i32([n, 1]), n, NH).float().cpu().view(n + 1, NH, HD)
+    last = dev.paged_attn_decode(kv, x[n - 1:].cuda(), i32([n, 1]), n, NH).float().cpu().view(2, NH, HD)
+    want = torch.zeros(n + 1, NH, HD)
+    want[0:n, 0:2, 3], want[40:n, 0:2, 7], want[250:n, 2:, 1], want[60:n, 2:, 9] = INF, -INF, INF, INF
+    want[61:n, 2:, 9], want[n, 0:2, 2] = NAN, -INF
+    for y, w in ((got, want), (last, want[n - 1:])):
+        assert torch.equal(torch.isnan(y), torch.isnan(w))
+        assert torch.equal(torch.where(torch.isinf(y), y, 0), torch.where(torch.isinf(w), w, 0))
+
 
 # ------------------------------------------------------------------ how split calls are made
 @pytest.fixture(scope="module")
