@@ -54,11 +54,13 @@ template <int CT> constexpr float kBias = CT == MLLM_F16 ? 7.0f : 0.0f;
 
 // x and y as planes of 16-bit values, one word each: bf16 takes three (8 + 8 + 8 bits), fp16 two
 // (11 + 11); NP == 1 rounds.  W: weights, x and y >= 0.  No plane of theirs is then negative, and none 0 beside
-// one that is not (they sum to x (1 + 2^-23); in fp16 as far as its subnormals reach): an infinity of V times
-// them is infinite, where a plane of 0 or below would make it NaN.
+// one that is not (they sum to kPlanesSum x; in fp16 as far as its subnormals reach): an infinity of V times
+// them is infinite, where a plane of 0 or below would make it NaN.  The sum of the weights is multiplied by
+// kPlanesSum as well, once, and the factor cancels.
+constexpr float kPlanesSum = 1.00000011920928955078125f;     // 1 + 2^-23
 template <int CT, int NP, bool W = false> __device__ __forceinline__ void pa_planes(float x, float y, uint32_t (&w)[NP])
 {
-    constexpr float E = W ? 1.00000011920928955078125f : 1.0f;
+    constexpr float E = W ? kPlanesSum : 1.0f;
     if constexpr (NP == 1) {
         w[0] = pack16(x, y, CT == MLLM_F16 ? MLLM_F16 : MLLM_BF16);
     } else if constexpr (CT == MLLM_F16) {

@@ -301,6 +301,7 @@ __global__ __launch_bounds__(256, HDB == 256 || (HP && HDB == 128) ? 1 : 2) void
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    l *= kPlanesSum;
 
     // the four waves' parts
     if (g == 0) { sm[w][i] = m; sl[w][i] = l; }

@@ -495,7 +495,7 @@ __global__ __launch_bounds__(64 * RG * KH * pa_parts(HDB), HP && HDB > 64 || RG 
         }
         __builtin_amdgcn_s_waitcnt(0x0F70);                  // no load may still be on its way into LDS at the end
     }
-    float l = l0 + l1;
+    float l = (l0 + l1) * kPlanesSum;
     if constexpr (KH == 2) {
         // the two halves of the rows of K and V: the second waves' sums through the buffers of the steps
         __shared__ float hm[RG][64], hl[RG][64];

@@ -234,6 +234,26 @@ def test_infinities_of_one_sign_stay_infinite(dev, cache, q, HD, page):
         assert torch.equal(torch.where(torch.isinf(y), y, 0), torch.where(torch.isinf(w), w, 0))
 
 
+@pytest.mark.parametrize("cache,q", SPLIT + [(F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("HD", [64, 128, 256])
+def test_a_row_of_all_the_weight_is_given_back(dev, cache, q, HD):
+    """A query that sees one row: V's row, by a whole call and by a split one whose window leaves that row.  The weight
+    w itself cancels between the sum and the product.  Its planes hold it to 2^-22 (fp16: 11 bits cut and 11 rounded;
+    bf16's three to 2^-23), the product's two or three sums, the sum's factor, its reciprocal and the last product round
+    once each in fp32: 6 * 2^-24 more, together below 2^-21.  bf16's two planes hold it to 2^-15.  A 16-bit output,
+    which holds the row, is nearer to it than to its neighbours, 2^-9 or 2^-12 away, and exact."""
+    rows, NKH, NH = [1, 2000], 2, 4
+    c = Cache(HD, rows, NKH, HD, 16, cache)
+    kv, x, v = c.view(dev), queries(HD, 3, NH, HD, q), torch.stack([c.v[0][0], c.v[1][1999]]).repeat_interleave(2, 1)
+    tol = 2.0 ** -21 if q == F32 else 0.0
+    calls = (dev.paged_attn_decode(kv, x[:2].cuda(), i32(rows), 2000, NH, window=1),
+             dev.paged_attn_prompt(kv, x[:2].cuda(), i32([0, 1, 2]), i32(rows), 2000, NH, window=1),
+             dev.paged_attn_decode(kv, x[:1].cuda(), i32([1]), 2000, NH))
+    for out in calls:
+        y = out.cpu().double().view(-1, NH, HD)
+        assert ((y - v[:len(y)]).abs() <= tol * v[:len(y)].abs()).all()
+
+
 # ------------------------------------------------------------------ how split calls are made
 @pytest.fixture(scope="module")
 def long(dev):
