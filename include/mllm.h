@@ -457,7 +457,8 @@ MLLM_API const int *mllm_page_table_entries(const mllm_page_table *pt);
  * sequence seq's row s; a row whose page is unmapped (outside [0, n_pages)) or
  * past max_blocks takes no part in attention and is not stored.  A sequence in
  * one piece is a page of its own length.  MLLM_E4M3: an element stands for
- * code * 2^(e - 127), e = k_exp / v_exp[(p * n_kv_head + h) * page_size + r].
+ * code * 2^(e - 127), e = k_exp / v_exp[(p * n_kv_head + h) * page_size + r],
+ * e < 255.
  * head_dim a multiple of 16 up to 256; k, v and the strides multiples of 16
  * bytes.  Pools may be longer than 32 bits count. */
 typedef struct {

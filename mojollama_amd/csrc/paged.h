@@ -35,9 +35,6 @@ inline int pk_fail(const char *who, const char *why)
     return -1;
 }
 
-// Rows [0, n) addressable through the tables.
-inline long pk_rows(const mllm_paged_kv *kv) { return (long)kv->max_blocks * kv->page_size; }
-
 // The page of row s of sequence seq (0 <= seq < n_seqs, s >= 0), -1 unmapped; s becomes the row in the page.
 __device__ __forceinline__ int pk_page(const mllm_paged_kv &kv, int seq, int &s)
 {

@@ -7,6 +7,13 @@
 // first in the order of the requests: ranks come from prefix sums in one
 // workgroup, never from the order of atomics, and the counts' atomic additions
 // give the same sum in any order.
+//
+// That workgroup passes over all pages and requests, which is short where they
+// are some thousands and is not in larger pools: compacting (nothing moves) 7.8,
+// 20 and 147 us at 1000, 10^4 and 10^5 pages; a step's reserve, nothing to add,
+// 7 us for 64 sequences of 128 blocks, 17 of 8192 blocks, 124 us for 1024
+// sequences and 944 for 4096 (each request is compared with those before it);
+// giving 90 % of 10^5 pages to 64 sequences 120 us.
 #include "paged.h"
 
 namespace {
@@ -286,7 +293,7 @@ __device__ __forceinline__ void copy_unit(const copy_args &c, int unit, int src,
     }
 }
 
-// Units blockIdx.x, + gridDim.x, ... of `moves` page copies (moves: on the device where cnt is given).
+// Units wg, + wgs, ... of `moves` page copies.
 __device__ __forceinline__ void copy_pages(const copy_args &c, const int *src, const int *dst, int moves, int wg, int wgs)
 {
     const int per = c.units[c.n_planes];

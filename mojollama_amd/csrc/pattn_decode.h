@@ -19,10 +19,11 @@
 // maximum per head and moves it rarely (kSlack), and each lane its own part of the sum, so the loop has
 // no exchange between lanes.  The four waves of a workgroup take every fourth tile pair and join in LDS.
 //
-// One sequence of 131072 rows, 32/4 heads of 128, bf16: 56.6 us with the join, 4.7 TB/s (a 1 GiB copy reaches
-// 5.1); eight of 2048 to 4096, 64/8 heads of 64, 16.5 us, of which the join and the launches are 6.  An e4m3 row
-// of one head is 128 bytes: 48 sequences of up to 9000 rows, 43 us, 2.5 TB/s: pieces that short, read by the kv
-// heads' workgroups on different XCDs, and workgroups that find nothing to do beside long sequences.  Tried: the
+// One sequence of 131072 rows, 32/4 heads of 128, bf16: 57 us with the join, 4.7 TB/s (a 1 GiB copy reaches
+// 5.1); eight of 2048 to 4096, 64/8 heads of 64, 16.7 us, of which the join and the launches are 6.  e4m3, 32/8 heads
+// of 128: 48 sequences of 9000 rows each 172 us, 5.2 TB/s, whatever the pool's order; 48 of up to 9000, 108 MB in
+// all, 43 us, 2.5 TB/s: the join (7 us) and the start of the workgroups weigh more, equal lengths of that sum take 38
+// us, on a [page][head][row] pool 32 (unequal 41).  L2 misses are the same in all four.  Tried: the
 // splits of all sequences in one list that 1024 workgroups walk (10 % slower: a scan of the lengths before each),
 // heads fastest in the launch order (12 % slower there, 6 % faster with eight equal sequences), three waves a SIMD
 // (no change), two tiles in flight a wave where the registers allow it (e4m3 43 -> 48 us, two waves a SIMD then).

@@ -36,11 +36,11 @@ template <int CT> __device__ __forceinline__ f32x16 pa_mfma32(uint4 x, uint4 y, 
 // some row of the tile is masked V is looked through for such rows; they are cleared in LDS and added
 // element by element to the queries that do see them.
 //
-// One prompt of 6011 tokens, 32/8 heads of 128, bf16: 418 us, 709 TFLOP/s of the operator's operations, 1063 with
-// the weights' second plane (a bf16 product of 8192^3 reaches 1288 on this card).  Per step of 32 x 64 scores a wave
+// One prompt of 6011 tokens, 32/8 heads of 128, bf16: 418 to 431 us on three cards, 697 TFLOP/s of the operator's
+// operations, 1046 with the weights' second plane (a bf16 product of 8192^3 reaches 1288).  Per step of 32 x 64 scores a wave
 // issues 48 matrix instructions (1536 cycles) and about 275 vector ones (32 exponentials among them, at a quarter of
-// the rate), and the two do not overlap on a SIMD: some 6000 cycles for its two waves (matrix cores busy 41 % of the
-// kernel).  The operand reads are issued ahead, but the waits, five a step, are for all of them at once: a part of
+// the rate), and the two hardly overlap on a SIMD: some 6000 cycles for its two waves (matrix cores busy 47 % of the
+// kernel's cycles).  The operand reads are issued ahead, but the waits, five a step, are for all of them at once: a part of
 // that lead is lost.  Tried, with one plane of weights (a step 4300 cycles of 4900 measured): three or four buffers
 // instead of two 1 to 2 % slower (the loads are hidden by then), 32-row steps 6 %, the sum of the weights by v_dot2
 // 16 % (it issues slowly), scores two waves a SIMD without the order of LDS reads fixed below 10 %, the page looked up
