@@ -2,7 +2,8 @@
 joins take over: prompts in tiles of 256 rows, splits of prompts and decode with
 windows and sinks, more splits than the join loads at once, 16 and more query
 heads above head size 128, unmapped pages at every page size's kernel, split
-calls captured and on two streams."""
+calls captured and on two streams; and at the ends of its range: windows up to
+2^31 - 1, infinities of V, a single row."""
 import pytest
 import torch
 
