@@ -616,6 +616,61 @@ MLLM_API int mllm_pages_copy(const mllm_page_plane *planes, int n_planes, int n_
  * sequence outside [0, n_seqs), one listed before in the same call (reserve: in
  * seqs, fork: in children), lens outside the tables' rows; compact: L. */
 
+/* ------------------------- layers in 8-bit integers: a scale per row and token
+ * A quantised row stands for scale * q[i], i < n, with 8-bit integers q and an
+ * fp32 scale.  The calls below that form one from values y[i] take
+ *   q[i] = y[i] * (127 * (1 / max|y|)) to the nearest integer (ties to even),
+ *   scale = max|y| / 127,
+ * in fp32, operation by operation; a row of zeros has scale 0 and zeros; a row that holds an
+ * infinity or a NaN has scale NaN and zeros, so that every product with it is
+ * NaN.  T rows of x lie x_ld elements apart (at least n; x_ld of codes in
+ * bytes), T = 0 does nothing, n is positive.  Rows need no alignment beyond
+ * their elements' own; wide loads and stores are used at any address.  type:
+ * MLLM_F32, MLLM_F16 or MLLM_BF16.  What lies between the rows of an output
+ * keeps its contents; outputs do not overlap inputs but where it says so. */
+#define MLLM_I8 4                  /* 8-bit integers (weights of mllm_i8_pack) */
+
+/* y = x. */
+MLLM_API int mllm_i8_quantize(int type, const void *x, long x_ld, int T, int n, int8_t *q, long q_ld, float *scale,
+                              void *stream);
+/* out[t][i] = scale[t] * q[t][i], rounded to type. */
+MLLM_API int mllm_i8_dequant(const int8_t *q, long q_ld, const float *scale, int T, int n, int type, void *out,
+                             long out_ld, void *stream);
+/* y = w h / sqrt(mean(h^2) + eps) with h = x + res rounded to res_type, which
+ * goes to res_out (res NULL: h = x, nothing is stored).  res_out may be res, or
+ * x where res_type is type, in the same stride.  w [n]: w_type MLLM_F32 or any
+ * of the three.  eps is finite and not negative.  The norm's factor is one
+ * number per row, so it enters the scale alone: q is formed from w h. */
+MLLM_API int mllm_i8_rms_norm(int type, const void *x, long x_ld, int res_type, const void *res, long res_ld,
+                              void *res_out, long res_out_ld, int w_type, const void *w, float eps, int T, int n,
+                              int8_t *q, long q_ld, float *scale, void *stream);
+/* y = gate / (1 + e^-gate) * up; gate and up may be halves of one buffer. */
+MLLM_API int mllm_i8_silu_mul(int type, const void *gate, long gate_ld, const void *up, long up_ld, int T, int n,
+                              int8_t *q, long q_ld, float *scale, void *stream);
+
+/* Weights [n_rows][n_cols] (rows w_ld elements apart) in the layout of
+ * mllm_i8_gemm, mllm_i8_packed_size bytes, 16-byte aligned.  type MLLM_F32,
+ * _F16, _BF16: rows are quantised as above, their scales (output channels) go to
+ * scale [n_rows].  MLLM_I8: w holds the integers, scale is the caller's and
+ * not touched.  n_cols is at most 131071: sums of products of 8-bit integers
+ * then stay inside 32 bits. */
+MLLM_API long mllm_i8_packed_size(int n_rows, int n_cols);
+MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_cols, void *packed, float *scale,
+                          void *stream);
+/* out[t][r] = (sum_k x[t][k] w[r][k]) * x_scale[t] * w_scale[r] (+ bias[r],
+ * fp32, optional), the sums exact in 32-bit integers, the rest in fp32 in that
+ * order, rounded to type once.  x: T rows of 8-bit integers (-128 among them)
+ * at multiples of 16 bytes (x and x_ld; what lies behind a row's n_cols up to
+ * the next multiple of 16 bytes may be read and has no part in the result).
+ * Any T: few tokens stream the weights once, many run on tiles.  Workspace:
+ * mllm_i8_gemm_workspace_size bytes, 16-byte aligned (NULL where that is 0);
+ * one for T tokens serves every smaller T, and calls that overlap need one
+ * each.  Results are the same from call to call. */
+MLLM_API long mllm_i8_gemm_workspace_size(int T, int n_rows, int n_cols);
+MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t *x, long x_ld, const float *x_scale,
+                          int T, int n_rows, int n_cols, const float *bias, int type, void *out, long out_ld,
+                          void *workspace, long ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,463 @@
+// i8_rows.hip — rows into 8-bit integers with a scale each: as they are, after the residual addition and
+// root-mean-square norm, and after silu(gate) * up; back to values; and weights into the packed layout.
+//
+// y[i] of a row, its largest |y| and (norm) the sum of squares are formed in one pass over memory and stay
+// in registers; the codes are rounded from there: memory is read and written once, which is what bounds
+// these kernels.  The norm's factor 1 / sqrt(mean + eps) is one number per row: it enters the scale alone,
+// and the codes do not wait for it.
+#include "i8.h"
+
+namespace {
+
+// N bytes from an address of any alignment (the hardware's unaligned access).
+template <int N> struct raw { uint32_t w[N / 4]; };
+template <int N> __device__ __forceinline__ raw<N> ld_any(const void *p)
+{
+    raw<N> r;
+    __builtin_memcpy(&r, p, N);
+    return r;
+}
+
+// Eight consecutive elements, W bytes each, as they lie in memory; those from `left` on are zeros.
+template <int W> __device__ __forceinline__ raw<8 * W> ld8(const void *p, long at, int left)
+{
+    if (left >= 8) return ld_any<8 * W>((const char *)p + at * W);
+    raw<8 * W> r{};
+    for (int i = 0; i < left; i++) {
+        if constexpr (W == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j == i) r.w[j] = ((const uint32_t *)p)[at + i];
+        } else {
+            const uint32_t h = ((const uint16_t *)p)[at + i];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j == i) r.w[j >> 1] |= h << (16 * (j & 1));
+        }
+    }
+    return r;
+}
+template <int W> __device__ __forceinline__ void to_f32(const raw<8 * W> &r, int type, float (&x)[8])
+{
+    if constexpr (W == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(r.w[i]);
+    } else if (type == MLLM_BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(r.w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f16x2 v = __builtin_bit_cast(f16x2, r.w[i]);
+            x[2 * i] = (float)v.x;
+            x[2 * i + 1] = (float)v.y;
+        }
+    }
+}
+template <int W> __device__ __forceinline__ raw<8 * W> from_f32(const float (&x)[8], int type)
+{
+    raw<8 * W> r;
+    if constexpr (W == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.w[i] = __float_as_uint(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = pack16(x[2 * i], x[2 * i + 1], type);
+    }
+    return r;
+}
+template <int W> __device__ __forceinline__ void st8(void *p, long at, int left, const raw<8 * W> &r)
+{
+    if (left >= 8) {
+        __builtin_memcpy((char *)p + at * W, &r, 8 * W);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < left) {
+            if constexpr (W == 4) ((uint32_t *)p)[at + i] = r.w[i];
+            else ((uint16_t *)p)[at + i] = (uint16_t)(r.w[i >> 1] >> (16 * (i & 1)));
+        }
+}
+
+// The step of a row: m is the largest |y| as fp32 bits, above or at those of infinity where the row holds an
+// infinity or a NaN.  Codes are rint(y * pre * inv), inv = 127 * (1 / (most * pre)); the power of two pre keeps
+// the reciprocal a normal number at either end of fp32.
+struct row_step { float pre, inv, most; bool bad; };
+__device__ __forceinline__ row_step step_of(uint32_t m)
+{
+    row_step s;
+    s.bad = m >= 0x7F800000u;
+    s.most = __uint_as_float(m);
+    s.pre = s.most < 0x1p-100f ? 0x1p64f : s.most > 0x1p100f ? 0x1p-64f : 1.0f;
+    s.inv = s.bad || m == 0 ? 0.0f : 1.0f / (s.most * s.pre) * 127.0f;
+    return s;
+}
+__device__ __forceinline__ uint32_t code(float y, const row_step &s)
+{
+    return s.bad ? 0u : (uint32_t)(int)rintf(y * s.pre * s.inv) & 0xFFu;
+}
+__device__ __forceinline__ uint2 codes(const float (&y)[8], const row_step &s)
+{
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i >> 2] |= code(y[i], s) << (8 * (i & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+enum { QUANTIZE, NORM, NORM_RES, SILU };
+
+struct row_args {
+    const void *x, *res, *w;       // SILU: gate, up
+    void *res_out;
+    long x_ld, res_ld, res_out_ld, q_ld;
+    int8_t *q;
+    float *scale;
+    float eps;
+    int type, res_type, w_type, T, n;
+    long kb;                       // packed weights: blocks along K (q then is the packed matrix)
+    int n_pad, T_pad;
+};
+
+// y of elements e .. e + 7 of row t; sq gains the squares of h.
+template <int KIND, int W, int RW>
+__device__ __forceinline__ void form(const row_args &a, const raw<8 * W> &xr, const raw<8 * RW> &rr, int e, long t, int left,
+                                     bool store, float (&y)[8], float &sq)
+{
+    to_f32<W>(xr, a.type, y);
+    if constexpr (KIND == SILU) {
+        float u[8];
+        to_f32<RW>(rr, a.res_type, u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = y[i] / (1.0f + expf(-y[i])) * u[i];
+    }
+    if constexpr (KIND == NORM_RES) {
+        float r[8];
+        to_f32<RW>(rr, a.res_type, r);
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] += r[i];
+        const raw<8 * RW> h = from_f32<RW>(y, a.res_type);
+        if (store) st8<RW>(a.res_out, t * a.res_out_ld + e, left, h);
+        to_f32<RW>(h, a.res_type, y);
+    }
+    if constexpr (KIND == NORM || KIND == NORM_RES) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) sq = fmaf(y[i], y[i], sq);
+        float w[8];
+        if (a.w_type == MLLM_F32) to_f32<4>(ld8<4>(a.w, e, left), a.w_type, w);
+        else to_f32<2>(ld8<2>(a.w, e, left), a.w_type, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] *= w[i];
+    }
+}
+
+template <int KIND, int W, int RW>
+__device__ __forceinline__ void load(const row_args &a, long t, int e, int left, raw<8 * W> &x, raw<8 * RW> &r)
+{
+    x = ld8<W>(a.x, t * a.x_ld + e, left);
+    if constexpr (KIND == NORM_RES || KIND == SILU) r = ld8<RW>(a.res, t * a.res_ld + e, left);
+}
+
+// The norm's factor with squares and their sum in 64 bits; every wave of the row forms it alike.
+template <int KIND, int W, int RW>
+__device__ float far_factor(const row_args &a, long t, int lane)
+{
+    double sum = 0.0;
+    for (int e = 8 * lane; e < a.n; e += 512) {
+        float h[8];
+        // the stored sum (x or res may be where it went): the barrier of the row's maximum lies between
+        if constexpr (KIND == NORM_RES) to_f32<RW>(ld8<RW>(a.res_out, t * a.res_out_ld + e, a.n - e), a.res_type, h);
+        else to_f32<W>(ld8<W>(a.x, t * a.x_ld + e, a.n - e), a.type, h);
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum += (double)h[i] * h[i];
+    }
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    return (float)(1.0 / sqrt(sum / a.n + (double)a.eps));
+}
+
+// A row over L = blockDim.x lanes (PER_WAVE: a row per wave).  NV vectors of eight elements a lane stay in
+// registers; longer rows are formed again for their codes.  PACK: codes go to the packed weight layout.
+template <int KIND, int W, int RW, int NV, bool PACK>
+__global__ __launch_bounds__(1024) void k_i8_rows(row_args a, int per_wave)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int L = per_wave ? 64 : blockDim.x, at = per_wave ? lane : threadIdx.x;
+    const long t = per_wave ? (long)blockIdx.x * waves + wave : blockIdx.x;
+    if (t >= (PACK ? a.T_pad : a.T)) return;             // a whole wave, or the whole workgroup
+    const bool real = !PACK || t < a.T;
+    float y[NV][8];
+    raw<8 * W> x[NV];
+    raw<8 * RW> r[NV];
+    float sq = 0.0f;
+    uint32_t m = 0;
+    if (real) {
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int e = 8 * (v * L + at);
+            if (e < a.n) load<KIND, W, RW>(a, t, e, a.n - e, x[v], r[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int e = 8 * (v * L + at);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[v][i] = 0.0f;
+            if (e < a.n) form<KIND, W, RW>(a, x[v], r[v], e, t, a.n - e, true, y[v], sq);
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(y[v][i]) & 0x7FFFFFFFu);
+        }
+        for (int e = 8 * (NV * L + at); e < a.n; e += 8 * L) {
+            float z[8];
+            load<KIND, W, RW>(a, t, e, a.n - e, x[0], r[0]);
+            form<KIND, W, RW>(a, x[0], r[0], e, t, a.n - e, true, z, sq);
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(z[i]) & 0x7FFFFFFFu);
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) {
+        m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+        if constexpr (KIND == NORM || KIND == NORM_RES) sq += __shfl_xor(sq, d, 64);
+    }
+    if (!per_wave && waves > 1) {
+        __shared__ uint32_t ms[16];
+        __shared__ float qs[16];
+        if (lane == 0) {
+            ms[wave] = m;
+            qs[wave] = sq;
+        }
+        __syncthreads();
+        m = 0;
+        sq = 0.0f;
+        for (int i = 0; i < waves; i++) {
+            m = max(m, ms[i]);
+            sq += qs[i];
+        }
+    }
+    const row_step s = step_of(m);
+    // squares that leave fp32, or vanish in it where eps does not stand above them, are summed again in 64 bits
+    float s_factor = 1.0f, mean = sq / (float)a.n;
+    if constexpr (KIND == NORM || KIND == NORM_RES) {
+        if (real && !s.bad && m != 0 && (!(mean < 0x1p100f) || (mean < 0x1p-100f && a.eps < 0x1p-100f)))
+            s_factor = far_factor<KIND, W, RW>(a, t, lane);
+        else s_factor = 1.0f / sqrtf(mean + a.eps);
+    }
+    if (at == 0 && real) {
+        float k = s.most;
+        k *= s_factor;
+        a.scale[t] = s.bad ? NAN : m == 0 ? 0.0f : k / 127.0f;
+    }
+    const int n = PACK ? a.n_pad : a.n;
+    auto put = [&](int e, const float (&z)[8]) {
+        const uint2 c = codes(z, s);
+        if constexpr (PACK) {
+            *(uint2 *)(a.q + i8_at(a.kb, (int)t, e)) = c;
+        } else {
+            int8_t *p = a.q + t * a.q_ld + e;
+            if (a.n - e >= 8) {
+                __builtin_memcpy(p, &c, 8);
+            } else {
+                for (int i = 0; i < a.n - e; i++) p[i] = (int8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+            }
+        }
+    };
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int e = 8 * (v * L + at);
+        if (!real) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[v][i] = 0.0f;
+        }
+        if (e < n) put(e, y[v]);
+    }
+    for (int e = 8 * (NV * L + at); e < n; e += 8 * L) {
+        float z[8] = {}, no = 0.0f;
+        if (real && e < a.n) {
+            if constexpr (KIND == NORM_RES) {            // the stored sum: x or res may be where it went
+                to_f32<RW>(ld8<RW>(a.res_out, t * a.res_out_ld + e, a.n - e), a.res_type, z);
+                float w[8];
+                if (a.w_type == MLLM_F32) to_f32<4>(ld8<4>(a.w, e, a.n - e), a.w_type, w);
+                else to_f32<2>(ld8<2>(a.w, e, a.n - e), a.w_type, w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) z[i] *= w[i];
+            } else {
+                load<KIND, W, RW>(a, t, e, a.n - e, x[0], r[0]);
+                form<KIND, W, RW>(a, x[0], r[0], e, t, a.n - e, false, z, no);
+            }
+        }
+        put(e, z);
+    }
+}
+
+template <int KIND, int W, int RW, bool PACK> void go_rows(const row_args &a, hipStream_t st)
+{
+    const int rows = PACK ? a.T_pad : a.T, n = PACK ? a.n_pad : a.n;
+    const int vecs = (n + 7) / 8;
+    const int per_wave = vecs <= 64;
+    const int threads = vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
+    const int grid = per_wave ? (rows + 3) / 4 : rows;
+    const int nv = per_wave ? 1 : (vecs + threads - 1) / threads;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, a, per_wave); };
+    if (nv <= 1) go(k_i8_rows<KIND, W, RW, 1, PACK>);
+    else if (nv == 2) go(k_i8_rows<KIND, W, RW, 2, PACK>);
+    else go(k_i8_rows<KIND, W, RW, 4, PACK>);
+}
+
+// Integers into the packed layout: a lane moves 16 of them.
+__global__ __launch_bounds__(256) void k_i8_pack(const int8_t *w, long w_ld, int n_rows, int n_cols, long kb, int8_t *packed)
+{
+    const int u = blockIdx.y * 256 + threadIdx.x;        // chunk of 16 columns
+    const int r = blockIdx.x;
+    if (u >= kb * 4) return;
+    raw<16> c{};
+    if (r < n_rows) {
+        const int8_t *p = w + r * w_ld + 16l * u;
+        if (16 * u + 16 <= n_cols) c = ld_any<16>(p);
+        else
+            for (int i = 0; i < n_cols - 16 * u; i++) c.w[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+    }
+    __builtin_memcpy(packed + i8_at(kb, r, 16 * u), &c, 16);
+}
+
+// 16 codes a lane, back to values.
+template <int W>
+__global__ __launch_bounds__(256) void k_i8_dequant(const int8_t *q, long q_ld, const float *scale, int n, int type, void *out,
+                                                    long out_ld, int chunks, long total)
+{
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const long t = i / chunks;
+    const int e = 16 * (int)(i - t * chunks);
+    const float s = scale[t];
+    const int8_t *p = q + t * q_ld + e;
+    if (n - e >= 16) {
+        const raw<16> c = ld_any<16>(p);
+        float y[2][8];
+#pragma unroll
+        for (int j = 0; j < 16; j++) y[j >> 3][j & 7] = (float)(int8_t)(c.w[j >> 2] >> (8 * (j & 3))) * s;
+        st8<W>(out, t * out_ld + e, 8, from_f32<W>(y[0], type));
+        st8<W>(out, t * out_ld + e + 8, 8, from_f32<W>(y[1], type));
+    } else {
+        for (int j = 0; j < n - e; j++) put1(out, t * out_ld + e + j, type, (float)p[j] * s);
+    }
+}
+
+const char *rows_refusal(int type, const void *x, long x_ld, int T, int n, const void *q, long q_ld, const float *scale)
+{
+    if (!i8_real(type)) return "the type is F32, F16 or BF16";
+    if (T < 0 || n <= 0 || n > 1 << 30) return "T is not negative, n positive and at most 2^30";
+    if (x_ld < n || q_ld < n) return "rows lie at least n elements apart";
+    if (T && (!x || !q || !scale)) return "x, q and scale are given";
+    return nullptr;
+}
+
+int done(const char *who) { return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed"); }
+
+} // namespace
+
+extern "C" {
+
+MLLM_API int mllm_i8_quantize(int type, const void *x, long x_ld, int T, int n, int8_t *q, long q_ld, float *scale,
+                              void *stream)
+{
+    const char *who = "mllm_i8_quantize";
+    if (const char *why = rows_refusal(type, x, x_ld, T, n, q, q_ld, scale)) return pk_fail(who, why);
+    if (!T) return 0;
+    row_args a{};
+    a.x = x; a.x_ld = x_ld; a.q = q; a.q_ld = q_ld; a.scale = scale; a.type = type; a.T = T; a.n = n;
+    hipStream_t st = (hipStream_t)stream;
+    type == MLLM_F32 ? go_rows<QUANTIZE, 4, 4, false>(a, st) : go_rows<QUANTIZE, 2, 2, false>(a, st);
+    return done(who);
+}
+
+MLLM_API int mllm_i8_dequant(const int8_t *q, long q_ld, const float *scale, int T, int n, int type, void *out,
+                             long out_ld, void *stream)
+{
+    const char *who = "mllm_i8_dequant";
+    if (const char *why = rows_refusal(type, out, out_ld, T, n, q, q_ld, scale)) return pk_fail(who, why);
+    if (!T) return 0;
+    const int chunks = (n + 15) / 16;
+    const long total = (long)T * chunks;
+    if (total > (1l << 31) * 128) return pk_fail(who, "T * n is at most 2^42");
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, q_ld, scale, n,
+                           type, out, out_ld, chunks, total);
+    };
+    type == MLLM_F32 ? go(k_i8_dequant<4>) : go(k_i8_dequant<2>);
+    return done(who);
+}
+
+MLLM_API int mllm_i8_rms_norm(int type, const void *x, long x_ld, int res_type, const void *res, long res_ld,
+                              void *res_out, long res_out_ld, int w_type, const void *w, float eps, int T, int n,
+                              int8_t *q, long q_ld, float *scale, void *stream)
+{
+    const char *who = "mllm_i8_rms_norm";
+    if (const char *why = rows_refusal(type, x, x_ld, T, n, q, q_ld, scale)) return pk_fail(who, why);
+    if (!i8_real(w_type) || (T && !w)) return pk_fail(who, "w is given, in F32, F16 or BF16");
+    if (!(eps >= 0.0f) || eps > 3.402823466e38f) return pk_fail(who, "eps is finite and not negative");
+    if (res) {
+        if (!i8_real(res_type)) return pk_fail(who, "the type of res is F32, F16 or BF16");
+        if (!res_out || res_ld < n || res_out_ld < n) return pk_fail(who, "res needs res_out, and rows at least n elements apart");
+        if (res_out == res && res_out_ld != res_ld) return pk_fail(who, "res_out may be res only in its stride");
+        if (res_out == x && (res_type != type || res_out_ld != x_ld))
+            return pk_fail(who, "res_out may be x only in its type and stride");
+    }
+    if (!T) return 0;
+    row_args a{};
+    a.x = x; a.x_ld = x_ld; a.res = res; a.res_ld = res_ld; a.res_out = res_out; a.res_out_ld = res_out_ld; a.w = w;
+    a.eps = eps; a.q = q; a.q_ld = q_ld; a.scale = scale; a.type = type; a.res_type = res_type; a.w_type = w_type;
+    a.T = T; a.n = n;
+    hipStream_t st = (hipStream_t)stream;
+    const bool wide = type == MLLM_F32, rwide = res_type == MLLM_F32;
+    if (!res) wide ? go_rows<NORM, 4, 4, false>(a, st) : go_rows<NORM, 2, 2, false>(a, st);
+    else if (wide) rwide ? go_rows<NORM_RES, 4, 4, false>(a, st) : go_rows<NORM_RES, 4, 2, false>(a, st);
+    else rwide ? go_rows<NORM_RES, 2, 4, false>(a, st) : go_rows<NORM_RES, 2, 2, false>(a, st);
+    return done(who);
+}
+
+MLLM_API int mllm_i8_silu_mul(int type, const void *gate, long gate_ld, const void *up, long up_ld, int T, int n,
+                              int8_t *q, long q_ld, float *scale, void *stream)
+{
+    const char *who = "mllm_i8_silu_mul";
+    if (const char *why = rows_refusal(type, gate, gate_ld, T, n, q, q_ld, scale)) return pk_fail(who, why);
+    if (up_ld < n || (T && !up)) return pk_fail(who, "up is given, its rows at least n elements apart");
+    if (!T) return 0;
+    row_args a{};
+    a.x = gate; a.x_ld = gate_ld; a.res = up; a.res_ld = up_ld; a.res_type = type; a.q = q; a.q_ld = q_ld; a.scale = scale;
+    a.type = type; a.T = T; a.n = n;
+    hipStream_t st = (hipStream_t)stream;
+    type == MLLM_F32 ? go_rows<SILU, 4, 4, false>(a, st) : go_rows<SILU, 2, 2, false>(a, st);
+    return done(who);
+}
+
+MLLM_API long mllm_i8_packed_size(int n_rows, int n_cols)
+{
+    if (n_rows <= 0 || n_cols <= 0 || n_cols > kI8MaxCols || n_rows > 1 << 30) return -1;
+    return i8_rblocks(n_rows) * i8_kblocks(n_cols) * 2048;
+}
+
+MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_cols, void *packed, float *scale,
+                          void *stream)
+{
+    const char *who = "mllm_i8_pack";
+    if (mllm_i8_packed_size(n_rows, n_cols) < 0) return pk_fail(who, "n_rows is positive, n_cols from 1 to 131071");
+    if (type != MLLM_I8 && !i8_real(type)) return pk_fail(who, "the type is F32, F16, BF16 or I8");
+    if (!w || !packed || ((uintptr_t)packed & 15) || w_ld < n_cols || (type != MLLM_I8 && !scale))
+        return pk_fail(who, "w, packed (16-byte aligned) and scale are given, rows at least n_cols apart");
+    const long kb = i8_kblocks(n_cols);
+    const int rows = (int)i8_rblocks(n_rows) * 32;
+    hipStream_t st = (hipStream_t)stream;
+    if (type == MLLM_I8) {
+        hipLaunchKernelGGL(k_i8_pack, dim3(rows, (unsigned)((kb * 4 + 255) / 256)), dim3(256), 0, st, (const int8_t *)w, w_ld,
+                           n_rows, n_cols, kb, (int8_t *)packed);
+        return done(who);
+    }
+    row_args a{};
+    a.x = w; a.x_ld = w_ld; a.q = (int8_t *)packed; a.scale = scale; a.type = type; a.T = n_rows; a.n = n_cols; a.kb = kb;
+    a.T_pad = rows; a.n_pad = (int)kb * 64;
+    type == MLLM_F32 ? go_rows<QUANTIZE, 4, 4, true>(a, st) : go_rows<QUANTIZE, 2, 2, true>(a, st);
+    return done(who);
+}
+
+} // extern "C"

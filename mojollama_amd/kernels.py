@@ -56,7 +56,7 @@ class KVView(ctypes.Structure):
 ATTN_CE, ATTN_GQA_C = 0, 1   # CE:141-158 gqa / gqa_attention.c:93 softmax
 
 # Element types, and the layouts and scalings of rotary positions (include/mllm.h).
-T_F32, T_F16, T_BF16, T_E4M3 = range(4)
+T_F32, T_F16, T_BF16, T_E4M3, T_I8 = range(5)
 ROPE_HALF, ROPE_PAIRS = 0, 1
 ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
 _cl = ctypes.c_long
@@ -274,6 +274,24 @@ def load_kernels(path=LIB_PATH):
     so.mllm_pages_compact.restype = ci
     so.mllm_pages_copy.argtypes = [pplane, ci, ci, ci, cvp, cvp, cvp]
     so.mllm_pages_copy.restype = ci
+    # --- layers in 8-bit integers
+    so.mllm_i8_quantize.argtypes = [ci, cvp, _cl, ci, ci, cvp, _cl, cvp, cvp]
+    so.mllm_i8_quantize.restype = ci
+    so.mllm_i8_dequant.argtypes = [cvp, _cl, cvp, ci, ci, ci, cvp, _cl, cvp]
+    so.mllm_i8_dequant.restype = ci
+    so.mllm_i8_rms_norm.argtypes = [ci, cvp, _cl, ci, cvp, _cl, cvp, _cl, ci, cvp, ctypes.c_float, ci, ci, cvp, _cl, cvp,
+                                    cvp]
+    so.mllm_i8_rms_norm.restype = ci
+    so.mllm_i8_silu_mul.argtypes = [ci, cvp, _cl, cvp, _cl, ci, ci, cvp, _cl, cvp, cvp]
+    so.mllm_i8_silu_mul.restype = ci
+    so.mllm_i8_packed_size.argtypes = [ci, ci]
+    so.mllm_i8_packed_size.restype = _cl
+    so.mllm_i8_pack.argtypes = [ci, cvp, _cl, ci, ci, cvp, cvp, cvp]
+    so.mllm_i8_pack.restype = ci
+    so.mllm_i8_gemm_workspace_size.argtypes = [ci, ci, ci]
+    so.mllm_i8_gemm_workspace_size.restype = _cl
+    so.mllm_i8_gemm.argtypes = [cvp, cvp, cvp, _cl, cvp, ci, ci, ci, cvp, ci, cvp, _cl, cvp, _cl, cvp]
+    so.mllm_i8_gemm.restype = ci
     # gptoss_forward (GO:96-130 argument list)
     pcu, pcf, pci = ctypes.POINTER(cu), ctypes.POINTER(cf), ctypes.POINTER(ci)
     so.gptoss_forward.argtypes = ([pci, ci, cf, ci] + [pcu] * 4 + [pcf] * 2 + [pci] * 8 + [cu, ci, ci, ci, cf, cf, pci,
@@ -712,6 +730,142 @@ class DeviceOps:
         self._check(self.so.mllm_pages_copy(planes, len(planes), n_pages, n, self._ints(src, "src", cur),
                                             self._ints(dst, "dst", cur, n), self._raw_stream(cur)), "mllm_pages_copy")
 
+    # ------------------------------------------- layers in 8-bit integers
+    def _mat(self, t, what, cur, T=None, n=None):
+        """(type, address, row stride) of a real [T, n] tensor on the current GPU."""
+        code = self._types.get(t.dtype, T_E4M3)
+        if code == T_E4M3:
+            raise TypeError(f"{what}: {t.dtype} is not served")
+        return code, *self._placed(t, what, cur, T, n)
+
+    def _codes(self, t, what, cur, T, n):
+        """(address, row stride) of an int8 [T, n] tensor on the current GPU."""
+        if t.dtype != self.torch.int8:
+            raise TypeError(f"{what}: {t.dtype}, not int8")
+        return self._placed(t, what, cur, T, n)
+
+    def _placed(self, t, what, cur, T, n):
+        if t.get_device() != cur:
+            self._elsewhere(t, what)
+        if t.dim() != 2 or (T is not None and t.shape[0] != T) or (n is not None and t.shape[1] != n):
+            raise ValueError(f"{what}: [{'T' if T is None else T}, {'n' if n is None else n}] is needed, got {list(t.shape)}")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{what}: the last dimension is not dense")
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+    def _floats(self, t, what, cur, n):
+        """Address of a dense float32 [n] tensor on the current GPU (None: a null pointer)."""
+        if t is None:
+            return None
+        if t.get_device() != cur:
+            self._elsewhere(t, what)
+        if t.dtype != self.torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what}: dense float32 [{n}]")
+        return t.data_ptr()
+
+    def _i8_out(self, q, scale, T, n, cur):
+        """The outputs of the calls that quantise: rows of codes at multiples of 16 bytes, as i8_gemm takes them."""
+        torch = self.torch
+        if q is None:
+            q = torch.empty((T, (n + 15) // 16 * 16), dtype=torch.int8, device="cuda")[:, :n]
+        if scale is None:
+            scale = torch.empty(T, dtype=torch.float32, device="cuda")
+        return q, scale, *self._codes(q, "q", cur, T, n), self._floats(scale, "scale", cur, T)
+
+    def i8_quantize(self, x, q=None, scale=None):
+        """mllm_i8_quantize: x [T, n] (float32, float16 or bfloat16) -> (q int8 [T, n], scale float32 [T])."""
+        cur = self._cur()
+        xt, xp, xl = self._mat(x, "x", cur)
+        T, n = x.shape
+        q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
+        self._check(self.so.mllm_i8_quantize(xt, xp, xl, T, n, qp, ql, sp, self._raw_stream(cur)), "mllm_i8_quantize")
+        return q, scale
+
+    def i8_dequant(self, q, scale, out=None, out_dtype=None):
+        """mllm_i8_dequant: scale[t] * q[t] in out_dtype (None: bfloat16)."""
+        cur = self._cur()
+        T, n = q.shape
+        qp, ql = self._codes(q, "q", cur, T, n)
+        if out is None:
+            out = self.torch.empty((T, n), dtype=out_dtype or self.torch.bfloat16, device="cuda")
+        ot, op, ol = self._mat(out, "out", cur, T, n)
+        self._check(self.so.mllm_i8_dequant(qp, ql, self._floats(scale, "scale", cur, T), T, n, ot, op, ol,
+                                            self._raw_stream(cur)), "mllm_i8_dequant")
+        return out
+
+    def i8_rms_norm(self, x, w, eps, res=None, res_out=None, q=None, scale=None):
+        """mllm_i8_rms_norm: x [T, n] plus the residual stream res (None: none), which goes on in res_out (None: res
+        itself), normed with w [n] -> (q, scale)."""
+        cur = self._cur()
+        xt, xp, xl = self._mat(x, "x", cur)
+        T, n = x.shape
+        rt = rp = op = None
+        rl = ol = 0
+        if res is not None:
+            rt, rp, rl = self._mat(res, "res", cur, T, n)
+            ot, op, ol = (rt, rp, rl) if res_out is None else self._mat(res_out, "res_out", cur, T, n)
+            if ot != rt:
+                raise TypeError("res and res_out have one type")
+        elif res_out is not None:
+            raise ValueError("res_out belongs to res")
+        wt = self._types.get(w.dtype, T_E4M3)
+        if wt == T_E4M3:
+            raise TypeError(f"w: {w.dtype} is not served")
+        if w.get_device() != cur:
+            self._elsewhere(w, "w")
+        if w.numel() != n or not w.is_contiguous():
+            raise ValueError(f"w: dense [{n}]")
+        q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
+        self._check(self.so.mllm_i8_rms_norm(xt, xp, xl, rt or 0, rp, rl, op, ol, wt, w.data_ptr(), eps, T, n, qp, ql, sp,
+                                             self._raw_stream(cur)), "mllm_i8_rms_norm")
+        return q, scale
+
+    def i8_silu_mul(self, gate, up, q=None, scale=None):
+        """mllm_i8_silu_mul: silu(gate) * up, [T, n] each (halves of one tensor may be passed as slices) -> (q, scale)."""
+        cur = self._cur()
+        gt, gp, gl = self._mat(gate, "gate", cur)
+        T, n = gate.shape
+        ut, up_, ul = self._mat(up, "up", cur, T, n)
+        if ut != gt:
+            raise TypeError("gate and up have one type")
+        q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
+        self._check(self.so.mllm_i8_silu_mul(gt, gp, gl, up_, ul, T, n, qp, ql, sp, self._raw_stream(cur)),
+                    "mllm_i8_silu_mul")
+        return q, scale
+
+    def i8_weights(self, w, scale=None):
+        """An I8Weights of w [n_rows, n_cols]: float32, float16 or bfloat16 rows, quantised here (a GGUF matrix through
+        dequant), or int8 rows with their own scale [n_rows]."""
+        return I8Weights(self, w, scale)
+
+    def i8_gemm_workspace(self, weights, T):
+        """A workspace for i8_gemm calls of up to T tokens."""
+        n = self.so.mllm_i8_gemm_workspace_size(T, weights.n_rows, weights.n_cols)
+        if n < 0:
+            raise ValueError("i8_gemm_workspace: sizes that are not served")
+        return self.torch.empty(max(n, 256), dtype=self.torch.uint8, device="cuda")
+
+    def i8_gemm(self, weights, q, scale, bias=None, out=None, out_dtype=None, ws=None):
+        """mllm_i8_gemm: q int8 [T, n_cols] (rows at multiples of 16 bytes, as the calls above make them) with scale
+        float32 [T] -> out [T, n_rows] in out_dtype (None: bfloat16)."""
+        cur = self._cur()
+        self._made_here(cur, weights)
+        T, R = q.shape[0], weights.n_rows
+        qp, ql = self._codes(q, "q", cur, T, weights.n_cols)
+        if T == 1:
+            ql = (ql + 15) // 16 * 16
+        if out is None:
+            out = self.torch.empty((T, R), dtype=out_dtype or self.torch.bfloat16, device="cuda")
+        ot, op, ol = self._mat(out, "out", cur, T, R)
+        if ws is None:
+            ws = self.i8_gemm_workspace(weights, T)
+        elif ws.get_device() != cur:
+            self._elsewhere(ws, "workspace")
+        self._check(self.so.mllm_i8_gemm(weights._packed, weights._scale, qp, ql, self._floats(scale, "scale", cur, T), T, R,
+                                         weights.n_cols, self._floats(bias, "bias", cur, R), ot, op, ol, ws.data_ptr(),
+                                         ws.nbytes, self._raw_stream(cur)), "mllm_i8_gemm")
+        return out
+
     def moe_prepare(self, qts, N, M, E, K, gates, ups, downs, router, renorm):
         """gates/ups/downs: per-expert raw GGUF uint8 tensors (GPU) in the
         reference's layout; router: fp32 [E][N] (GPU).  Returns a MoELayer."""
@@ -790,3 +944,25 @@ class MoELayer:
                 self.ops.so.mllm_moe_release(self.h)
         except Exception:
             pass
+
+
+class I8Weights:
+    """Weights in 8-bit integers with a scale per row (mllm_i8_pack), as DeviceOps.i8_gemm takes them."""
+
+    def __init__(self, ops, w, scale=None):
+        torch, cur = ops.torch, ops._cur()
+        if (w.dtype == torch.int8) != (scale is not None):
+            raise ValueError("scale belongs to int8 weights")
+        if scale is None:
+            code, wp, wl = ops._mat(w, "w", cur)
+        else:
+            code, (wp, wl) = T_I8, ops._codes(w, "w", cur, None, None)
+        self.n_rows, self.n_cols, self._device = w.shape[0], w.shape[1], cur
+        n = ops.so.mllm_i8_packed_size(self.n_rows, self.n_cols)
+        if n < 0:
+            raise ValueError("w: 1 to 131071 columns, at least one row")
+        self.packed = torch.empty(n, dtype=torch.uint8, device="cuda")
+        self.scale = torch.empty(self.n_rows, dtype=torch.float32, device="cuda") if scale is None else scale
+        self._scale, self._packed = ops._floats(self.scale, "scale", cur, self.n_rows), self.packed.data_ptr()
+        ops._check(ops.so.mllm_i8_pack(code, wp, wl, self.n_rows, self.n_cols, self._packed, self._scale,
+                                       ops._raw_stream(cur)), "mllm_i8_pack")
