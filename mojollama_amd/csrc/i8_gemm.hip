@@ -3,29 +3,349 @@
 //
 // out[t][r] = (sum_k x[t][k] w[r][k]) * xs[t] * ws[r] + bias[r]; the sums are whole numbers below 2^31 and
 // exact in any order, so K may be split freely and the result does not depend on how.
+//
+// Both kernels multiply weights (MFMA rows) by tokens (MFMA columns): a lane then holds four neighbouring
+// output channels of one token.
+#include <type_traits>
 #include "i8.h"
 
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
 
 struct gemm_args {
     const int8_t *w, *x;
     const float *ws, *xs, *bias;
     void *out;
-    long x_ld, out_ld, kb;
+    long x_ld, out_ld;
+    int kb;                        // blocks of 64 columns
     int T, R, K, type;
+    int nt, nr;                    // tiles along tokens and rows
+    int splits, per;               // K in `splits` runs of `per` blocks
+    int *part;                     // [split][tile][wave's sums in register order], where splits > 1
 };
+
+template <int N> using I = std::integral_constant<int, N>;
+// f(I<0>{}) .. f(I<N - 1>{}): indexes of register arrays stay constants whatever the loop's size.
+template <int N, int K = 0, class F> __device__ __forceinline__ void each(F &&f)
+{
+    if constexpr (K < N) {
+        f(I<K>{});
+        each<N, K + 1>(f);
+    }
+}
 
 __device__ __forceinline__ float value(int acc, float xs, float ws) { return (float)acc * xs * ws; }
 
-// A wave per 32 weight rows x 32 tokens, operands from global memory.
-__global__ __launch_bounds__(64) void k_i8_gemm(gemm_args a)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, bytes, 0x00020000);
+}
+
+// 16 bytes a lane from r + at + base straight to LDS: 1 KB from `to` on in lane order.
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t r, uint8_t *to, int at, int base)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)to, 16, at, base, 0, 0);
+}
+
+// Vector memory operations younger than n may be under way, no LDS access.
+template <int n> __device__ __forceinline__ void wait_mem()
+{
+    static_assert(n < 64, "vmcnt is six bits");
+    __builtin_amdgcn_s_waitcnt((n & 15) | ((n >> 4) << 14) | 0x0070);
+}
+
+// The order of half a step: READS operand reads and LOADS loads spread over the first half of MUL matrix
+// instructions, so that the operands are there when the next half step begins; and nothing across.
+template <int READS, int MUL, int LOADS> __device__ __forceinline__ void order()
+{
+    each<MUL>([](auto i) __attribute__((always_inline)) {
+        constexpr int H = (MUL + 1) / 2, a = i < H ? i : H, b = i + 1 < H ? i + 1 : H;
+        constexpr int r = b * READS / H - a * READS / H, v = b * LOADS / H - a * LOADS / H;
+        if constexpr (v > 0) __builtin_amdgcn_sched_group_barrier(0x10, v, 0);
+        if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// ------------------------------------------------------------------------------------ the tail
+// NF x 32 output channels from r0 on and 32 tokens from t0 on, from a wave's sums to out: through `room` (wave's own
+// LDS, 32 rows of 32 NF elements + 16 bytes) to whole runs of a token's channels.
+template <int NF, int S> constexpr int room_bytes() { return 32 * (32 * NF * S + 16); }
+
+template <int NF, class T> __device__ __forceinline__ void tail_as(const gemm_args &a, const i32x16 (&acc)[NF], int t0, int r0,
+                                                                   uint8_t *room, int lane)
+{
+    constexpr int S = sizeof(T), LD = 32 * NF * S + 16, PER = 16 / S, LPR = 32 * NF / PER;   // lanes per token's run
+    const int l = lane & 31, h = lane >> 5;
+    const float xs = a.xs[min(t0 + l, a.T - 1)];
+    // the reads of the rows before are done: they are waited for by their stores
+#pragma unroll
+    for (int n = 0; n < NF; n++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int c = 32 * n + 8 * g + 4 * h;
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = min(r0 + c + i, a.R - 1);
+                y[i] = value(acc[n][4 * g + i], xs, a.ws[r]);
+                if (a.bias) y[i] += a.bias[r];
+            }
+            if constexpr (S == 4) {
+                *(f32x4 *)(room + l * LD + c * S) = (f32x4){y[0], y[1], y[2], y[3]};
+            } else {
+                const int type = std::is_same<T, __bf16>::value ? MLLM_BF16 : MLLM_F16;
+                *(uint2 *)(room + l * LD + c * S) = make_uint2(pack16(y[0], y[1], type), pack16(y[2], y[3], type));
+            }
+        }
+    __builtin_amdgcn_wave_barrier();
+    T *out = (T *)a.out;
+#pragma unroll
+    for (int j = 0; j < 32 * LPR / 64; j++) {
+        const int t = (64 * j + lane) / LPR, c = (64 * j + lane) % LPR * PER;
+        const u32x4 v = *(const u32x4 *)(room + t * LD + c * S);
+        if (t0 + t >= a.T) continue;
+        T *p = out + (long)(t0 + t) * a.out_ld + r0 + c;
+        if (r0 + c + PER <= a.R) {
+            __builtin_memcpy(p, &v, 16);
+        } else {
+            const T *e = (const T *)&v;
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (r0 + c + i < a.R) p[i] = e[i];
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int NF> __device__ __forceinline__ void tail(const gemm_args &a, const i32x16 (&acc)[NF], int t0, int r0, uint8_t *room,
+                                                       int lane)
+{
+    if (a.type == MLLM_F32) tail_as<NF, float>(a, acc, t0, r0, room, lane);
+    else if (a.type == MLLM_BF16) tail_as<NF, __bf16>(a, acc, t0, r0, room, lane);
+    else tail_as<NF, _Float16>(a, acc, t0, r0, room, lane);
+}
+
+// ------------------------------------------------------------------------------------ many tokens
+// A workgroup of WM x WN waves makes a tile of 32 MF WM tokens x 32 NF WN rows, a wave 32 MF x 32 NF of it.  K goes by
+// 64 columns a step; both operands come to LDS past the registers, three steps ahead, into four buffers.
+template <int MF, int NF, int WM, int WN> struct tile_of {
+    static constexpr int waves = WM * WN, TT = 32 * MF * WM, TR = 32 * NF * WN;
+    // 1 KB pieces of a step, and a wave's
+    static constexpr int xp = TT / 16, wp = TR / 16, px = xp / waves, pw = wp / waves, per = px + pw;
+    static_assert(xp % waves == 0 && wp % waves == 0, "pieces go evenly to waves");
+    static constexpr int bytes = 1024 * (xp + wp);
+    static constexpr int tail = waves * room_bytes<NF, 4>();
+};
+
+__device__ __forceinline__ int swz(int row) { return ((row >> 1) & 3) ^ ((row >> 3) & 1); }
+
+template <int MF, int NF, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
+{
+    using C = tile_of<MF, NF, WM, WN>;
+    __shared__ __attribute__((aligned(1024))) uint8_t b0[C::bytes], b1[C::bytes], b2[C::bytes], b3[C::bytes];
+    static_assert(C::tail <= C::bytes || C::waves == 4, "");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % WM, wn = wave / WM, l = lane & 31, h = lane >> 5;
+    const int z = __builtin_amdgcn_readfirstlane(blockIdx.x / (a.nt * a.nr)), tile = blockIdx.x - z * a.nt * a.nr;
+    const int ty = __builtin_amdgcn_readfirstlane(tile / a.nt), t0 = (tile - ty * a.nt) * C::TT, r0 = ty * C::TR;
+    const int s_beg = z * a.per, s_end = min(a.kb, s_beg + a.per);      // multiples of four
+
+    // ---- loads: pieces 0 .. xp - 1 are 16 tokens x 64 columns (lane: token lane / 4, slot lane % 4, which holds chunk
+    // slot ^ swz(token)), the others 1 KB of the packed weights
+    const int8_t *xb = a.x + (long)t0 * a.x_ld;
+    const long left = (long)(min(a.T - t0, C::TT) - 1) * a.x_ld + (a.K + 15) / 16 * 16;
+    const __amdgpu_buffer_rsrc_t xr = rsrc(xb, (int)left), wr = rsrc(a.w + (long)(r0 >> 5) * a.kb * 2048, -1);
+    int xo[C::px], wo[C::pw];
+#pragma unroll
+    for (int p = 0; p < C::px; p++) {
+        const int row = 16 * (p * C::waves + wave) + (lane >> 2);
+        xo[p] = row * (int)a.x_ld + 16 * ((lane & 3) ^ swz(row)) + 64 * s_beg;
+    }
+#pragma unroll
+    for (int p = 0; p < C::pw; p++) {
+        const int q = p * C::waves + wave, rb = min(q >> 1, ((a.R - 1) >> 5) - (r0 >> 5));
+        wo[p] = rb * a.kb * 2048 + (q & 1) * 1024 + lane * 16;
+    }
+    int ahead = s_beg;                                       // the next step to load; the last one over and over
+    auto load = [&](uint8_t *to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < C::px; p++)
+            to_lds(xr, to + 1024 * (p * C::waves + wave), xo[p], 0);
+#pragma unroll
+        for (int p = 0; p < C::pw; p++)
+            to_lds(wr, to + 1024 * (C::xp + p * C::waves + wave), wo[p], ahead * 2048);
+        const int more = ahead + 1 < s_end;
+        ahead += more;
+#pragma unroll
+        for (int p = 0; p < C::px; p++) xo[p] += 64 * more;
+    };
+    i32x16 acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[m][n] = i32x16{};
+    // ---- operands of half a step (32 columns)
+    struct frags { i32x4 x[MF], w[NF]; };
+    int xa[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) xa[j] = l * 64 + 16 * ((2 * j + h) ^ swz(l));
+    auto get = [&](const uint8_t *from, auto j, frags &f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NF; n++) f.w[n] = *(const i32x4 *)(from + 1024 * C::xp + (wn * NF + n) * 2048 + j * 1024 + lane * 16);
+#pragma unroll
+        for (int m = 0; m < MF; m++) f.x[m] = *(const i32x4 *)(from + (wm * MF + m) * 2048 + xa[j]);
+    };
+    auto multiply = [&](const frags &f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+            for (int n = 0; n < NF; n++) acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[n], f.x[m], acc[m][n], 0, 0, 0);
+    };
+    frags f0, f1;
+    load(b0);
+    load(b1);
+    load(b2);
+    load(b3);
+    wait_mem<3 * C::per>();
+    __builtin_amdgcn_s_barrier();
+    get(b0, I<0>{}, f0);
+    // A step: its second half's operands are read while the first half multiplies, the next step's first while the
+    // second does.  Between, the loads of the next step have landed for every wave, and nobody reads this step's
+    // buffer any more: it takes the loads of the fourth step from here.
+    auto step = [&](uint8_t *here, const uint8_t *next) __attribute__((always_inline)) {
+        get(here, I<1>{}, f1);
+        multiply(f0);
+        order<MF + NF, MF * NF, 0>();
+        wait_mem<2 * C::per>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        load(here);
+        get(next, I<0>{}, f0);
+        multiply(f1);
+        order<MF + NF, MF * NF, C::per>();
+    };
+    for (int s = s_beg; s < s_end; s += 4) {
+        step(b0, b1);
+        step(b1, b2);
+        step(b2, b3);
+        step(b3, b0);
+    }
+    wait_mem<0>();
+    __builtin_amdgcn_s_barrier();
+
+    if (a.splits > 1) {
+        int *p = a.part + (((long)z * a.nt * a.nr + tile) * C::waves + wave) * (MF * NF * 1024) + lane * 4;
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+            for (int n = 0; n < NF; n++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *(i32x4 *)(p + ((m * NF + n) * 4 + g) * 256) =
+                        (i32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
+        return;
+    }
+    uint8_t *room = wave == 0 ? b0 : wave == 1 ? b1 : wave == 2 ? b2 : b3;
+    each<MF>([&](auto m) __attribute__((always_inline)) {
+        tail<NF>(a, acc[m], t0 + (wm * MF + m) * 32, r0 + wn * NF * 32, room, lane);
+    });
+}
+
+// The sums of all splits, and the tail.
+template <int MF, int NF, int WM, int WN> __global__ __launch_bounds__(64) void k_i8_join(gemm_args a)
+{
+    using C = tile_of<MF, NF, WM, WN>;
+    __shared__ __attribute__((aligned(16))) uint8_t room[room_bytes<NF, 4>()];
+    const int lane = threadIdx.x;
+    const int m = blockIdx.x % MF, wave = blockIdx.x / MF % C::waves, tile = blockIdx.x / (MF * C::waves);
+    const int wm = wave % WM, wn = wave / WM;
+    const int t = tile % a.nt * C::TT + (wm * MF + m) * 32, r = tile / a.nt * C::TR + wn * NF * 32;
+    if (t >= a.T || r >= a.R) return;
+    i32x16 acc[NF];
+#pragma unroll
+    for (int n = 0; n < NF; n++) acc[n] = i32x16{};
+    const int *p = a.part + ((long)tile * C::waves + wave) * (MF * NF * 1024) + m * NF * 1024 + lane * 4;
+    for (int z = 0; z < a.splits; z++, p += (long)a.nt * a.nr * C::waves * MF * NF * 1024)
+#pragma unroll
+        for (int n = 0; n < NF; n++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const i32x4 v = *(const i32x4 *)(p + (n * 4 + g) * 256);
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[n][4 * g + i] += v[i];
+            }
+    tail<NF>(a, acc, t, r, room, lane);
+}
+
+// ------------------------------------------------------------------------------------ few tokens
+// 16 weight rows x 16 TF tokens a workgroup of W waves, which take blocks of 64 columns in turn and join their sums in
+// LDS.  Weights stream from memory straight into the matrix cores, each byte once; x comes from the caches.
+template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
+{
+    constexpr int D = TF == 1 ? 8 : TF == 2 ? 4 : 2;               // blocks under way
+    __shared__ __attribute__((aligned(16))) int sums[W][TF][64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, c = lane >> 4;
+    const int r0 = blockIdx.x * 16;
+    const int8_t *w = a.w + (long)(r0 >> 5) * a.kb * 2048 + (r0 & 16) * 16 + c * 512 + l * 16;
+    const __amdgpu_buffer_rsrc_t xr = rsrc(a.x, (int)((a.T - 1) * a.x_ld + (a.K + 15) / 16 * 16));
+    int xo[TF];
+#pragma unroll
+    for (int f = 0; f < TF; f++) xo[f] = 16 * f + l < a.T ? (16 * f + l) * (int)a.x_ld + 16 * c : 0x7FFFFF00;
+    i32x4 acc[TF] = {};
+    for (int b = wave; b < a.kb; b += W * D) {
+        i32x4 wf[D], xf[D][TF];
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            const int k = min(b + d * W, a.kb - 1);
+            wf[d] = *(const i32x4 *)(w + (long)k * 2048);
+#pragma unroll
+            for (int f = 0; f < TF; f++)
+                xf[d][f] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, 16 * f + l < a.T ? xo[f] + 64 * k : xo[f], 0, 0));
+        }
+#pragma unroll
+        for (int d = 0; d < D; d++)
+            if (b + d * W < a.kb) {
+#pragma unroll
+                for (int f = 0; f < TF; f++) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d], xf[d][f], acc[f], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int f = 0; f < TF; f++) *(i32x4 *)sums[wave][f][lane] = acc[f];
+    __syncthreads();
+    // lane: token f * 16 + l, rows 4 c + i
+    for (int f = wave; f < TF; f += W) {
+        const int t = 16 * f + l;
+        i32x4 s = {};
+#pragma unroll
+        for (int i = 0; i < W; i++) s += *(const i32x4 *)sums[i][f][lane];
+        if (t >= a.T) continue;
+        const float xs = a.xs[t];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = r0 + 4 * c + i;
+            if (r < a.R) {
+                const float y = value(s[i], xs, a.ws[r]);
+                put1(a.out, t * a.out_ld + r, a.type, a.bias ? y + a.bias[r] : y);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ rows far apart
+// Rows of x so far apart that a tile's offsets leave 32 bits: a wave per 32 weight rows x 32 tokens, operands from
+// global memory.
+__global__ __launch_bounds__(64) void k_i8_far(gemm_args a)
 {
     const int lane = threadIdx.x, l = lane & 31, h = lane >> 5;
-    const int r0 = blockIdx.x * 32, t0 = blockIdx.y * 32;
-    const int8_t *w = a.w + (r0 >> 5) * a.kb * 2048 + lane * 16;
+    const unsigned tile = blockIdx.x;
+    const int r0 = (int)(tile / a.nt) * 32, t0 = (int)(tile % a.nt) * 32;
+    const int8_t *w = a.w + (long)(r0 >> 5) * a.kb * 2048 + lane * 16;
     const int8_t *x = a.x + (long)min(t0 + l, a.T - 1) * a.x_ld;
     const int last = (a.K - 1) / 16 * 16;
     i32x16 acc = {};
@@ -44,6 +364,24 @@ __global__ __launch_bounds__(64) void k_i8_gemm(gemm_args a)
         const float y = value(acc[i], xs, a.ws[r]);
         put1(a.out, t * a.out_ld + r, a.type, a.bias ? y + a.bias[r] : y);
     }
+}
+
+// ------------------------------------------------------------------------------------ the choice
+struct plan { int few, kind, nt, nr, splits, per; long part; };
+
+plan plan_of(int T, int R, int kb)
+{
+    plan p{};
+    if (T <= 64) {
+        p.few = 1;
+        p.kind = T <= 16 ? 1 : T <= 32 ? 2 : 4;
+        return p;
+    }
+    p.nt = (T + 255) / 256;
+    p.nr = (R + 255) / 256;
+    p.splits = 1;
+    p.per = kb;
+    return p;
 }
 
 } // namespace
@@ -72,10 +410,28 @@ MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t
     const long need = mllm_i8_gemm_workspace_size(T, n_rows, n_cols);
     if (need > 0 && (!workspace || ws_bytes < need)) return pk_fail(who, "the workspace is too small");
     if (!T) return 0;
-    gemm_args a{(const int8_t *)packed, x, w_scale, x_scale, bias, out, x_ld, out_ld, i8_kblocks(n_cols), T, n_rows, n_cols,
-                type};
-    hipLaunchKernelGGL(k_i8_gemm, dim3((unsigned)i8_rblocks(n_rows), (unsigned)((T + 31l) / 32)), dim3(64), 0,
-                       (hipStream_t)stream, a);
+    const int kb = (int)i8_kblocks(n_cols);
+    plan p = plan_of(T, n_rows, kb);
+    const bool far = x_ld >= 1l << 22;                       // 256 rows and a step more stay below 2^31
+    if (far) {
+        p.nt = (T + 31) / 32;
+        p.nr = (n_rows + 31) / 32;
+        p.splits = 1;
+    }
+    if ((long)p.nt * p.nr * p.splits > 1l << 31) return pk_fail(who, "T * n_rows is too large for one call");
+    gemm_args a{(const int8_t *)packed, x, w_scale, x_scale, bias, out, x_ld, out_ld, kb, T, n_rows, n_cols, type,
+                p.nt, p.nr, p.splits, p.per, (int *)workspace};
+    hipStream_t st = (hipStream_t)stream;
+    if (far) {
+        hipLaunchKernelGGL(k_i8_far, dim3((unsigned)((long)p.nt * p.nr)), dim3(64), 0, st, a);
+    } else if (p.few) {
+        const dim3 grid((n_rows + 15) / 16);
+        if (p.kind == 1) hipLaunchKernelGGL((k_i8_few<1, 8>), grid, dim3(512), 0, st, a);
+        else if (p.kind == 2) hipLaunchKernelGGL((k_i8_few<2, 8>), grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((k_i8_few<4, 8>), grid, dim3(512), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((k_i8_tiles<4, 4, 2, 2>), dim3((unsigned)(p.nt * p.nr * p.splits)), dim3(256), 0, st, a);
+    }
     return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed");
 }
 
