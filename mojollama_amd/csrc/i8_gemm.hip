@@ -57,13 +57,13 @@ template <int n> __device__ __forceinline__ void wait_mem()
     __builtin_amdgcn_s_waitcnt((n & 15) | ((n >> 4) << 14) | 0x0070);
 }
 
-// The order of half a step: READS operand reads and LOADS loads spread over the first half of MUL matrix
-// instructions, so that the operands are there when the next half step begins; and nothing across.
+// The order of half a step: LOADS loads spread over MUL matrix instructions, READS operand reads over the first half
+// of them, so that the operands are there when the next half begins; and nothing across.
 template <int READS, int MUL, int LOADS> __device__ __forceinline__ void order()
 {
     each<MUL>([](auto i) __attribute__((always_inline)) {
         constexpr int H = (MUL + 1) / 2, a = i < H ? i : H, b = i + 1 < H ? i + 1 : H;
-        constexpr int r = b * READS / H - a * READS / H, v = b * LOADS / H - a * LOADS / H;
+        constexpr int r = b * READS / H - a * READS / H, v = (i + 1) * LOADS / MUL - i * LOADS / MUL;
         if constexpr (v > 0) __builtin_amdgcn_sched_group_barrier(0x10, v, 0);
         if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
@@ -72,134 +72,189 @@ template <int READS, int MUL, int LOADS> __device__ __forceinline__ void order()
 }
 
 // ------------------------------------------------------------------------------------ the tail
-// NF x 32 output channels from r0 on and 32 tokens from t0 on, from a wave's sums to out: through `room` (wave's own
-// LDS, 32 rows of 32 NF elements + 16 bytes) to whole runs of a token's channels.
-template <int NF, int S> constexpr int room_bytes() { return 32 * (32 * NF * S + 16); }
-
-template <int NF, class T> __device__ __forceinline__ void tail_as(const gemm_args &a, const i32x16 (&acc)[NF], int t0, int r0,
-                                                                   uint8_t *room, int lane)
+// What the tail needs of a tile of TT tokens and TR rows, in LDS from the start.
+template <int TT, int TR> struct scales {
+    float ws[TR], bias[TR], xs[TT];
+};
+// Asked for before the loop's loads, stored behind them: nothing waits for them alone.  IDS lanes share the work.
+template <int TT, int TR, int IDS> struct scales_of {
+    float ws[(TR + IDS - 1) / IDS], bias[(TR + IDS - 1) / IDS], xs[(TT + IDS - 1) / IDS];
+};
+template <int TT, int TR, int IDS> __device__ __forceinline__ void get_scales(const gemm_args &a, int t0, int r0,
+                                                                              scales_of<TT, TR, IDS> &s, int id)
 {
-    constexpr int S = sizeof(T), LD = 32 * NF * S + 16, PER = 16 / S, LPR = 32 * NF / PER;   // lanes per token's run
-    const int l = lane & 31, h = lane >> 5;
-    const float xs = a.xs[min(t0 + l, a.T - 1)];
-    // the reads of the rows before are done: they are waited for by their stores
 #pragma unroll
-    for (int n = 0; n < NF; n++)
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int c = 32 * n + 8 * g + 4 * h;
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = min(r0 + c + i, a.R - 1);
-                y[i] = value(acc[n][4 * g + i], xs, a.ws[r]);
-                if (a.bias) y[i] += a.bias[r];
-            }
-            if constexpr (S == 4) {
-                *(f32x4 *)(room + l * LD + c * S) = (f32x4){y[0], y[1], y[2], y[3]};
-            } else {
-                const int type = std::is_same<T, __bf16>::value ? MLLM_BF16 : MLLM_F16;
-                *(uint2 *)(room + l * LD + c * S) = make_uint2(pack16(y[0], y[1], type), pack16(y[2], y[3], type));
-            }
-        }
-    __builtin_amdgcn_wave_barrier();
-    T *out = (T *)a.out;
-#pragma unroll
-    for (int j = 0; j < 32 * LPR / 64; j++) {
-        const int t = (64 * j + lane) / LPR, c = (64 * j + lane) % LPR * PER;
-        const u32x4 v = *(const u32x4 *)(room + t * LD + c * S);
-        if (t0 + t >= a.T) continue;
-        T *p = out + (long)(t0 + t) * a.out_ld + r0 + c;
-        if (r0 + c + PER <= a.R) {
-            __builtin_memcpy(p, &v, 16);
-        } else {
-            const T *e = (const T *)&v;
-#pragma unroll
-            for (int i = 0; i < PER; i++)
-                if (r0 + c + i < a.R) p[i] = e[i];
-        }
+    for (int i = 0; i < (TR + IDS - 1) / IDS; i++) {
+        const int r = min(r0 + i * IDS + id, a.R - 1);
+        s.ws[i] = a.ws[r];
+        s.bias[i] = a.bias ? a.bias[r] : -0.0f;              // y + -0 is y, -0 too
     }
-    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < (TT + IDS - 1) / IDS; i++) s.xs[i] = a.xs[min(t0 + i * IDS + id, a.T - 1)];
+}
+template <int TT, int TR, int IDS> __device__ __forceinline__ void put_scales(const scales_of<TT, TR, IDS> &s, scales<TT, TR> &to,
+                                                                              int id)
+{
+#pragma unroll
+    for (int i = 0; i < (TR + IDS - 1) / IDS; i++)
+        if (i * IDS + id < TR) {
+            to.ws[i * IDS + id] = s.ws[i];
+            to.bias[i * IDS + id] = s.bias[i];
+        }
+#pragma unroll
+    for (int i = 0; i < (TT + IDS - 1) / IDS; i++)
+        if (i * IDS + id < TT) to.xs[i * IDS + id] = s.xs[i];
 }
 
-template <int NF> __device__ __forceinline__ void tail(const gemm_args &a, const i32x16 (&acc)[NF], int t0, int r0, uint8_t *room,
-                                                       int lane)
+// A wave's sums of 32 tokens x 32 NF output channels to out, by way of `room`, its own LDS: there the channels of a
+// token lie side by side, and a lane scales and stores eight of them, in whole lines.  The code is short (the sums
+// pass through LDS as integers, the rest is a loop): a tail of straight code took as long as 40 steps of K, most of it
+// for its instructions.
+template <int NF> constexpr int room_bytes() { return 32 * 128 * NF; }
+// Byte of four channels (chunk c) of token t there: eight tokens' chunks of one number meet distinct banks.
+template <int NF> __device__ __forceinline__ int room_at(int t, int c) { return t * 128 * NF + ((c ^ (t & 7)) << 4); }
+
+template <int NF, class T> __device__ __forceinline__ void tail_as(const gemm_args &a, int t0, int r0, const uint8_t *room,
+                                                                   const float *xs, const float (&ws)[8], const float (&bias)[8],
+                                                                   int lane)
 {
-    if (a.type == MLLM_F32) tail_as<NF, float>(a, acc, t0, r0, room, lane);
-    else if (a.type == MLLM_BF16) tail_as<NF, __bf16>(a, acc, t0, r0, room, lane);
-    else tail_as<NF, _Float16>(a, acc, t0, r0, room, lane);
+    constexpr int LPR = 4 * NF, TPW = 64 / LPR;              // lanes of a token, tokens of a pass
+    constexpr int type = sizeof(T) == 4 ? MLLM_F32 : std::is_same<T, __bf16>::value ? MLLM_BF16 : MLLM_F16;
+    const int c = lane % LPR * 8, t = lane / LPR;
+    T *to = (T *)a.out + (long)(t0 + t) * a.out_ld + r0 + c;
+    auto form = [&](int t, float (&y)[8]) __attribute__((always_inline)) {
+        const i32x4 u = *(const i32x4 *)(room + room_at<NF>(t, c >> 2)), v = *(const i32x4 *)(room + room_at<NF>(t, (c >> 2) + 1));
+        const float x = xs[t];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = value(i < 4 ? u[i] : v[i - 4], x, ws[i]) + bias[i];
+    };
+    if (t0 + 32 <= a.T && r0 + 32 * NF <= a.R) {
+#pragma unroll 4
+        for (int j = 0; j < 32 / TPW; j++, to += TPW * a.out_ld) {
+            float y[8];
+            form(t + j * TPW, y);
+            if constexpr (sizeof(T) == 4) {
+                __builtin_memcpy(to, y, 32);
+            } else {
+                const u32x4 w = {pack16(y[0], y[1], type), pack16(y[2], y[3], type), pack16(y[4], y[5], type), pack16(y[6], y[7], type)};
+                __builtin_memcpy(to, &w, 16);
+            }
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int j = t; j < min(32, a.T - t0); j += TPW, to += TPW * a.out_ld) {
+        float y[8];
+        form(j, y);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (r0 + c + i < a.R) to[i] = (T)y[i];
+    }
+}
+
+// All MF x 32 tokens of a wave, 32 at a time, in a loop that stays one (the sums of a turn, by constant index, in a
+// case of their own).
+template <int MF, int NF> __device__ __forceinline__ void tail(const gemm_args &a, const i32x16 (&acc)[MF][NF], int t0, int r0,
+                                                               uint8_t *room, const float *xs, const float (&ws)[8],
+                                                               const float (&bias)[8], int lane)
+{
+    const int l = lane & 31, h = lane >> 5;
+#pragma unroll 1
+    for (int m = 0; m < MF; m++, t0 += 32, xs += 32) {
+        __builtin_amdgcn_wave_barrier();                     // the reads before are done
+        each<MF>([&](auto k) __attribute__((always_inline)) {
+            if (k != m) return;
+#pragma unroll
+            for (int n = 0; n < NF; n++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *(i32x4 *)(room + room_at<NF>(l, 8 * n + 2 * g + h)) =
+                        (i32x4){acc[k][n][4 * g], acc[k][n][4 * g + 1], acc[k][n][4 * g + 2], acc[k][n][4 * g + 3]};
+        });
+        __builtin_amdgcn_wave_barrier();
+        if (a.type == MLLM_F32) tail_as<NF, float>(a, t0, r0, room, xs, ws, bias, lane);
+        else if (a.type == MLLM_BF16) tail_as<NF, __bf16>(a, t0, r0, room, xs, ws, bias, lane);
+        else tail_as<NF, _Float16>(a, t0, r0, room, xs, ws, bias, lane);
+    }
 }
 
 // ------------------------------------------------------------------------------------ many tokens
 // A workgroup of WM x WN waves makes a tile of 32 MF WM tokens x 32 NF WN rows, a wave 32 MF x 32 NF of it.  K goes by
-// 64 columns a step; both operands come to LDS past the registers, three steps ahead, into four buffers.
+// 64 columns a step.  Both operands come to LDS past the registers: the weights of a step into one of four buffers, up
+// to four steps ahead; x for two steps at once, so that a row is read in whole lines of 128 bytes (64 bytes at a time
+// cost twice the L2 traffic), into one of two.
 template <int MF, int NF, int WM, int WN> struct tile_of {
     static constexpr int waves = WM * WN, TT = 32 * MF * WM, TR = 32 * NF * WN;
-    // 1 KB pieces of a step, and a wave's
-    static constexpr int xp = TT / 16, wp = TR / 16, px = xp / waves, pw = wp / waves, per = px + pw;
+    // 1 KB pieces of two steps of x, of a step of weights, and a wave's
+    static constexpr int xp = TT / 8, wp = TR / 16, px = xp / waves, pw = wp / waves;
     static_assert(xp % waves == 0 && wp % waves == 0, "pieces go evenly to waves");
-    static constexpr int bytes = 1024 * (xp + wp);
-    static constexpr int tail = waves * room_bytes<NF, 4>();
 };
 
-__device__ __forceinline__ int swz(int row) { return ((row >> 1) & 3) ^ ((row >> 3) & 1); }
+// Slot of a row's chunk of 16 bytes is chunk ^ swz(row): the reads of 16 rows, one chunk each, meet distinct banks.
+__device__ __forceinline__ int swz(int row) { return (row ^ (row >> 3 & 3)) & 7; }
 
 template <int MF, int NF, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
 {
     using C = tile_of<MF, NF, WM, WN>;
-    __shared__ __attribute__((aligned(1024))) uint8_t b0[C::bytes], b1[C::bytes], b2[C::bytes], b3[C::bytes];
-    static_assert(C::tail <= C::bytes || C::waves == 4, "");
+    // buffers of their own each: the compiler then knows which loads a read may meet
+    __shared__ __attribute__((aligned(1024))) uint8_t x0[C::xp * 1024], x1[C::xp * 1024], w0[C::wp * 1024], w1[C::wp * 1024],
+        w2[C::wp * 1024], w3[C::wp * 1024];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM, l = lane & 31, h = lane >> 5;
     const int z = __builtin_amdgcn_readfirstlane(blockIdx.x / (a.nt * a.nr)), tile = blockIdx.x - z * a.nt * a.nr;
     const int ty = __builtin_amdgcn_readfirstlane(tile / a.nt), t0 = (tile - ty * a.nt) * C::TT, r0 = ty * C::TR;
     const int s_beg = z * a.per, s_end = min(a.kb, s_beg + a.per);      // multiples of four
+    __shared__ scales<C::TT, C::TR> sc;
+    scales_of<C::TT, C::TR, 64 * C::waves> have;
+    if (a.splits == 1) get_scales(a, t0, r0, have, threadIdx.x);
 
-    // ---- loads: pieces 0 .. xp - 1 are 16 tokens x 64 columns (lane: token lane / 4, slot lane % 4, which holds chunk
-    // slot ^ swz(token)), the others 1 KB of the packed weights
+    // ---- loads: a piece of x is 8 tokens x 128 columns (lane: token lane / 8, slot lane % 8), of the weights 1 KB as
+    // they lie.  What lies behind the last row of x is not read, what lies behind a row meets weights of zero.
     const int8_t *xb = a.x + (long)t0 * a.x_ld;
     const long left = (long)(min(a.T - t0, C::TT) - 1) * a.x_ld + (a.K + 15) / 16 * 16;
     const __amdgpu_buffer_rsrc_t xr = rsrc(xb, (int)left), wr = rsrc(a.w + (long)(r0 >> 5) * a.kb * 2048, -1);
     int xo[C::px], wo[C::pw];
 #pragma unroll
     for (int p = 0; p < C::px; p++) {
-        const int row = 16 * (p * C::waves + wave) + (lane >> 2);
-        xo[p] = row * (int)a.x_ld + 16 * ((lane & 3) ^ swz(row)) + 64 * s_beg;
+        const int row = 8 * (p * C::waves + wave) + (lane >> 3);
+        xo[p] = row * (int)a.x_ld + 16 * ((lane & 7) ^ swz(row)) + 64 * s_beg;
     }
 #pragma unroll
     for (int p = 0; p < C::pw; p++) {
         const int q = p * C::waves + wave, rb = min(q >> 1, ((a.R - 1) >> 5) - (r0 >> 5));
         wo[p] = rb * a.kb * 2048 + (q & 1) * 1024 + lane * 16;
     }
-    int ahead = s_beg;                                       // the next step to load; the last one over and over
-    auto load = [&](uint8_t *to) __attribute__((always_inline)) {
+    int xs = s_beg, ws = s_beg;                              // the next steps to load; the last ones over and over
+    auto load_x = [&](uint8_t *to) __attribute__((always_inline)) {
+        const int more = xs + 2 < s_end;
 #pragma unroll
-        for (int p = 0; p < C::px; p++)
+        for (int p = 0; p < C::px; p++) {
             to_lds(xr, to + 1024 * (p * C::waves + wave), xo[p], 0);
+            xo[p] += 128 * more;
+        }
+        xs += 2 * more;
+    };
+    auto load_w = [&](uint8_t *to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < C::pw; p++)
-            to_lds(wr, to + 1024 * (C::xp + p * C::waves + wave), wo[p], ahead * 2048);
-        const int more = ahead + 1 < s_end;
-        ahead += more;
-#pragma unroll
-        for (int p = 0; p < C::px; p++) xo[p] += 64 * more;
+        for (int p = 0; p < C::pw; p++) to_lds(wr, to + 1024 * (p * C::waves + wave), wo[p], ws * 2048);
+        ws += ws + 1 < s_end;
     };
     i32x16 acc[MF][NF];
 #pragma unroll
     for (int m = 0; m < MF; m++)
 #pragma unroll
         for (int n = 0; n < NF; n++) acc[m][n] = i32x16{};
-    // ---- operands of half a step (32 columns)
+    // ---- operands of half a step (32 columns), j: which of the four of a pair of steps
     struct frags { i32x4 x[MF], w[NF]; };
-    int xa[2];
+    int xa[4];
 #pragma unroll
-    for (int j = 0; j < 2; j++) xa[j] = l * 64 + 16 * ((2 * j + h) ^ swz(l));
-    auto get = [&](const uint8_t *from, auto j, frags &f) __attribute__((always_inline)) {
+    for (int j = 0; j < 4; j++) xa[j] = l * 128 + 16 * ((2 * j + h) ^ swz(l));
+    auto get = [&](const uint8_t *fx, const uint8_t *fw, auto j, frags &f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NF; n++) f.w[n] = *(const i32x4 *)(from + 1024 * C::xp + (wn * NF + n) * 2048 + j * 1024 + lane * 16);
+        for (int n = 0; n < NF; n++) f.w[n] = *(const i32x4 *)(fw + (wn * NF + n) * 2048 + (j & 1) * 1024 + lane * 16);
 #pragma unroll
-        for (int m = 0; m < MF; m++) f.x[m] = *(const i32x4 *)(from + (wm * MF + m) * 2048 + xa[j]);
+        for (int m = 0; m < MF; m++) f.x[m] = *(const i32x4 *)(fx + (wm * MF + m) * 4096 + xa[j]);
     };
     auto multiply = [&](const frags &f) __attribute__((always_inline)) {
 #pragma unroll
@@ -208,34 +263,50 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
             for (int n = 0; n < NF; n++) acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[n], f.x[m], acc[m][n], 0, 0, 0);
     };
     frags f0, f1;
-    load(b0);
-    load(b1);
-    load(b2);
-    load(b3);
-    wait_mem<3 * C::per>();
+    auto then = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+    load_x(x0);
+    load_w(w0);
+    then();
+    load_w(w1);
+    then();
+    load_w(w2);
+    then();
+    load_x(x1);
+    then();
+    if (a.splits == 1) put_scales(have, sc, threadIdx.x);
+    wait_mem<2 * C::pw + C::px>();
     __builtin_amdgcn_s_barrier();
-    get(b0, I<0>{}, f0);
+    get(x0, w0, I<0>{}, f0);
     // A step: its second half's operands are read while the first half multiplies, the next step's first while the
-    // second does.  Between, the loads of the next step have landed for every wave, and nobody reads this step's
-    // buffer any more: it takes the loads of the fourth step from here.
-    auto step = [&](uint8_t *here, const uint8_t *next) __attribute__((always_inline)) {
-        get(here, I<1>{}, f1);
+    // second does.  Between, the loads that the next step needs have landed for every wave, and nobody reads this step's
+    // buffers any more.  Loads are spread evenly: the first half of an even step asks for weights (into the buffer of
+    // the step before), the second for weights again (its own), the second half of an odd step for x of the second
+    // pair from here.  So under way may be, in the middle of an even step, whose next needs the weights of the first
+    // half two steps ago: weights, x, weights; in the middle of an odd step, whose next needs x of two steps ago:
+    // weights twice.  The order of loads within a half has no part in this.
+    auto step = [&](auto odd, uint8_t *x_here, const uint8_t *x_next, uint8_t *w_before, uint8_t *w_here, const uint8_t *w_next)
+                    __attribute__((always_inline)) {
+        if constexpr (!odd) load_w(w_before);
+        get(x_here, w_here, I<2 * odd + 1>{}, f1);
         multiply(f0);
-        order<MF + NF, MF * NF, 0>();
-        wait_mem<2 * C::per>();
+        order<MF + NF, MF * NF, odd ? 0 : C::pw>();
+        wait_mem<odd ? 2 * C::pw : 2 * C::pw + C::px>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        load(here);
-        get(next, I<0>{}, f0);
+        if constexpr (odd) load_x(x_here);
+        else load_w(w_here);
+        get(x_next, w_next, I<odd ? 0 : 2>{}, f0);
         multiply(f1);
-        order<MF + NF, MF * NF, C::per>();
+        order<MF + NF, MF * NF, odd ? C::px : C::pw>();
     };
-    for (int s = s_beg; s < s_end; s += 4) {
-        step(b0, b1);
-        step(b1, b2);
-        step(b2, b3);
-        step(b3, b0);
-    }
+    int s = s_beg;
+    do {
+        step(I<0>{}, x0, x0, w3, w0, w1);
+        step(I<1>{}, x0, x1, w0, w1, w2);
+        step(I<0>{}, x1, x1, w1, w2, w3);
+        step(I<1>{}, x1, x0, w2, w3, w0);
+        s += 4;
+    } while (s < s_end);
     wait_mem<0>();
     __builtin_amdgcn_s_barrier();
 
@@ -251,25 +322,37 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
                         (i32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
         return;
     }
-    uint8_t *room = wave == 0 ? b0 : wave == 1 ? b1 : wave == 2 ? b2 : b3;
-    each<MF>([&](auto m) __attribute__((always_inline)) {
-        tail<NF>(a, acc[m], t0 + (wm * MF + m) * 32, r0 + wn * NF * 32, room, lane);
-    });
+    static_assert(C::waves == 4 && 2 * room_bytes<NF>() <= C::xp * 1024, "the tail of two waves fits a buffer of x");
+    uint8_t *room = (wave < 2 ? x0 : x1) + (wave & 1) * room_bytes<NF>();
+    const int c = wn * NF * 32 + lane % (4 * NF) * 8;
+    float rs[8], bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        rs[i] = sc.ws[c + i];
+        bias[i] = sc.bias[c + i];
+    }
+    const int t = wm * MF * 32;
+    tail<MF, NF>(a, acc, t0 + t, r0 + wn * NF * 32, room, sc.xs + t, rs, bias, lane);
 }
 
 // The sums of all splits, and the tail.
 template <int MF, int NF, int WM, int WN> __global__ __launch_bounds__(64) void k_i8_join(gemm_args a)
 {
     using C = tile_of<MF, NF, WM, WN>;
-    __shared__ __attribute__((aligned(16))) uint8_t room[room_bytes<NF, 4>()];
+    __shared__ __attribute__((aligned(16))) uint8_t room[room_bytes<NF>()];
     const int lane = threadIdx.x;
     const int m = blockIdx.x % MF, wave = blockIdx.x / MF % C::waves, tile = blockIdx.x / (MF * C::waves);
     const int wm = wave % WM, wn = wave / WM;
     const int t = tile % a.nt * C::TT + (wm * MF + m) * 32, r = tile / a.nt * C::TR + wn * NF * 32;
     if (t >= a.T || r >= a.R) return;
-    i32x16 acc[NF];
+    __shared__ scales<32, 32 * NF> sc;
+    scales_of<32, 32 * NF, 64> have;
+    get_scales(a, t, r, have, lane);
+    put_scales(have, sc, lane);
+    __syncthreads();
+    i32x16 acc[1][NF];
 #pragma unroll
-    for (int n = 0; n < NF; n++) acc[n] = i32x16{};
+    for (int n = 0; n < NF; n++) acc[0][n] = i32x16{};
     const int *p = a.part + ((long)tile * C::waves + wave) * (MF * NF * 1024) + m * NF * 1024 + lane * 4;
     for (int z = 0; z < a.splits; z++, p += (long)a.nt * a.nr * C::waves * MF * NF * 1024)
 #pragma unroll
@@ -278,9 +361,16 @@ template <int MF, int NF, int WM, int WN> __global__ __launch_bounds__(64) void 
             for (int g = 0; g < 4; g++) {
                 const i32x4 v = *(const i32x4 *)(p + (n * 4 + g) * 256);
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[n][4 * g + i] += v[i];
+                for (int i = 0; i < 4; i++) acc[0][n][4 * g + i] += v[i];
             }
-    tail<NF>(a, acc, t, r, room, lane);
+    const int c = lane % (4 * NF) * 8;
+    float rs[8], bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        rs[i] = sc.ws[c + i];
+        bias[i] = sc.bias[c + i];
+    }
+    tail<1, NF>(a, acc, t, r, room, sc.xs, rs, bias, lane);
 }
 
 // ------------------------------------------------------------------------------------ few tokens
