@@ -6,6 +6,7 @@
 //
 // Both kernels multiply weights (MFMA rows) by tokens (MFMA columns): a lane then holds four neighbouring
 // output channels of one token.
+#include <algorithm>
 #include <type_traits>
 #include "i8.h"
 
@@ -24,6 +25,7 @@ struct gemm_args {
     int T, R, K, type;
     int nt, nr;                    // tiles along tokens and rows
     int splits, per;               // K in `splits` runs of `per` blocks
+    int panel;
     int *part;                     // [split][tile][wave's sums in register order], where splits > 1
 };
 
@@ -179,6 +181,22 @@ template <int MF, int NF> __device__ __forceinline__ void tail(const gemm_args &
 }
 
 // ------------------------------------------------------------------------------------ many tokens
+// Workgroup b of n runs on XCD b % 8: each XCD takes one run of the tiles, in panels of a.panel tiles of tokens with
+// the rows in turn inside, so that the tiles it works on at a time are a block of the output and share both operands
+// in its L2.
+struct work_tile { int z, t, r; };
+__device__ __forceinline__ work_tile tile_at(const gemm_args &a, int b, int n)
+{
+    const int xcd = b & 7;
+    int i = xcd * (n >> 3) + min(xcd, n & 7) + (b >> 3);
+    const int z = __builtin_amdgcn_readfirstlane(i / (a.nt * a.nr));
+    i -= z * a.nt * a.nr;
+    const int p = __builtin_amdgcn_readfirstlane(i / (a.panel * a.nr)), wide = min(a.panel, a.nt - p * a.panel);
+    i -= p * a.panel * a.nr;
+    const int r = __builtin_amdgcn_readfirstlane(i / wide);
+    return {z, p * a.panel + i - r * wide, r};
+}
+
 // A workgroup of WM x WN waves makes a tile of 32 MF WM tokens x 32 NF WN rows, a wave 32 MF x 32 NF of it.  K goes by
 // 64 columns a step.  Both operands come to LDS past the registers: the weights of a step into one of four buffers, up
 // to four steps ahead; x for two steps at once, so that a row is read in whole lines of 128 bytes (64 bytes at a time
@@ -193,8 +211,8 @@ template <int MF, int NF, int WM, int WN> struct tile_of {
 // Slot of a row's chunk of 16 bytes is chunk ^ swz(row): the reads of 16 rows, one chunk each, meet distinct banks.
 __device__ __forceinline__ int swz(int row) { return (row ^ (row >> 3 & 3)) & 7; }
 
-template <int MF, int NF, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
+template <int MF, int NF, int WM, int WN, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_i8_tiles(gemm_args a)
 {
     using C = tile_of<MF, NF, WM, WN>;
     // buffers of their own each: the compiler then knows which loads a read may meet
@@ -202,8 +220,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
         w2[C::wp * 1024], w3[C::wp * 1024];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM, l = lane & 31, h = lane >> 5;
-    const int z = __builtin_amdgcn_readfirstlane(blockIdx.x / (a.nt * a.nr)), tile = blockIdx.x - z * a.nt * a.nr;
-    const int ty = __builtin_amdgcn_readfirstlane(tile / a.nt), t0 = (tile - ty * a.nt) * C::TT, r0 = ty * C::TR;
+    const work_tile wt = tile_at(a, blockIdx.x, gridDim.x);
+    const int z = wt.z, tile = wt.r * a.nt + wt.t, t0 = wt.t * C::TT, r0 = wt.r * C::TR;
     const int s_beg = z * a.per, s_end = min(a.kb, s_beg + a.per);      // multiples of four
     __shared__ scales<C::TT, C::TR> sc;
     scales_of<C::TT, C::TR, 64 * C::waves> have;
@@ -322,8 +340,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_i8_tiles(gemm_args a)
                         (i32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
         return;
     }
-    static_assert(C::waves == 4 && 2 * room_bytes<NF>() <= C::xp * 1024, "the tail of two waves fits a buffer of x");
-    uint8_t *room = (wave < 2 ? x0 : x1) + (wave & 1) * room_bytes<NF>();
+    static_assert(C::waves == 4 && room_bytes<NF>() <= C::wp * 1024, "the tail of a wave fits a buffer of weights");
+    uint8_t *room = wave == 0 ? w0 : wave == 1 ? w1 : wave == 2 ? w2 : w3;
     const int c = wn * NF * 32 + lane % (4 * NF) * 8;
     float rs[8], bias[8];
 #pragma unroll
@@ -378,7 +396,7 @@ template <int MF, int NF, int WM, int WN> __global__ __launch_bounds__(64) void 
 // LDS.  Weights stream from memory straight into the matrix cores, each byte once; x comes from the caches.
 template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
 {
-    constexpr int D = TF == 1 ? 8 : TF == 2 ? 4 : 2;               // blocks under way
+    constexpr int D = 2;                                     // blocks under way a wave
     __shared__ __attribute__((aligned(16))) int sums[W][TF][64][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, c = lane >> 4;
     const int r0 = blockIdx.x * 16;
@@ -457,21 +475,77 @@ __global__ __launch_bounds__(64) void k_i8_far(gemm_args a)
 }
 
 // ------------------------------------------------------------------------------------ the choice
-struct plan { int few, kind, nt, nr, splits, per; long part; };
-
-plan plan_of(int T, int R, int kb)
+struct tile_kind {
+    int TT, TR, per_cu;            // workgroups of it that a CU holds
+    float step, each, tail;        // microseconds of a step of K, of each workgroup in it, of a workgroup beside
+    void (*go)(const gemm_args &, int grid, hipStream_t);
+    bool fits(int T) const { return TT < 64 || TT < 2 * T; }             // not mostly empty
+    long at_once() const { return 256l * per_cu; }                       // workgroups that the GPU holds: splits go no further
+};
+constexpr int kMostSplits = 12;
+template <int MF, int NF, int WM, int WN, int OCC> void go_tiles(const gemm_args &a, int grid, hipStream_t st)
 {
-    plan p{};
-    if (T <= 64) {
-        p.few = 1;
-        p.kind = T <= 16 ? 1 : T <= 32 ? 2 : 4;
-        return p;
+    hipLaunchKernelGGL((k_i8_tiles<MF, NF, WM, WN, OCC>), dim3(grid), dim3(64 * WM * WN), 0, st, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL((k_i8_join<MF, NF, WM, WN>), dim3(a.nt * a.nr * MF * WM * WN), dim3(64), 0, st, a);
+}
+template <int MF, int NF, int WM, int WN, int OCC> constexpr tile_kind kind_of(float step, float each, float tail)
+{
+    using C = tile_of<MF, NF, WM, WN>;
+    return {C::TT, C::TR, OCC, step, each, tail, go_tiles<MF, NF, WM, WN, OCC>};
+}
+const tile_kind kinds[] = {
+    kind_of<4, 4, 2, 2, 1>(0.0906f, 0.507f, 10.09f),
+    kind_of<2, 4, 2, 2, 1>(0.0899f, 0.2054f, 6.625f),
+    kind_of<2, 2, 2, 2, 2>(0.0f, 0.2337f, 1.912f),
+    kind_of<1, 2, 2, 2, 3>(0.0f, 0.1574f, 1.201f),
+    kind_of<1, 1, 1, 4, 3>(0.0422f, 0.0907f, 1.022f)};
+
+struct plan {
+    const tile_kind *kind;         // null: few tokens
+    int nt, nr, splits, per;
+};
+
+plan plan_of(int T, int R, int kb, int cols)
+{
+    plan best{};
+    float least = INFINITY;
+    if (T <= 32) {
+        const int n = (R + 15) / 16, turns = (cols + 1023) / 1024;
+        least = 2.925f + (n + 511) / 512 * (0.9204f + turns * 0.3931f) + turns * (n / 512.0f) * 0.5291f * ((T <= 16 ? 1 : 2) + 0.3911f);
     }
-    p.nt = (T + 255) / 256;
-    p.nr = (R + 255) / 256;
-    p.splits = 1;
-    p.per = kb;
-    return p;
+    const int quads = kb / 4;
+    for (const tile_kind &k : kinds) {
+        if (!k.fits(T)) continue;
+        for (int want : {1, 2, 3, 4, 6, 8, kMostSplits}) {
+            plan p{&k, (T + k.TT - 1) / k.TT, (R + k.TR - 1) / k.TR, 0, 0};
+            if (want > quads) continue;
+            p.per = (quads + want - 1) / want * 4;
+            p.splits = (kb + p.per - 1) / p.per;
+            const long n = (long)p.nt * p.nr * want;
+            if (p.splits != want || n > (want > 1 ? k.at_once() : 1l << 30)) continue;
+            const int most = (int)((n + 255) / 256), full = most / k.per_cu, rest = most % k.per_cu;
+            float us = full * (p.per * (k.step + k.per_cu * k.each) + k.tail) + (rest ? p.per * (k.step + rest * k.each) + k.tail : 0.0f);
+            us = 3.088f + std::max(us, (float)cols * ((float)R + T) / 10.28e6f);
+            if (want > 1) us += 3.422f + (float)n * k.TT * k.TR * 8 / 6.818e6f;
+            if (us < least) {
+                least = us;
+                best = p;
+            }
+        }
+    }
+    return best;
+}
+
+// Bytes of the sums of any plan with splits for T tokens or fewer.
+long sums_of(int T, int R, int kb)
+{
+    long most = 0;
+    for (const tile_kind &k : kinds) {
+        const long nr = (R + k.TR - 1) / k.TR, n = std::min((long)std::min(kb / 4, kMostSplits) * ((T + k.TT - 1) / k.TT) * nr, k.at_once());
+        if (k.fits(T) && kb > 4 && 2 * nr <= k.at_once()) most = std::max(most, n * k.TT * k.TR * 4);
+    }
+    return most;
 }
 
 } // namespace
@@ -481,7 +555,7 @@ extern "C" {
 MLLM_API long mllm_i8_gemm_workspace_size(int T, int n_rows, int n_cols)
 {
     if (T < 0 || mllm_i8_packed_size(n_rows, n_cols) < 0) return -1;
-    return 0;
+    return T ? sums_of(T, n_rows, (int)i8_kblocks(n_cols)) : 0;
 }
 
 MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t *x, long x_ld, const float *x_scale,
@@ -501,26 +575,27 @@ MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t
     if (need > 0 && (!workspace || ws_bytes < need)) return pk_fail(who, "the workspace is too small");
     if (!T) return 0;
     const int kb = (int)i8_kblocks(n_cols);
-    plan p = plan_of(T, n_rows, kb);
     const bool far = x_ld >= 1l << 22;                       // 256 rows and a step more stay below 2^31
-    if (far) {
-        p.nt = (T + 31) / 32;
-        p.nr = (n_rows + 31) / 32;
-        p.splits = 1;
-    }
-    if ((long)p.nt * p.nr * p.splits > 1l << 31) return pk_fail(who, "T * n_rows is too large for one call");
+    const plan p = plan_of(T, n_rows, kb, n_cols);
     gemm_args a{(const int8_t *)packed, x, w_scale, x_scale, bias, out, x_ld, out_ld, kb, T, n_rows, n_cols, type,
-                p.nt, p.nr, p.splits, p.per, (int *)workspace};
+                p.nt, p.nr, p.splits, p.per, p.nt < 4 ? p.nt : 4, (int *)workspace};
     hipStream_t st = (hipStream_t)stream;
     if (far) {
-        hipLaunchKernelGGL(k_i8_far, dim3((unsigned)((long)p.nt * p.nr)), dim3(64), 0, st, a);
-    } else if (p.few) {
-        const dim3 grid((n_rows + 15) / 16);
-        if (p.kind == 1) hipLaunchKernelGGL((k_i8_few<1, 8>), grid, dim3(512), 0, st, a);
-        else if (p.kind == 2) hipLaunchKernelGGL((k_i8_few<2, 8>), grid, dim3(512), 0, st, a);
-        else hipLaunchKernelGGL((k_i8_few<4, 8>), grid, dim3(512), 0, st, a);
+        a.nt = (T + 31) / 32;
+        a.nr = (n_rows + 31) / 32;
+        if ((long)a.nt * a.nr > 1l << 30) return pk_fail(who, "T * n_rows is too large for one call");
+        hipLaunchKernelGGL(k_i8_far, dim3(a.nt * a.nr), dim3(64), 0, st, a);
+    } else if (p.kind) {
+        p.kind->go(a, p.nt * p.nr * p.splits, st);
+    } else if (T <= 32) {
+        const int grid = (n_rows + 15) / 16;
+        auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, st, a); };
+        // many workgroups hide each other's ends: eight waves each then (32000 x 2048, one token: 17.3 -> 14.9 us), few
+        // are done sooner with sixteen (2048 x 5632: 7.0 -> 5.4 us)
+        if (grid > 1024) T <= 16 ? go(k_i8_few<1, 8>, 8) : go(k_i8_few<2, 8>, 8);
+        else T <= 16 ? go(k_i8_few<1, 16>, 16) : go(k_i8_few<2, 16>, 16);
     } else {
-        hipLaunchKernelGGL((k_i8_tiles<4, 4, 2, 2>), dim3((unsigned)(p.nt * p.nr * p.splits)), dim3(256), 0, st, a);
+        return pk_fail(who, "T * n_rows is too large for one call");
     }
     return hipGetLastError() == hipSuccess ? 0 : pk_fail(who, "the launch failed");
 }
