@@ -337,6 +337,9 @@ class DeviceOps:
         import torch
         self.torch = torch
         self.so = so or load_kernels()
+        # the current device as the runtime has it (no call here makes it the first to ask: tensors are there by then)
+        self._cur_raw = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self._reals = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
         self._types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}
 
     def _stream(self):
@@ -731,27 +734,30 @@ class DeviceOps:
                                             self._ints(dst, "dst", cur, n), self._raw_stream(cur)), "mllm_pages_copy")
 
     # ------------------------------------------- layers in 8-bit integers
-    def _mat(self, t, what, cur, T=None, n=None):
-        """(type, address, row stride) of a real [T, n] tensor on the current GPU."""
-        code = self._types.get(t.dtype, T_E4M3)
-        if code == T_E4M3:
+    # (a call's own time is that of a launch, so the checks of a tensor that is as it should be are few)
+    def _real(self, t, what):
+        """mllm type of a float32, float16 or bfloat16 tensor."""
+        code = self._reals.get(t.dtype)
+        if code is None:
             raise TypeError(f"{what}: {t.dtype} is not served")
-        return code, *self._placed(t, what, cur, T, n)
+        return code
+
+    def _at(self, t, what, cur, T, n):
+        """(address, row stride) of a [T, n] tensor on the current GPU (cur) whose last dimension is dense."""
+        st = t.stride()
+        if t.shape != (T, n) or t.get_device() != cur or (st[1] != 1 and n > 1):
+            if t.get_device() != cur:
+                self._elsewhere(t, what)
+            if t.shape != (T, n):
+                raise ValueError(f"{what}: [{T}, {n}] is needed, got {list(t.shape)}")
+            raise ValueError(f"{what}: the last dimension is not dense")
+        return t.data_ptr(), st[0] if T > 1 else n
 
     def _codes(self, t, what, cur, T, n):
-        """(address, row stride) of an int8 [T, n] tensor on the current GPU."""
+        """_at of int8."""
         if t.dtype != self.torch.int8:
             raise TypeError(f"{what}: {t.dtype}, not int8")
-        return self._placed(t, what, cur, T, n)
-
-    def _placed(self, t, what, cur, T, n):
-        if t.get_device() != cur:
-            self._elsewhere(t, what)
-        if t.dim() != 2 or (T is not None and t.shape[0] != T) or (n is not None and t.shape[1] != n):
-            raise ValueError(f"{what}: [{'T' if T is None else T}, {'n' if n is None else n}] is needed, got {list(t.shape)}")
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"{what}: the last dimension is not dense")
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+        return self._at(t, what, cur, T, n)
 
     def _floats(self, t, what, cur, n):
         """Address of a dense float32 [n] tensor on the current GPU (None: a null pointer)."""
@@ -763,74 +769,88 @@ class DeviceOps:
             raise ValueError(f"{what}: dense float32 [{n}]")
         return t.data_ptr()
 
+    @staticmethod
+    def _sizes(t, what):
+        if t.dim() != 2:
+            raise ValueError(f"{what}: [tokens, elements], got {list(t.shape)}")
+        return t.shape
+
     def _i8_out(self, q, scale, T, n, cur):
         """The outputs of the calls that quantise: rows of codes at multiples of 16 bytes, as i8_gemm takes them."""
-        torch = self.torch
         if q is None:
-            q = torch.empty((T, (n + 15) // 16 * 16), dtype=torch.int8, device="cuda")[:, :n]
+            q = self.torch.empty((T, (n + 15) // 16 * 16), dtype=self.torch.int8, device="cuda")[:, :n]
         if scale is None:
-            scale = torch.empty(T, dtype=torch.float32, device="cuda")
-        return q, scale, *self._codes(q, "q", cur, T, n), self._floats(scale, "scale", cur, T)
+            scale = self.torch.empty(T, dtype=self.torch.float32, device="cuda")
+        qp, ql = self._codes(q, "q", cur, T, n)
+        return q, scale, qp, ql, self._floats(scale, "scale", cur, T)
 
     def i8_quantize(self, x, q=None, scale=None):
         """mllm_i8_quantize: x [T, n] (float32, float16 or bfloat16) -> (q int8 [T, n], scale float32 [T])."""
-        cur = self._cur()
-        xt, xp, xl = self._mat(x, "x", cur)
-        T, n = x.shape
+        cur, xt = self._cur_raw(), self._real(x, "x")
+        T, n = self._sizes(x, "x")
+        xp, xl = self._at(x, "x", cur, T, n)
         q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
-        self._check(self.so.mllm_i8_quantize(xt, xp, xl, T, n, qp, ql, sp, self._raw_stream(cur)), "mllm_i8_quantize")
+        rc = self.so.mllm_i8_quantize(xt, xp, xl, T, n, qp, ql, sp, self._raw_stream(cur))
+        if rc:
+            self._check(rc, "mllm_i8_quantize")
         return q, scale
 
     def i8_dequant(self, q, scale, out=None, out_dtype=None):
         """mllm_i8_dequant: scale[t] * q[t] in out_dtype (None: bfloat16)."""
-        cur = self._cur()
-        T, n = q.shape
+        cur = self._cur_raw()
+        T, n = self._sizes(q, "q")
         qp, ql = self._codes(q, "q", cur, T, n)
         if out is None:
             out = self.torch.empty((T, n), dtype=out_dtype or self.torch.bfloat16, device="cuda")
-        ot, op, ol = self._mat(out, "out", cur, T, n)
-        self._check(self.so.mllm_i8_dequant(qp, ql, self._floats(scale, "scale", cur, T), T, n, ot, op, ol,
-                                            self._raw_stream(cur)), "mllm_i8_dequant")
+        ot = self._real(out, "out")
+        op, ol = self._at(out, "out", cur, T, n)
+        rc = self.so.mllm_i8_dequant(qp, ql, self._floats(scale, "scale", cur, T), T, n, ot, op, ol, self._raw_stream(cur))
+        if rc:
+            self._check(rc, "mllm_i8_dequant")
         return out
 
     def i8_rms_norm(self, x, w, eps, res=None, res_out=None, q=None, scale=None):
         """mllm_i8_rms_norm: x [T, n] plus the residual stream res (None: none), which goes on in res_out (None: res
         itself), normed with w [n] -> (q, scale)."""
-        cur = self._cur()
-        xt, xp, xl = self._mat(x, "x", cur)
-        T, n = x.shape
-        rt = rp = op = None
-        rl = ol = 0
+        cur, xt, wt = self._cur_raw(), self._real(x, "x"), self._real(w, "w")
+        T, n = self._sizes(x, "x")
+        xp, xl = self._at(x, "x", cur, T, n)
+        rt = rl = ol = 0
+        rp = op = None
         if res is not None:
-            rt, rp, rl = self._mat(res, "res", cur, T, n)
-            ot, op, ol = (rt, rp, rl) if res_out is None else self._mat(res_out, "res_out", cur, T, n)
-            if ot != rt:
-                raise TypeError("res and res_out have one type")
+            rt = self._real(res, "res")
+            rp, rl = self._at(res, "res", cur, T, n)
+            if res_out is None:
+                op, ol = rp, rl
+            else:
+                op, ol = self._at(res_out, "res_out", cur, T, n)
+                if res_out.dtype != res.dtype:
+                    raise TypeError("res and res_out have one type")
         elif res_out is not None:
             raise ValueError("res_out belongs to res")
-        wt = self._types.get(w.dtype, T_E4M3)
-        if wt == T_E4M3:
-            raise TypeError(f"w: {w.dtype} is not served")
         if w.get_device() != cur:
             self._elsewhere(w, "w")
         if w.numel() != n or not w.is_contiguous():
             raise ValueError(f"w: dense [{n}]")
         q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
-        self._check(self.so.mllm_i8_rms_norm(xt, xp, xl, rt or 0, rp, rl, op, ol, wt, w.data_ptr(), eps, T, n, qp, ql, sp,
-                                             self._raw_stream(cur)), "mllm_i8_rms_norm")
+        rc = self.so.mllm_i8_rms_norm(xt, xp, xl, rt, rp, rl, op, ol, wt, w.data_ptr(), eps, T, n, qp, ql, sp,
+                                      self._raw_stream(cur))
+        if rc:
+            self._check(rc, "mllm_i8_rms_norm")
         return q, scale
 
     def i8_silu_mul(self, gate, up, q=None, scale=None):
         """mllm_i8_silu_mul: silu(gate) * up, [T, n] each (halves of one tensor may be passed as slices) -> (q, scale)."""
-        cur = self._cur()
-        gt, gp, gl = self._mat(gate, "gate", cur)
-        T, n = gate.shape
-        ut, up_, ul = self._mat(up, "up", cur, T, n)
-        if ut != gt:
+        cur, gt = self._cur_raw(), self._real(gate, "gate")
+        T, n = self._sizes(gate, "gate")
+        gp, gl = self._at(gate, "gate", cur, T, n)
+        if self._real(up, "up") != gt:
             raise TypeError("gate and up have one type")
+        up_, ul = self._at(up, "up", cur, T, n)
         q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
-        self._check(self.so.mllm_i8_silu_mul(gt, gp, gl, up_, ul, T, n, qp, ql, sp, self._raw_stream(cur)),
-                    "mllm_i8_silu_mul")
+        rc = self.so.mllm_i8_silu_mul(gt, gp, gl, up_, ul, T, n, qp, ql, sp, self._raw_stream(cur))
+        if rc:
+            self._check(rc, "mllm_i8_silu_mul")
         return q, scale
 
     def i8_weights(self, w, scale=None):
@@ -848,22 +868,26 @@ class DeviceOps:
     def i8_gemm(self, weights, q, scale, bias=None, out=None, out_dtype=None, ws=None):
         """mllm_i8_gemm: q int8 [T, n_cols] (rows at multiples of 16 bytes, as the calls above make them) with scale
         float32 [T] -> out [T, n_rows] in out_dtype (None: bfloat16)."""
-        cur = self._cur()
-        self._made_here(cur, weights)
-        T, R = q.shape[0], weights.n_rows
+        cur, R = self._cur_raw(), weights.n_rows
+        if weights._device != cur:
+            self._made_here(cur, weights)
+        T = self._sizes(q, "q")[0]
         qp, ql = self._codes(q, "q", cur, T, weights.n_cols)
-        if T == 1:
+        if T <= 1:
             ql = (ql + 15) // 16 * 16
         if out is None:
             out = self.torch.empty((T, R), dtype=out_dtype or self.torch.bfloat16, device="cuda")
-        ot, op, ol = self._mat(out, "out", cur, T, R)
+        ot = self._real(out, "out")
+        op, ol = self._at(out, "out", cur, T, R)
         if ws is None:
             ws = self.i8_gemm_workspace(weights, T)
         elif ws.get_device() != cur:
             self._elsewhere(ws, "workspace")
-        self._check(self.so.mllm_i8_gemm(weights._packed, weights._scale, qp, ql, self._floats(scale, "scale", cur, T), T, R,
-                                         weights.n_cols, self._floats(bias, "bias", cur, R), ot, op, ol, ws.data_ptr(),
-                                         ws.nbytes, self._raw_stream(cur)), "mllm_i8_gemm")
+        rc = self.so.mllm_i8_gemm(weights._packed, weights._scale, qp, ql, self._floats(scale, "scale", cur, T), T, R,
+                                  weights.n_cols, self._floats(bias, "bias", cur, R), ot, op, ol, ws.data_ptr(), ws.nbytes,
+                                  self._raw_stream(cur))
+        if rc:
+            self._check(rc, "mllm_i8_gemm")
         return out
 
     def moe_prepare(self, qts, N, M, E, K, gates, ups, downs, router, renorm):
@@ -953,11 +977,9 @@ class I8Weights:
         torch, cur = ops.torch, ops._cur()
         if (w.dtype == torch.int8) != (scale is not None):
             raise ValueError("scale belongs to int8 weights")
-        if scale is None:
-            code, wp, wl = ops._mat(w, "w", cur)
-        else:
-            code, (wp, wl) = T_I8, ops._codes(w, "w", cur, None, None)
-        self.n_rows, self.n_cols, self._device = w.shape[0], w.shape[1], cur
+        self.n_rows, self.n_cols = ops._sizes(w, "w")
+        code, self._device = T_I8 if scale is not None else ops._real(w, "w"), cur
+        wp, wl = ops._at(w, "w", cur, self.n_rows, self.n_cols)
         n = ops.so.mllm_i8_packed_size(self.n_rows, self.n_cols)
         if n < 0:
             raise ValueError("w: 1 to 131071 columns, at least one row")
