@@ -5,6 +5,8 @@
 // in registers; the codes are rounded from there: memory is read and written once, which is what bounds
 // these kernels.  The norm's factor 1 / sqrt(mean + eps) is one number per row: it enters the scale alone,
 // and the codes do not wait for it.
+#include <algorithm>
+#include <type_traits>
 #include "i8.h"
 
 namespace {
@@ -37,12 +39,14 @@ template <int W> __device__ __forceinline__ raw<8 * W> ld8(const void *p, long a
     }
     return r;
 }
-template <int W> __device__ __forceinline__ void to_f32(const raw<8 * W> &r, int type, float (&x)[8])
+constexpr int size_of(int type) { return type == MLLM_F32 ? 4 : 2; }
+template <int TYPE> using raw8 = raw<8 * size_of(TYPE)>;
+template <int TYPE> __device__ __forceinline__ void to_f32(const raw8<TYPE> &r, float (&x)[8])
 {
-    if constexpr (W == 4) {
+    if constexpr (TYPE == MLLM_F32) {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = __uint_as_float(r.w[i]);
-    } else if (type == MLLM_BF16) {
+    } else if constexpr (TYPE == MLLM_BF16) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[2 * i] = __uint_as_float(r.w[i] << 16);
@@ -57,15 +61,20 @@ template <int W> __device__ __forceinline__ void to_f32(const raw<8 * W> &r, int
         }
     }
 }
-template <int W> __device__ __forceinline__ raw<8 * W> from_f32(const float (&x)[8], int type)
+template <int TYPE> __device__ __forceinline__ raw8<TYPE> from_f32(const float (&x)[8])
 {
-    raw<8 * W> r;
-    if constexpr (W == 4) {
+    raw8<TYPE> r;
+    if constexpr (TYPE == MLLM_F32) {
 #pragma unroll
         for (int i = 0; i < 8; i++) r.w[i] = __float_as_uint(x[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) r.w[i] = pack16(x[2 * i], x[2 * i + 1], type);
+        for (int i = 0; i < 4; i++) {
+            float a = x[2 * i], b = x[2 * i + 1];
+            // a sum or product is a number of 32 bits before it is one of 16: the compiler would round some of them once
+            if constexpr (TYPE == MLLM_F16) asm("" : "+v"(a), "+v"(b));
+            r.w[i] = pack16(a, b, TYPE);
+        }
     }
     return r;
 }
@@ -83,6 +92,22 @@ template <int W> __device__ __forceinline__ void st8(void *p, long at, int left,
         }
 }
 
+// The largest |y|, gathered as bits: of the positive numbers as signed, of the negative as unsigned integers (one
+// instruction for two elements each, and infinities and NaNs come out on top).
+struct top {
+    int pos = 0;
+    uint32_t neg = 0;
+    __device__ __forceinline__ void add(const float (&y)[8])
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            pos = max(max(pos, __float_as_int(y[i])), __float_as_int(y[i + 1]));
+            neg = max(max(neg, __float_as_uint(y[i])), __float_as_uint(y[i + 1]));
+        }
+    }
+    __device__ __forceinline__ uint32_t get() const { return max((uint32_t)pos, neg >> 31 ? neg & 0x7FFFFFFFu : 0u); }
+};
+
 // The step of a row: m is the largest |y| as fp32 bits, above or at those of infinity where the row holds an
 // infinity or a NaN.  Codes are rint(y * pre * inv), inv = 127 * (1 / (most * pre)); the power of two pre keeps
 // the reciprocal a normal number at either end of fp32.
@@ -96,16 +121,39 @@ __device__ __forceinline__ row_step step_of(uint32_t m)
     s.inv = s.bad || m == 0 ? 0.0f : 1.0f / (s.most * s.pre) * 127.0f;
     return s;
 }
-__device__ __forceinline__ uint32_t code(float y, const row_step &s)
+// The nearest integer of f, |f| <= 127, is the low byte of f + 1.5 * 2^23 (ties to even, as the sum rounds).
+__device__ __forceinline__ uint32_t four(float a, float b, float c, float d)
 {
-    return s.bad ? 0u : (uint32_t)(int)rintf(y * s.pre * s.inv) & 0xFFu;
+#pragma clang fp contract(off)
+    constexpr float M = 12582912.0f;
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b + M), __float_as_uint(a + M), 0x0C0C0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(d + M), __float_as_uint(c + M), 0x04000C0Cu);
+    return lo | hi;
 }
 __device__ __forceinline__ uint2 codes(const float (&y)[8], const row_step &s)
 {
-    uint32_t w[2] = {0, 0};
+#pragma clang fp contract(off)                               // the product rounds before the sum that makes it whole
+    if (s.bad) return make_uint2(0, 0);
+    float f[8];
+    if (s.pre != 1.0f) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) w[i >> 2] |= code(y[i], s) << (8 * (i & 3));
-    return make_uint2(w[0], w[1]);
+        for (int i = 0; i < 8; i++) f[i] = y[i] * s.pre * s.inv;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = y[i] * s.inv;
+    }
+    return make_uint2(four(f[0], f[1], f[2], f[3]), four(f[4], f[5], f[6], f[7]));
+}
+
+// g / d, 1 <= d <= 2^100: the reciprocal with one Newton step, the quotient with its remainder taken back (the rounded
+// quotient but for about one in a million, there its neighbour), in six instructions for the ten of a division that
+// serves every number.
+__device__ __forceinline__ float quotient(float g, float d)
+{
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    const float q = g * r;
+    return fmaf(fmaf(-d, q, g), r, q);
 }
 
 enum { QUANTIZE, NORM, NORM_RES, SILU };
@@ -117,60 +165,84 @@ struct row_args {
     int8_t *q;
     float *scale;
     float eps;
-    int type, res_type, w_type, T, n;
+    int w_type, T, n;
     long kb;                       // packed weights: blocks along K (q then is the packed matrix)
     int n_pad, T_pad;
 };
 
+template <int TYPE> __device__ __forceinline__ void times(const void *w, int e, int left, float (&y)[8])
+{
+    float f[8];
+    to_f32<TYPE>(ld8<size_of(TYPE)>(w, e, left), f);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] *= f[i];
+}
+__device__ __forceinline__ void weigh(const row_args &a, int e, int left, float (&y)[8])
+{
+    if (a.w_type == MLLM_F32) times<MLLM_F32>(a.w, e, left, y);
+    else if (a.w_type == MLLM_BF16) times<MLLM_BF16>(a.w, e, left, y);
+    else times<MLLM_F16>(a.w, e, left, y);
+}
+
 // y of elements e .. e + 7 of row t; sq gains the squares of h.
-template <int KIND, int W, int RW>
-__device__ __forceinline__ void form(const row_args &a, const raw<8 * W> &xr, const raw<8 * RW> &rr, int e, long t, int left,
+template <int KIND, int XT, int RT>
+__device__ __forceinline__ void form(const row_args &a, const raw8<XT> &xr, const raw8<RT> &rr, int e, long t, int left,
                                      bool store, float (&y)[8], float &sq)
 {
-    to_f32<W>(xr, a.type, y);
+    to_f32<XT>(xr, y);
     if constexpr (KIND == SILU) {
-        float u[8];
-        to_f32<RW>(rr, a.res_type, u);
+        float u[8], g[8], least = 0.0f;
+        to_f32<RT>(rr, u);
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = y[i] / (1.0f + expf(-y[i])) * u[i];
+        for (int i = 0; i < 8; i++) {
+            g[i] = y[i];
+            least = fminf(least, g[i]);
+            y[i] = quotient(g[i], 1.0f + expf(-g[i]));
+        }
+        // far below zero, where e^-g goes out of the quotient's reach, 1 + e^-g is e^-g
+        if (__any(least < -69.0f)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float h = expf(0.5f * g[i]);
+                y[i] = g[i] < -69.0f ? g[i] * h * h : y[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] *= u[i];
     }
     if constexpr (KIND == NORM_RES) {
         float r[8];
-        to_f32<RW>(rr, a.res_type, r);
+        to_f32<RT>(rr, r);
 #pragma unroll
         for (int i = 0; i < 8; i++) y[i] += r[i];
-        const raw<8 * RW> h = from_f32<RW>(y, a.res_type);
-        if (store) st8<RW>(a.res_out, t * a.res_out_ld + e, left, h);
-        to_f32<RW>(h, a.res_type, y);
+        const raw8<RT> h = from_f32<RT>(y);
+        if (store) st8<size_of(RT)>(a.res_out, t * a.res_out_ld + e, left, h);
+        to_f32<RT>(h, y);
     }
     if constexpr (KIND == NORM || KIND == NORM_RES) {
 #pragma unroll
         for (int i = 0; i < 8; i++) sq = fmaf(y[i], y[i], sq);
-        float w[8];
-        if (a.w_type == MLLM_F32) to_f32<4>(ld8<4>(a.w, e, left), a.w_type, w);
-        else to_f32<2>(ld8<2>(a.w, e, left), a.w_type, w);
-#pragma unroll
-        for (int i = 0; i < 8; i++) y[i] *= w[i];
+        weigh(a, e, left, y);
     }
 }
 
-template <int KIND, int W, int RW>
-__device__ __forceinline__ void load(const row_args &a, long t, int e, int left, raw<8 * W> &x, raw<8 * RW> &r)
+template <int KIND, int XT, int RT>
+__device__ __forceinline__ void load(const row_args &a, long t, int e, int left, raw8<XT> &x, raw8<RT> &r)
 {
-    x = ld8<W>(a.x, t * a.x_ld + e, left);
-    if constexpr (KIND == NORM_RES || KIND == SILU) r = ld8<RW>(a.res, t * a.res_ld + e, left);
+    x = ld8<size_of(XT)>(a.x, t * a.x_ld + e, left);
+    if constexpr (KIND == NORM_RES || KIND == SILU) r = ld8<size_of(RT)>(a.res, t * a.res_ld + e, left);
 }
 
 // The norm's factor with squares and their sum in 64 bits; every wave of the row forms it alike.
-template <int KIND, int W, int RW>
+template <int KIND, int XT, int RT>
 __device__ float far_factor(const row_args &a, long t, int lane)
 {
     double sum = 0.0;
     for (int e = 8 * lane; e < a.n; e += 512) {
         float h[8];
         // the stored sum (x or res may be where it went): the barrier of the row's maximum lies between
-        if constexpr (KIND == NORM_RES) to_f32<RW>(ld8<RW>(a.res_out, t * a.res_out_ld + e, a.n - e), a.res_type, h);
-        else to_f32<W>(ld8<W>(a.x, t * a.x_ld + e, a.n - e), a.type, h);
+        if constexpr (KIND == NORM_RES) to_f32<RT>(ld8<size_of(RT)>(a.res_out, t * a.res_out_ld + e, a.n - e), h);
+        else to_f32<XT>(ld8<size_of(XT)>(a.x, t * a.x_ld + e, a.n - e), h);
 #pragma unroll
         for (int i = 0; i < 8; i++) sum += (double)h[i] * h[i];
     }
@@ -180,8 +252,8 @@ __device__ float far_factor(const row_args &a, long t, int lane)
 
 // A row over L = blockDim.x lanes (PER_WAVE: a row per wave).  NV vectors of eight elements a lane stay in
 // registers; longer rows are formed again for their codes.  PACK: codes go to the packed weight layout.
-template <int KIND, int W, int RW, int NV, bool PACK>
-__global__ __launch_bounds__(1024) void k_i8_rows(row_args a, int per_wave)
+template <int KIND, int XT, int RT, int NV, bool PACK>
+__global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int per_wave)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int L = per_wave ? 64 : blockDim.x, at = per_wave ? lane : threadIdx.x;
@@ -189,33 +261,32 @@ __global__ __launch_bounds__(1024) void k_i8_rows(row_args a, int per_wave)
     if (t >= (PACK ? a.T_pad : a.T)) return;             // a whole wave, or the whole workgroup
     const bool real = !PACK || t < a.T;
     float y[NV][8];
-    raw<8 * W> x[NV];
-    raw<8 * RW> r[NV];
+    raw8<XT> x[NV];
+    raw8<RT> r[NV];
     float sq = 0.0f;
-    uint32_t m = 0;
+    top mm;
     if (real) {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int e = 8 * (v * L + at);
-            if (e < a.n) load<KIND, W, RW>(a, t, e, a.n - e, x[v], r[v]);
+            if (e < a.n) load<KIND, XT, RT>(a, t, e, a.n - e, x[v], r[v]);
         }
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int e = 8 * (v * L + at);
 #pragma unroll
             for (int i = 0; i < 8; i++) y[v][i] = 0.0f;
-            if (e < a.n) form<KIND, W, RW>(a, x[v], r[v], e, t, a.n - e, true, y[v], sq);
-#pragma unroll
-            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(y[v][i]) & 0x7FFFFFFFu);
+            if (e < a.n) form<KIND, XT, RT>(a, x[v], r[v], e, t, a.n - e, true, y[v], sq);
+            mm.add(y[v]);
         }
         for (int e = 8 * (NV * L + at); e < a.n; e += 8 * L) {
             float z[8];
-            load<KIND, W, RW>(a, t, e, a.n - e, x[0], r[0]);
-            form<KIND, W, RW>(a, x[0], r[0], e, t, a.n - e, true, z, sq);
-#pragma unroll
-            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(z[i]) & 0x7FFFFFFFu);
+            load<KIND, XT, RT>(a, t, e, a.n - e, x[0], r[0]);
+            form<KIND, XT, RT>(a, x[0], r[0], e, t, a.n - e, true, z, sq);
+            mm.add(z);
         }
     }
+    uint32_t m = mm.get();
     for (int d = 32; d > 0; d >>= 1) {
         m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
         if constexpr (KIND == NORM || KIND == NORM_RES) sq += __shfl_xor(sq, d, 64);
@@ -235,12 +306,12 @@ __global__ __launch_bounds__(1024) void k_i8_rows(row_args a, int per_wave)
             sq += qs[i];
         }
     }
-    const row_step s = step_of(m);
+    const row_step s = step_of(__builtin_amdgcn_readfirstlane(m));
     // squares that leave fp32, or vanish in it where eps does not stand above them, are summed again in 64 bits
     float s_factor = 1.0f, mean = sq / (float)a.n;
     if constexpr (KIND == NORM || KIND == NORM_RES) {
         if (real && !s.bad && m != 0 && (!(mean < 0x1p100f) || (mean < 0x1p-100f && a.eps < 0x1p-100f)))
-            s_factor = far_factor<KIND, W, RW>(a, t, lane);
+            s_factor = far_factor<KIND, XT, RT>(a, t, lane);
         else s_factor = 1.0f / sqrtf(mean + a.eps);
     }
     if (at == 0 && real) {
@@ -275,33 +346,37 @@ __global__ __launch_bounds__(1024) void k_i8_rows(row_args a, int per_wave)
         float z[8] = {}, no = 0.0f;
         if (real && e < a.n) {
             if constexpr (KIND == NORM_RES) {            // the stored sum: x or res may be where it went
-                to_f32<RW>(ld8<RW>(a.res_out, t * a.res_out_ld + e, a.n - e), a.res_type, z);
-                float w[8];
-                if (a.w_type == MLLM_F32) to_f32<4>(ld8<4>(a.w, e, a.n - e), a.w_type, w);
-                else to_f32<2>(ld8<2>(a.w, e, a.n - e), a.w_type, w);
-#pragma unroll
-                for (int i = 0; i < 8; i++) z[i] *= w[i];
+                to_f32<RT>(ld8<size_of(RT)>(a.res_out, t * a.res_out_ld + e, a.n - e), z);
+                weigh(a, e, a.n - e, z);
             } else {
-                load<KIND, W, RW>(a, t, e, a.n - e, x[0], r[0]);
-                form<KIND, W, RW>(a, x[0], r[0], e, t, a.n - e, false, z, no);
+                load<KIND, XT, RT>(a, t, e, a.n - e, x[0], r[0]);
+                form<KIND, XT, RT>(a, x[0], r[0], e, t, a.n - e, false, z, no);
             }
         }
         put(e, z);
     }
 }
 
-template <int KIND, int W, int RW, bool PACK> void go_rows(const row_args &a, hipStream_t st)
+template <int KIND, int XT, int RT, bool PACK> void go_rows(const row_args &a, hipStream_t st)
 {
     const int rows = PACK ? a.T_pad : a.T, n = PACK ? a.n_pad : a.n;
     const int vecs = (n + 7) / 8;
-    const int per_wave = vecs <= 64;
-    const int threads = vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
+    // A wave a row where it is short (many rows of 1024: 5.6 us for 4096 of them, 7.6 with a workgroup each).  Many
+    // rows: workgroups of 256 lanes, or 512 where a vector is 32 bytes, which leave several to a CU to hide each
+    // other's barrier (silu of 4096 x 11264: 53 us, 75 with 1024).  Few: a lane for each vector.
+    const bool many = rows >= 256;
+    const int per_wave = vecs <= (rows >= 1024 ? 128 : 64);
+    const int threads = per_wave || vecs <= 256 ? 256
+                      : many && vecs <= 2048    ? (size_of(XT) + size_of(RT) > 4 ? 512 : 256)
+                                                : vecs <= 512 ? 512 : 1024;
     const int grid = per_wave ? (rows + 3) / 4 : rows;
-    const int nv = per_wave ? 1 : (vecs + threads - 1) / threads;
+    const int nv = per_wave ? (vecs + 63) / 64 : (vecs + threads - 1) / threads;
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, a, per_wave); };
-    if (nv <= 1) go(k_i8_rows<KIND, W, RW, 1, PACK>);
-    else if (nv == 2) go(k_i8_rows<KIND, W, RW, 2, PACK>);
-    else go(k_i8_rows<KIND, W, RW, 4, PACK>);
+    if (nv <= 1) go(k_i8_rows<KIND, XT, RT, 1, PACK>);
+    else if (nv == 2) go(k_i8_rows<KIND, XT, RT, 2, PACK>);
+    else if (nv <= 4 || threads > 256) go(k_i8_rows<KIND, XT, RT, 4, PACK>);
+    else if (nv <= 6) go(k_i8_rows<KIND, XT, RT, 6, PACK>);
+    else go(k_i8_rows<KIND, XT, RT, 8, PACK>);
 }
 
 // Integers into the packed layout: a lane moves 16 of them.
@@ -320,27 +395,45 @@ __global__ __launch_bounds__(256) void k_i8_pack(const int8_t *w, long w_ld, int
     __builtin_memcpy(packed + i8_at(kb, r, 16 * u), &c, 16);
 }
 
-// 16 codes a lane, back to values.
-template <int W>
-__global__ __launch_bounds__(256) void k_i8_dequant(const int8_t *q, long q_ld, const float *scale, int n, int type, void *out,
-                                                    long out_ld, int chunks, long total)
+// Back to values: 2^lpr_log lanes a row, eight codes of each of four vectors a lane (four loads under way).
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_i8_dequant(const int8_t *q, long q_ld, const float *scale, int T, int n, void *out,
+                                                    long out_ld, int lpr_log)
 {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const long t = i / chunks;
-    const int e = 16 * (int)(i - t * chunks);
+    const long t = (long)blockIdx.x * (256 >> lpr_log) + (threadIdx.x >> lpr_log);
+    if (t >= T) return;
+    const int lpr = 1 << lpr_log, lane = threadIdx.x & (lpr - 1);
     const float s = scale[t];
-    const int8_t *p = q + t * q_ld + e;
-    if (n - e >= 16) {
-        const raw<16> c = ld_any<16>(p);
-        float y[2][8];
+    for (long v = (long)blockIdx.y * 4 * lpr + lane; 8 * v < n; v += (long)gridDim.y * 4 * lpr) {
+        raw<8> c[4];
 #pragma unroll
-        for (int j = 0; j < 16; j++) y[j >> 3][j & 7] = (float)(int8_t)(c.w[j >> 2] >> (8 * (j & 3))) * s;
-        st8<W>(out, t * out_ld + e, 8, from_f32<W>(y[0], type));
-        st8<W>(out, t * out_ld + e + 8, 8, from_f32<W>(y[1], type));
-    } else {
-        for (int j = 0; j < n - e; j++) put1(out, t * out_ld + e + j, type, (float)p[j] * s);
+        for (int k = 0; k < 4; k++) {
+            const int e = (int)(8 * (v + k * lpr)), left = n - e;
+            const int8_t *p = q + t * q_ld + e;
+            if (left >= 8) c[k] = ld_any<8>(p);
+            else {
+                c[k] = raw<8>{};
+#pragma unroll
+                for (int i = 0; i < 7; i++)
+                    if (i < left) c[k].w[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int e = (int)(8 * (v + k * lpr)), left = n - e;
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = (float)(int8_t)(c[k].w[i >> 2] >> (8 * (i & 3))) * s;
+            if (left > 0) st8<size_of(TYPE)>(out, t * out_ld + e, left, from_f32<TYPE>(y));
+        }
     }
+}
+
+// f of the type as a constant.
+template <int T> using type_is = std::integral_constant<int, T>;
+template <class F> void by_type(int type, F &&f)
+{
+    type == MLLM_F32 ? f(type_is<MLLM_F32>{}) : type == MLLM_BF16 ? f(type_is<MLLM_BF16>{}) : f(type_is<MLLM_F16>{});
 }
 
 const char *rows_refusal(int type, const void *x, long x_ld, int T, int n, const void *q, long q_ld, const float *scale)
@@ -365,9 +458,9 @@ MLLM_API int mllm_i8_quantize(int type, const void *x, long x_ld, int T, int n, 
     if (const char *why = rows_refusal(type, x, x_ld, T, n, q, q_ld, scale)) return pk_fail(who, why);
     if (!T) return 0;
     row_args a{};
-    a.x = x; a.x_ld = x_ld; a.q = q; a.q_ld = q_ld; a.scale = scale; a.type = type; a.T = T; a.n = n;
+    a.x = x; a.x_ld = x_ld; a.q = q; a.q_ld = q_ld; a.scale = scale; a.T = T; a.n = n;
     hipStream_t st = (hipStream_t)stream;
-    type == MLLM_F32 ? go_rows<QUANTIZE, 4, 4, false>(a, st) : go_rows<QUANTIZE, 2, 2, false>(a, st);
+    by_type(type, [&](auto x) { go_rows<QUANTIZE, x, x, false>(a, st); });
     return done(who);
 }
 
@@ -377,14 +470,15 @@ MLLM_API int mllm_i8_dequant(const int8_t *q, long q_ld, const float *scale, int
     const char *who = "mllm_i8_dequant";
     if (const char *why = rows_refusal(type, out, out_ld, T, n, q, q_ld, scale)) return pk_fail(who, why);
     if (!T) return 0;
-    const int chunks = (n + 15) / 16;
-    const long total = (long)T * chunks;
-    if (total > (1l << 31) * 128) return pk_fail(who, "T * n is at most 2^42");
+    const int vecs = (n + 7) / 8;
+    int lpr_log = 2;
+    while (lpr_log < 8 && 1 << lpr_log < vecs) lpr_log++;
+    const int rows = 256 >> lpr_log, grid_y = std::min((vecs + (4 << lpr_log) - 1) / (4 << lpr_log), 1 << 14);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, q_ld, scale, n,
-                           type, out, out_ld, chunks, total);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long)T + rows - 1) / rows), grid_y), dim3(256), 0, (hipStream_t)stream, q,
+                           q_ld, scale, T, n, out, out_ld, lpr_log);
     };
-    type == MLLM_F32 ? go(k_i8_dequant<4>) : go(k_i8_dequant<2>);
+    type == MLLM_F32 ? go(k_i8_dequant<MLLM_F32>) : type == MLLM_BF16 ? go(k_i8_dequant<MLLM_BF16>) : go(k_i8_dequant<MLLM_F16>);
     return done(who);
 }
 
@@ -406,13 +500,13 @@ MLLM_API int mllm_i8_rms_norm(int type, const void *x, long x_ld, int res_type, 
     if (!T) return 0;
     row_args a{};
     a.x = x; a.x_ld = x_ld; a.res = res; a.res_ld = res_ld; a.res_out = res_out; a.res_out_ld = res_out_ld; a.w = w;
-    a.eps = eps; a.q = q; a.q_ld = q_ld; a.scale = scale; a.type = type; a.res_type = res_type; a.w_type = w_type;
+    a.eps = eps; a.q = q; a.q_ld = q_ld; a.scale = scale; a.w_type = w_type;
     a.T = T; a.n = n;
     hipStream_t st = (hipStream_t)stream;
-    const bool wide = type == MLLM_F32, rwide = res_type == MLLM_F32;
-    if (!res) wide ? go_rows<NORM, 4, 4, false>(a, st) : go_rows<NORM, 2, 2, false>(a, st);
-    else if (wide) rwide ? go_rows<NORM_RES, 4, 4, false>(a, st) : go_rows<NORM_RES, 4, 2, false>(a, st);
-    else rwide ? go_rows<NORM_RES, 2, 4, false>(a, st) : go_rows<NORM_RES, 2, 2, false>(a, st);
+    by_type(type, [&](auto x) {
+        if (!res) go_rows<NORM, x, x, false>(a, st);
+        else by_type(res_type, [&](auto r) { go_rows<NORM_RES, x, r, false>(a, st); });
+    });
     return done(who);
 }
 
@@ -424,10 +518,10 @@ MLLM_API int mllm_i8_silu_mul(int type, const void *gate, long gate_ld, const vo
     if (up_ld < n || (T && !up)) return pk_fail(who, "up is given, its rows at least n elements apart");
     if (!T) return 0;
     row_args a{};
-    a.x = gate; a.x_ld = gate_ld; a.res = up; a.res_ld = up_ld; a.res_type = type; a.q = q; a.q_ld = q_ld; a.scale = scale;
-    a.type = type; a.T = T; a.n = n;
+    a.x = gate; a.x_ld = gate_ld; a.res = up; a.res_ld = up_ld; a.q = q; a.q_ld = q_ld; a.scale = scale;
+    a.T = T; a.n = n;
     hipStream_t st = (hipStream_t)stream;
-    type == MLLM_F32 ? go_rows<SILU, 4, 4, false>(a, st) : go_rows<SILU, 2, 2, false>(a, st);
+    by_type(type, [&](auto x) { go_rows<SILU, x, x, false>(a, st); });
     return done(who);
 }
 
@@ -454,9 +548,9 @@ MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_
         return done(who);
     }
     row_args a{};
-    a.x = w; a.x_ld = w_ld; a.q = (int8_t *)packed; a.scale = scale; a.type = type; a.T = n_rows; a.n = n_cols; a.kb = kb;
+    a.x = w; a.x_ld = w_ld; a.q = (int8_t *)packed; a.scale = scale; a.T = n_rows; a.n = n_cols; a.kb = kb;
     a.T_pad = rows; a.n_pad = (int)kb * 64;
-    type == MLLM_F32 ? go_rows<QUANTIZE, 4, 4, true>(a, st) : go_rows<QUANTIZE, 2, 2, true>(a, st);
+    by_type(type, [&](auto x) { go_rows<QUANTIZE, x, x, true>(a, st); });
     return done(who);
 }
 
