@@ -618,7 +618,7 @@ MLLM_API int mllm_pages_copy(const mllm_page_plane *planes, int n_planes, int n_
 
 /* ------------------------- layers in 8-bit integers: a scale per row and token
  * A quantised row stands for scale * q[i], i < n, with 8-bit integers q and an
- * fp32 scale.  The calls below that form one from values y[i] take
+ * fp32 scale.  T, n and n_rows are at most 2^30.  The calls below that form one from values y[i] take
  *   q[i] = y[i] * (127 * (1 / max|y|)) to the nearest integer (ties to even),
  *   scale = max|y| / 127,
  * in fp32, operation by operation; a row of zeros has scale 0 and zeros; a row that holds an
@@ -659,7 +659,8 @@ MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_
                           void *stream);
 /* out[t][r] = (sum_k x[t][k] w[r][k]) * x_scale[t] * w_scale[r] (+ bias[r],
  * fp32, optional), the sums exact in 32-bit integers, the rest in fp32 in that
- * order, rounded to type once.  x: T rows of 8-bit integers (-128 among them)
+ * order (the second product and the bias as one fma), then rounded to type: a
+ * token's results are the same bits whatever T is.  x: T rows of 8-bit integers (-128 among them)
  * at multiples of 16 bytes (x and x_ld; what lies behind a row's n_cols up to
  * the next multiple of 16 bytes may be read and has no part in the result).
  * Any T: few tokens stream the weights once, many run on tiles.  Workspace:

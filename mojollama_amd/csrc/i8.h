@@ -27,10 +27,17 @@ __host__ __device__ inline long i8_at(long kb, int r, int k)
 
 inline bool i8_real(int type) { return type == MLLM_F32 || type == MLLM_F16 || type == MLLM_BF16; }
 
-// One float as an element of the type.
+// One or two floats as elements of the type.  A sum or product is a number of 32 bits before it is one of 16: the
+// compiler would round some of them to F16 once.
 __device__ __forceinline__ void put1(void *p, long at, int type, float x)
 {
-    if (type == MLLM_F32) ((float *)p)[at] = x;
-    else if (type == MLLM_BF16) ((__bf16 *)p)[at] = (__bf16)x;
+    if (type == MLLM_F32) { ((float *)p)[at] = x; return; }
+    asm("" : "+v"(x));
+    if (type == MLLM_BF16) ((__bf16 *)p)[at] = (__bf16)x;
     else ((_Float16 *)p)[at] = (_Float16)x;
+}
+template <int TYPE> __device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    if constexpr (TYPE == MLLM_F16) asm("" : "+v"(a), "+v"(b));
+    return pack16(a, b, TYPE);
 }

@@ -39,7 +39,9 @@ template <int N, int K = 0, class F> __device__ __forceinline__ void each(F &&f)
     }
 }
 
-__device__ __forceinline__ float value(int acc, float xs, float ws) { return (float)acc * xs * ws; }
+// The result of a sum, the same bits from every kernel here.  bias: -0 where there is none (y + -0 is y, -0 too).
+__device__ __forceinline__ float value(int acc, float xs, float ws, float bias) { return fmaf((float)acc * xs, ws, bias); }
+__device__ __forceinline__ float bias_of(const gemm_args &a, int r) { return a.bias ? a.bias[r] : -0.0f; }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int bytes)
 {
@@ -89,7 +91,7 @@ template <int TT, int TR, int IDS> __device__ __forceinline__ void get_scales(co
     for (int i = 0; i < (TR + IDS - 1) / IDS; i++) {
         const int r = min(r0 + i * IDS + id, a.R - 1);
         s.ws[i] = a.ws[r];
-        s.bias[i] = a.bias ? a.bias[r] : -0.0f;              // y + -0 is y, -0 too
+        s.bias[i] = bias_of(a, r);
     }
 #pragma unroll
     for (int i = 0; i < (TT + IDS - 1) / IDS; i++) s.xs[i] = a.xs[min(t0 + i * IDS + id, a.T - 1)];
@@ -128,7 +130,7 @@ template <int NF, class T> __device__ __forceinline__ void tail_as(const gemm_ar
         const i32x4 u = *(const i32x4 *)(room + room_at<NF>(t, c >> 2)), v = *(const i32x4 *)(room + room_at<NF>(t, (c >> 2) + 1));
         const float x = xs[t];
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = value(i < 4 ? u[i] : v[i - 4], x, ws[i]) + bias[i];
+        for (int i = 0; i < 8; i++) y[i] = value(i < 4 ? u[i] : v[i - 4], x, ws[i], bias[i]);
     };
     if (t0 + 32 <= a.T && r0 + 32 * NF <= a.R) {
 #pragma unroll 4
@@ -138,7 +140,7 @@ template <int NF, class T> __device__ __forceinline__ void tail_as(const gemm_ar
             if constexpr (sizeof(T) == 4) {
                 __builtin_memcpy(to, y, 32);
             } else {
-                const u32x4 w = {pack16(y[0], y[1], type), pack16(y[2], y[3], type), pack16(y[4], y[5], type), pack16(y[6], y[7], type)};
+                const u32x4 w = {pack2<type>(y[0], y[1]), pack2<type>(y[2], y[3]), pack2<type>(y[4], y[5]), pack2<type>(y[6], y[7])};
                 __builtin_memcpy(to, &w, 16);
             }
         }
@@ -150,7 +152,7 @@ template <int NF, class T> __device__ __forceinline__ void tail_as(const gemm_ar
         form(j, y);
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (r0 + c + i < a.R) to[i] = (T)y[i];
+            if (r0 + c + i < a.R) put1(to, i, type, y[i]);
     }
 }
 
@@ -392,56 +394,113 @@ template <int MF, int NF, int WM, int WN> __global__ __launch_bounds__(64) void 
 }
 
 // ------------------------------------------------------------------------------------ few tokens
-// 16 weight rows x 16 TF tokens a workgroup of W waves, which take blocks of 64 columns in turn and join their sums in
+// 16 weight rows x up to 16 tokens a workgroup of W waves, which take blocks of 64 columns in turn and join their sums in
 // LDS.  Weights stream from memory straight into the matrix cores, each byte once; x comes from the caches.
-template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
+template <int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
 {
     constexpr int D = 2;                                     // blocks under way a wave
-    __shared__ __attribute__((aligned(16))) int sums[W][TF][64][4];
+    __shared__ __attribute__((aligned(16))) int sums[W][64][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, c = lane >> 4;
-    const int r0 = blockIdx.x * 16;
+    const int r0 = blockIdx.x * 16, nb = (a.K + 63) / 64;
     const int8_t *w = a.w + (long)(r0 >> 5) * a.kb * 2048 + (r0 & 16) * 16 + c * 512 + l * 16;
     const __amdgpu_buffer_rsrc_t xr = rsrc(a.x, (int)((a.T - 1) * a.x_ld + (a.K + 15) / 16 * 16));
-    int xo[TF];
-#pragma unroll
-    for (int f = 0; f < TF; f++) xo[f] = 16 * f + l < a.T ? (16 * f + l) * (int)a.x_ld + 16 * c : 0x7FFFFF00;
-    i32x4 acc[TF] = {};
-    for (int b = wave; b < a.kb; b += W * D) {
-        i32x4 wf[D], xf[D][TF];
+    const bool live = l < a.T;                               // the other lanes ask for what is not there: zeros
+    const int xo = live ? l * (int)a.x_ld + 16 * c : 0x7FFFFF00;
+    i32x4 acc = {};
+    for (int b = wave; b < nb; b += W * D) {
+        i32x4 wf[D], xf[D];
 #pragma unroll
         for (int d = 0; d < D; d++) {
-            const int k = min(b + d * W, a.kb - 1);
+            const int k = min(b + d * W, nb - 1);
             wf[d] = *(const i32x4 *)(w + (long)k * 2048);
-#pragma unroll
-            for (int f = 0; f < TF; f++)
-                xf[d][f] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, 16 * f + l < a.T ? xo[f] + 64 * k : xo[f], 0, 0));
+            xf[d] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, live ? xo + 64 * k : xo, 0, 0));
         }
 #pragma unroll
         for (int d = 0; d < D; d++)
-            if (b + d * W < a.kb) {
+            if (b + d * W < nb) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d], xf[d], acc, 0, 0, 0);
+    }
+    *(i32x4 *)sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0 || l >= a.T) return;                        // lane: token l, rows 4 c + i
+    i32x4 s = {};
 #pragma unroll
-                for (int f = 0; f < TF; f++) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d], xf[d][f], acc[f], 0, 0, 0);
-            }
+    for (int i = 0; i < W; i++) s += *(const i32x4 *)sums[i][lane];
+    const float xs = a.xs[l];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = r0 + 4 * c + i;
+        if (r < a.R) put1(a.out, l * a.out_ld + r, a.type, value(s[i], xs, a.ws[r], bias_of(a, r)));
+    }
+}
+
+// 32 weight rows x 32 TF tokens a workgroup of W waves, which take blocks of 128 columns in turn and join their sums in
+// LDS.  A wave's block of x comes to its own part of LDS in whole lines and its weights to registers, two blocks under
+// way; waves meet at the end alone.
+template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_stream(gemm_args a)
+{
+    constexpr int XB = TF * 4096, LOADS = 4 * TF + 4;            // bytes and loads of a block
+    __shared__ __attribute__((aligned(1024))) uint8_t x0[W * XB], x1[W * XB];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    const int r0 = blockIdx.x * 32, nb = (a.K + 127) / 128;
+    const int8_t *w = a.w + (long)blockIdx.x * a.kb * 2048 + lane * 16;
+    const __amdgpu_buffer_rsrc_t xr = rsrc(a.x, (int)((a.T - 1) * a.x_ld + (a.K + 15) / 16 * 16));
+    int xo[4 * TF], xa[4];
+#pragma unroll
+    for (int p = 0; p < 4 * TF; p++) {
+        const int row = 8 * p + (lane >> 3);
+        xo[p] = row * (int)a.x_ld + 16 * ((lane & 7) ^ swz(row));
     }
 #pragma unroll
-    for (int f = 0; f < TF; f++) *(i32x4 *)sums[wave][f][lane] = acc[f];
+    for (int j = 0; j < 4; j++) xa[j] = wave * XB + l * 128 + 16 * ((2 * j + h) ^ swz(l));
+    auto load = [&](uint8_t *to, i32x4 (&wf)[4], int b) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int p = 0; p < 4 * TF; p++) to_lds(xr, to + wave * XB + 1024 * p, xo[p] + 128 * b, 0);
+#pragma unroll
+        for (int j = 0; j < 4; j++) wf[j] = *(const i32x4 *)(w + (long)b * 4096 + j * 1024);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    i32x16 acc[TF];
+#pragma unroll
+    for (int f = 0; f < TF; f++) acc[f] = i32x16{};
+    i32x4 w0[4], w1[4];
+    if (wave < nb) load(x0, w0, wave);
+    if (wave + W < nb) load(x1, w1, wave + W);
+    // block b: its loads have landed (those of block b + W, if there is one, may be under way); when its operands are
+    // read, its buffer takes block b + 2 W
+    auto block = [&](uint8_t *x, i32x4 (&wf)[4], int b) __attribute__((always_inline)) {
+        if (b + W < nb) wait_mem<LOADS>();
+        else wait_mem<0>();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int f = 0; f < TF; f++)
+                acc[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], *(const i32x4 *)(x + f * 4096 + xa[j]), acc[f], 0, 0, 0);
+        if (b + 2 * W < nb) load(x, wf, b + 2 * W);
+    };
+    for (int b = wave; b < nb; b += 2 * W) {
+        block(x0, w0, b);
+        if (b + W < nb) block(x1, w1, b + W);
+    }
     __syncthreads();
-    // lane: token f * 16 + l, rows 4 c + i
-    for (int f = wave; f < TF; f += W) {
-        const int t = 16 * f + l;
+#pragma unroll
+    for (int f = 0; f < TF; f++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(i32x4 *)(x0 + ((wave * TF + f) * 4 + g) * 1024 + lane * 16) =
+                (i32x4){acc[f][4 * g], acc[f][4 * g + 1], acc[f][4 * g + 2], acc[f][4 * g + 3]};
+    __syncthreads();
+    for (int u = wave; u < 4 * TF; u += W) {                     // frag u / 4, rows 8 (u % 4) + 4 h and on
+        const int t = u / 4 * 32 + l, r = r0 + u % 4 * 8 + 4 * h;
         i32x4 s = {};
 #pragma unroll
-        for (int i = 0; i < W; i++) s += *(const i32x4 *)sums[i][f][lane];
+        for (int i = 0; i < W; i++) s += *(const i32x4 *)(x0 + (i * 4 * TF + u) * 1024 + lane * 16);
         if (t >= a.T) continue;
         const float xs = a.xs[t];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = r0 + 4 * c + i;
-            if (r < a.R) {
-                const float y = value(s[i], xs, a.ws[r]);
-                put1(a.out, t * a.out_ld + r, a.type, a.bias ? y + a.bias[r] : y);
-            }
-        }
+        for (int i = 0; i < 4; i++)
+            if (r + i < a.R) put1(a.out, t * a.out_ld + r + i, a.type, value(s[i], xs, a.ws[r + i], bias_of(a, r + i)));
     }
 }
 
@@ -468,9 +527,7 @@ __global__ __launch_bounds__(64) void k_i8_far(gemm_args a)
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         const int r = r0 + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (r >= a.R) continue;
-        const float y = value(acc[i], xs, a.ws[r]);
-        put1(a.out, t * a.out_ld + r, a.type, a.bias ? y + a.bias[r] : y);
+        if (r < a.R) put1(a.out, t * a.out_ld + r, a.type, value(acc[i], xs, a.ws[r], bias_of(a, r)));
     }
 }
 
@@ -502,23 +559,37 @@ const tile_kind kinds[] = {
     kind_of<1, 1, 1, 4, 3>(0.0422f, 0.0907f, 1.022f)};
 
 struct plan {
-    const tile_kind *kind;         // null: few tokens
+    const tile_kind *kind;         // or null:
+    int few;                       // 0: k_i8_few, 1, 2: k_i8_stream<few>
     int nt, nr, splits, per;
 };
 
+// The kernel that an estimate of their times in microseconds, from sizes alone, puts first; its constants are fitted to
+// the kernels' times over 17 to 4096 tokens and nine matrices from 512 x 2048 to 32000 x 2048 and 1024 x 14336, where its
+// choice is 1 % slower than the best on average and 23 % at most.
 plan plan_of(int T, int R, int kb, int cols)
 {
     plan best{};
     float least = INFINITY;
-    if (T <= 32) {
+    const float mb = (float)cols * R * 1e-6f;
+    if (T <= 16) {
         const int n = (R + 15) / 16, turns = (cols + 1023) / 1024;
-        least = 2.925f + (n + 511) / 512 * (0.9204f + turns * 0.3931f) + turns * (n / 512.0f) * 0.5291f * ((T <= 16 ? 1 : 2) + 0.3911f);
+        least = 2.9f + std::max((n + 511) / 512 * (0.6f + turns * 0.33f) + turns * (n / 512.0f) * (0.74f + T / 64.0f), mb / (5.3f - 0.08f * T));
+    }
+    if (T <= 64) {
+        const int n = (R + 31) / 32, turns = (cols + 1023) / 1024;
+        const float us = T <= 32 ? (T <= 16 ? 4.0f : 3.4f) + std::max(turns * 0.67f, mb / 5.3f) + n / 256.0f * 0.5f
+                                 : 4.0f + std::max(turns * 1.0f, mb / 4.2f) + n / 256.0f * 1.2f;
+        if (us < least) {
+            least = us;
+            best.few = T <= 32 ? 1 : 2;
+        }
     }
     const int quads = kb / 4;
     for (const tile_kind &k : kinds) {
         if (!k.fits(T)) continue;
         for (int want : {1, 2, 3, 4, 6, 8, kMostSplits}) {
-            plan p{&k, (T + k.TT - 1) / k.TT, (R + k.TR - 1) / k.TR, 0, 0};
+            plan p{&k, 0, (T + k.TT - 1) / k.TT, (R + k.TR - 1) / k.TR, 0, 0};
             if (want > quads) continue;
             p.per = (quads + want - 1) / want * 4;
             p.splits = (kb + p.per - 1) / p.per;
@@ -526,7 +597,7 @@ plan plan_of(int T, int R, int kb, int cols)
             if (p.splits != want || n > (want > 1 ? k.at_once() : 1l << 30)) continue;
             const int most = (int)((n + 255) / 256), full = most / k.per_cu, rest = most % k.per_cu;
             float us = full * (p.per * (k.step + k.per_cu * k.each) + k.tail) + (rest ? p.per * (k.step + rest * k.each) + k.tail : 0.0f);
-            us = 3.088f + std::max(us, (float)cols * ((float)R + T) / 10.28e6f);
+            us = 3.088f + std::max(us, (float)cols * ((float)R + T) / 5.7e6f);
             if (want > 1) us += 3.422f + (float)n * k.TT * k.TR * 8 / 6.818e6f;
             if (us < least) {
                 least = us;
@@ -554,7 +625,7 @@ extern "C" {
 
 MLLM_API long mllm_i8_gemm_workspace_size(int T, int n_rows, int n_cols)
 {
-    if (T < 0 || mllm_i8_packed_size(n_rows, n_cols) < 0) return -1;
+    if (T < 0 || T > 1 << 30 || mllm_i8_packed_size(n_rows, n_cols) < 0) return -1;
     return T ? sums_of(T, n_rows, (int)i8_kblocks(n_cols)) : 0;
 }
 
@@ -563,8 +634,8 @@ MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t
                           void *workspace, long ws_bytes, void *stream)
 {
     const char *who = "mllm_i8_gemm";
-    if (T < 0 || mllm_i8_packed_size(n_rows, n_cols) < 0)
-        return pk_fail(who, "T is not negative, n_rows positive, n_cols from 1 to 131071");
+    if (T < 0 || T > 1 << 30 || mllm_i8_packed_size(n_rows, n_cols) < 0)
+        return pk_fail(who, "T is not negative, n_rows positive (both at most 2^30), n_cols from 1 to 131071");
     if (!i8_real(type)) return pk_fail(who, "the type of out is F32, F16 or BF16");
     if (x_ld < n_cols || out_ld < n_rows) return pk_fail(who, "rows of x lie at least n_cols apart, of out n_rows");
     if (((uintptr_t)x | (uintptr_t)x_ld | (uintptr_t)packed | (uintptr_t)workspace) & 15)
@@ -587,13 +658,16 @@ MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t
         hipLaunchKernelGGL(k_i8_far, dim3(a.nt * a.nr), dim3(64), 0, st, a);
     } else if (p.kind) {
         p.kind->go(a, p.nt * p.nr * p.splits, st);
-    } else if (T <= 32) {
+    } else if (p.few) {
+        const int grid = (n_rows + 31) / 32;
+        if (p.few == 1) hipLaunchKernelGGL((k_i8_stream<1, 8>), dim3(grid), dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((k_i8_stream<2, 8>), dim3(grid), dim3(512), 0, st, a);
+    } else if (T <= 16) {
         const int grid = (n_rows + 15) / 16;
-        auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, st, a); };
         // many workgroups hide each other's ends: eight waves each then (32000 x 2048, one token: 17.3 -> 14.9 us), few
         // are done sooner with sixteen (2048 x 5632: 7.0 -> 5.4 us)
-        if (grid > 1024) T <= 16 ? go(k_i8_few<1, 8>, 8) : go(k_i8_few<2, 8>, 8);
-        else T <= 16 ? go(k_i8_few<1, 16>, 16) : go(k_i8_few<2, 16>, 16);
+        if (grid > 1024) hipLaunchKernelGGL(k_i8_few<8>, dim3(grid), dim3(512), 0, st, a);
+        else hipLaunchKernelGGL(k_i8_few<16>, dim3(grid), dim3(1024), 0, st, a);
     } else {
         return pk_fail(who, "T * n_rows is too large for one call");
     }

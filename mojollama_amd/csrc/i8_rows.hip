@@ -69,12 +69,7 @@ template <int TYPE> __device__ __forceinline__ raw8<TYPE> from_f32(const float (
         for (int i = 0; i < 8; i++) r.w[i] = __float_as_uint(x[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float a = x[2 * i], b = x[2 * i + 1];
-            // a sum or product is a number of 32 bits before it is one of 16: the compiler would round some of them once
-            if constexpr (TYPE == MLLM_F16) asm("" : "+v"(a), "+v"(b));
-            r.w[i] = pack16(a, b, TYPE);
-        }
+        for (int i = 0; i < 4; i++) r.w[i] = pack2<TYPE>(x[2 * i], x[2 * i + 1]);
     }
     return r;
 }
@@ -439,7 +434,7 @@ template <class F> void by_type(int type, F &&f)
 const char *rows_refusal(int type, const void *x, long x_ld, int T, int n, const void *q, long q_ld, const float *scale)
 {
     if (!i8_real(type)) return "the type is F32, F16 or BF16";
-    if (T < 0 || n <= 0 || n > 1 << 30) return "T is not negative, n positive and at most 2^30";
+    if (T < 0 || T > 1 << 30 || n <= 0 || n > 1 << 30) return "T is not negative, n positive, both at most 2^30";
     if (x_ld < n || q_ld < n) return "rows lie at least n elements apart";
     if (T && (!x || !q || !scale)) return "x, q and scale are given";
     return nullptr;

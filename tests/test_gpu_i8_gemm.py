@@ -177,6 +177,46 @@ def test_workspace_of_more_tokens(dev):
         dev.i8_gemm(W, padded(codes(g, 300, 4096)), torch.ones(300, device="cuda"), ws=ws[:need - 16])
 
 
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("R,C", [(200, 320), (1000, 2881), (70, 20000)])
+def test_a_token_alone_or_among_others(dev, R, C, out):
+    """A token's results are the same bits whatever the number of tokens, and whichever kernel that takes."""
+    g = torch.Generator().manual_seed(R)
+    W = dev.i8_weights(codes(g, R, C).cuda(), (torch.rand(R, generator=g) * 0.01).cuda())
+    bias = torch.randn(R, generator=g).cuda()
+    q, s = padded(codes(g, 1100, C)), torch.rand(1100, generator=g).cuda()
+    for b in (None, bias):
+        want = dev.i8_gemm(W, q, s, bias=b, out_dtype=TYPES[out])
+        for T in (1, 5, 16, 17, 32, 40, 64, 70, 128, 200, 300, 600):
+            at = slice(1100 - T, 1100)
+            assert torch.equal(dev.i8_gemm(W, q[at], s[at], bias=b, out_dtype=TYPES[out]), want[at]), T
+
+
+@pytest.mark.parametrize("T", [1, 30, 64, 200, 300])
+def test_wide_strides(dev, T):
+    """Rows of x just below 4 MB apart (32-bit offsets inside a tile) and at 4 MB (addresses of 64 bits)."""
+    R, C = 150, 1000
+    g = torch.Generator().manual_seed(T)
+    w = codes(g, R, C).cuda()
+    W, s = dev.i8_weights(w, torch.ones(R, device="cuda")), torch.ones(T, device="cuda")
+    for ld in ((1 << 22) - 16, 1 << 22):
+        q = torch.empty(T * ld, dtype=torch.int8, device="cuda").view(T, ld)[:, :C]
+        q.copy_(codes(g, T, C))
+        out = dev.i8_gemm(W, q, s, out_dtype=torch.float32)
+        assert torch.equal(out.double(), q.double() @ w.double().T.contiguous())
+
+
+def test_many_results(dev):
+    """More than 2^31 results."""
+    T, R, C = 70001, 32768, 48
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randint(-128, 128, (R, C), dtype=torch.int8, device="cuda", generator=g)
+    q = torch.randint(-128, 128, (T, C), dtype=torch.int8, device="cuda", generator=g)
+    out = dev.i8_gemm(dev.i8_weights(w, torch.ones(R, device="cuda")), q, torch.ones(T, device="cuda"))
+    at = torch.tensor([0, 1, 255, 256, 30000, 65535, 65536, 69999, 70000], device="cuda")
+    assert torch.equal(out[at], (q[at].double() @ w.double().T.contiguous()).float().bfloat16())
+
+
 def test_far_rows(dev):
     """Rows of x and out beyond 2^31 bytes from the first."""
     T, C, R = 40, 100, 70

@@ -232,6 +232,23 @@ def test_many_short_rows(dev):
     assert torch.equal(dev.i8_dequant(q, scale), (q.float() * scale[:, None]).bfloat16())
 
 
+def test_many_elements(dev):
+    """More than 2^31 elements: the last rows lie behind 32-bit offsets."""
+    T, n = 65600, 32776
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty((T, n), dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 32767, 65520, 65535, 65536, T - 1], device="cuda")
+    rows = torch.randn((len(at), n), device="cuda", generator=g).bfloat16()
+    x[at] = rows
+    w = torch.ones(n, device="cuda")
+    for call, alone in ((lambda: dev.i8_quantize(x), lambda: dev.i8_quantize(rows)),
+                        (lambda: dev.i8_rms_norm(x, w, 1e-6), lambda: dev.i8_rms_norm(rows, w, 1e-6)),
+                        (lambda: dev.i8_silu_mul(x, x), lambda: dev.i8_silu_mul(rows, rows))):
+        (q, s), (q1, s1) = call(), alone()
+        assert torch.equal(q[at], q1) and torch.equal(s[at], s1)
+    assert torch.equal(dev.i8_dequant(q, s)[at], dev.i8_dequant(q1, s1))
+
+
 def test_refused_tensors(dev):
     x, w = torch.zeros((3, 64), device="cuda"), torch.ones(64, device="cuda")
     cpu = torch.zeros((3, 64))

@@ -47,7 +47,7 @@ def pack(so, **c):
     return so.mllm_i8_pack(*a.values(), None)
 
 
-ROWS = [dict(type=K.T_E4M3), dict(type=K.T_I8), dict(type=-1), dict(T=-1), dict(n=0), dict(n=-5), dict(x_ld=99), dict(q_ld=99),
+ROWS = [dict(T=(1 << 30) + 1), dict(type=K.T_E4M3), dict(type=K.T_I8), dict(type=-1), dict(T=-1), dict(n=0), dict(n=-5), dict(x_ld=99), dict(q_ld=99),
         dict(x=None), dict(q=None), dict(scale=None), dict(n=(1 << 30) + 1, x_ld=BIG, q_ld=BIG)]
 
 
@@ -70,7 +70,7 @@ def test_silu(so, c):
     assert silu(so, **c) == -1 and so.mllm_last_error().startswith(b"mllm_i8_silu_mul")
 
 
-@pytest.mark.parametrize("c", [dict(T=-1), dict(rows=0), dict(rows=-3), dict(cols=0), dict(cols=131072, x_ld=131072),
+@pytest.mark.parametrize("c", [dict(T=-1), dict(T=(1 << 30) + 1), dict(rows=0), dict(rows=-3), dict(cols=0), dict(cols=131072, x_ld=131072),
                                dict(type=K.T_I8), dict(type=K.T_E4M3), dict(x_ld=96), dict(x_ld=100), dict(x_ld=104), dict(out_ld=39),
                                dict(x=P + 1), dict(x=P + 8), dict(packed=P + 4), dict(work=P + 8), dict(packed=None), dict(ws=None),
                                dict(x=None), dict(xs=None), dict(out=None)])
