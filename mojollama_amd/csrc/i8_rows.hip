@@ -3,8 +3,10 @@
 //
 // y[i] of a row, its largest |y| and (norm) the sum of squares are formed in one pass over memory and stay
 // in registers; the codes are rounded from there: memory is read and written once, which is what bounds
-// these kernels.  The norm's factor 1 / sqrt(mean + eps) is one number per row: it enters the scale alone,
-// and the codes do not wait for it.
+// these kernels where there are many rows (norm of 8192 x 4096 with residual, 16 bits: 47 us, 5.0 TB/s; silu of
+// 4096 x 11264: 52 us, 4.4 TB/s, its exponentials beside it; the card copies 4 GiB at 4.7).  A few rows take the
+// launch and one memory round trip (3 to 5 us).  The norm's factor 1 / sqrt(mean + eps) is one number per row: it
+// enters the scale alone, and the codes do not wait for it.
 #include <algorithm>
 #include <type_traits>
 #include "i8.h"
@@ -390,7 +392,8 @@ __global__ __launch_bounds__(256) void k_i8_pack(const int8_t *w, long w_ld, int
     __builtin_memcpy(packed + i8_at(kb, r, 16 * u), &c, 16);
 }
 
-// Back to values: 2^lpr_log lanes a row, eight codes of each of four vectors a lane (four loads under way).
+// Back to values: 2^lpr_log lanes a row, eight codes of each of four vectors a lane (four loads under way; 8192 x 4096
+// to 16 bits: 22.4 us, 4.5 TB/s).
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_i8_dequant(const int8_t *q, long q_ld, const float *scale, int T, int n, void *out,
                                                     long out_ld, int lpr_log)

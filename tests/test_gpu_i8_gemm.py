@@ -86,6 +86,19 @@ def test_outputs(dev, T, R, C, out, bias, ld):
     case(dev, T, R, C, out, bias, ld, extra=ld)
 
 
+@pytest.mark.parametrize("T", [1, 20, 60, 150, 600])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_out_inside_a_wider_tensor(dev, T, out):
+    """out begins at an odd element of its rows."""
+    g = torch.Generator().manual_seed(T)
+    w, q = codes(g, 333, 500), codes(g, T, 500)
+    buf = torch.full((T, 341), 9.0, dtype=TYPES[out], device="cuda")
+    dev.i8_gemm(dev.i8_weights(w.cuda(), torch.full((333,), 2.0 ** -8, device="cuda")), padded(q), torch.ones(T, device="cuda"),
+                out=buf[:, 3:336])
+    assert (buf[:, :3] == 9).all() and (buf[:, 336:] == 9).all()
+    assert torch.equal(buf[:, 3:336].cpu(), (q.double() @ w.double().T / 256).to(TYPES[out]))
+
+
 @pytest.mark.parametrize("T,R,C", [(1, 32000, 2048), (16, 4096, 4096), (96, 11264, 2048), (1021, 2883, 2881), (2048, 4096, 4096),
                                    (700, 8200, 1024), (5000, 256, 8192), (4099, 2048, 640), (3, 201088, 2880)])
 def test_large(dev, T, R, C):
@@ -123,7 +136,7 @@ def test_scales_that_stand_out(dev, T):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("R,C,lead", [(1, 1, 0), (33, 100, 0), (40, 2881, 3), (70, 513, 1), (5, 40000, 0), (64, 2048, 0)])
+@pytest.mark.parametrize("R,C,lead", [(1, 1, 0), (33, 100, 0), (40, 2881, 3), (70, 513, 1), (5, 40000, 0), (64, 2048, 0), (300, 9001, 2), (1100, 700, 0)])
 def test_weights(dev, kind, R, C, lead):
     """Weights quantised here are those of i8_quantize: the product is the same, bit by bit."""
     g = torch.Generator().manual_seed(R + C)

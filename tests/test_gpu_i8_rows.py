@@ -70,7 +70,8 @@ def scales(scale, want, roundings, names=""):
 
 
 SIZES = [(1, 1), (1, 7), (3, 8), (1, 64), (5, 100), (2, 511), (3, 512), (9, 513), (1, 2048), (7, 2049), (1, 2880), (4, 4095),
-         (2, 4097), (3, 8191), (2, 8200), (1, 16385), (2, 32768), (1, 32777), (2, 70001), (130, 33), (1021, 257)]
+         (2, 4097), (3, 8191), (2, 8200), (1, 16385), (2, 32768), (1, 32777), (2, 70001), (130, 33), (1021, 257), (1025, 1000), (256, 4097), (256, 9001),
+         (257, 12300), (260, 16383), (256, 20000)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
