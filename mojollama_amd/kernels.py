@@ -339,6 +339,7 @@ class DeviceOps:
         self.so = so or load_kernels()
         # the current device as the runtime has it (no call here makes it the first to ask: tensors are there by then)
         self._cur_raw = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self._int8, self._f32 = torch.int8, torch.float32
         self._reals = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
         self._types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}
 
@@ -755,7 +756,7 @@ class DeviceOps:
 
     def _codes(self, t, what, cur, T, n):
         """_at of int8."""
-        if t.dtype != self.torch.int8:
+        if t.dtype != self._int8:
             raise TypeError(f"{what}: {t.dtype}, not int8")
         return self._at(t, what, cur, T, n)
 
@@ -763,33 +764,37 @@ class DeviceOps:
         """Address of a dense float32 [n] tensor on the current GPU (None: a null pointer)."""
         if t is None:
             return None
-        if t.get_device() != cur:
-            self._elsewhere(t, what)
-        if t.dtype != self.torch.float32 or t.numel() != n or not t.is_contiguous():
+        if t.dtype != self._f32 or t.numel() != n or not t.is_contiguous() or t.get_device() != cur:
+            if t.get_device() != cur:
+                self._elsewhere(t, what)
             raise ValueError(f"{what}: dense float32 [{n}]")
         return t.data_ptr()
 
     @staticmethod
     def _sizes(t, what):
-        if t.dim() != 2:
-            raise ValueError(f"{what}: [tokens, elements], got {list(t.shape)}")
-        return t.shape
+        s = t.shape
+        if len(s) != 2:
+            raise ValueError(f"{what}: [tokens, elements], got {list(s)}")
+        return s
 
-    def _i8_out(self, q, scale, T, n, cur):
-        """The outputs of the calls that quantise: rows of codes at multiples of 16 bytes, as i8_gemm takes them."""
+    def _i8_new(self, q, scale, T, n):
+        """The outputs of the calls that quantise, where they are not given: rows of codes at multiples of 16 bytes, as
+        i8_gemm takes them."""
         if q is None:
-            q = self.torch.empty((T, (n + 15) // 16 * 16), dtype=self.torch.int8, device="cuda")[:, :n]
+            q = self.torch.empty((T, (n + 15) // 16 * 16), dtype=self._int8, device="cuda")[:, :n]
         if scale is None:
-            scale = self.torch.empty(T, dtype=self.torch.float32, device="cuda")
-        qp, ql = self._codes(q, "q", cur, T, n)
-        return q, scale, qp, ql, self._floats(scale, "scale", cur, T)
+            scale = self.torch.empty(T, dtype=self._f32, device="cuda")
+        return q, scale
 
     def i8_quantize(self, x, q=None, scale=None):
         """mllm_i8_quantize: x [T, n] (float32, float16 or bfloat16) -> (q int8 [T, n], scale float32 [T])."""
         cur, xt = self._cur_raw(), self._real(x, "x")
         T, n = self._sizes(x, "x")
         xp, xl = self._at(x, "x", cur, T, n)
-        q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
+        if q is None or scale is None:
+            q, scale = self._i8_new(q, scale, T, n)
+        qp, ql = self._codes(q, "q", cur, T, n)
+        sp = self._floats(scale, "scale", cur, T)
         rc = self.so.mllm_i8_quantize(xt, xp, xl, T, n, qp, ql, sp, self._raw_stream(cur))
         if rc:
             self._check(rc, "mllm_i8_quantize")
@@ -828,11 +833,14 @@ class DeviceOps:
                     raise TypeError("res and res_out have one type")
         elif res_out is not None:
             raise ValueError("res_out belongs to res")
-        if w.get_device() != cur:
-            self._elsewhere(w, "w")
-        if w.numel() != n or not w.is_contiguous():
+        if w.numel() != n or not w.is_contiguous() or w.get_device() != cur:
+            if w.get_device() != cur:
+                self._elsewhere(w, "w")
             raise ValueError(f"w: dense [{n}]")
-        q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
+        if q is None or scale is None:
+            q, scale = self._i8_new(q, scale, T, n)
+        qp, ql = self._codes(q, "q", cur, T, n)
+        sp = self._floats(scale, "scale", cur, T)
         rc = self.so.mllm_i8_rms_norm(xt, xp, xl, rt, rp, rl, op, ol, wt, w.data_ptr(), eps, T, n, qp, ql, sp,
                                       self._raw_stream(cur))
         if rc:
@@ -847,7 +855,10 @@ class DeviceOps:
         if self._real(up, "up") != gt:
             raise TypeError("gate and up have one type")
         up_, ul = self._at(up, "up", cur, T, n)
-        q, scale, qp, ql, sp = self._i8_out(q, scale, T, n, cur)
+        if q is None or scale is None:
+            q, scale = self._i8_new(q, scale, T, n)
+        qp, ql = self._codes(q, "q", cur, T, n)
+        sp = self._floats(scale, "scale", cur, T)
         rc = self.so.mllm_i8_silu_mul(gt, gp, gl, up_, ul, T, n, qp, ql, sp, self._raw_stream(cur))
         if rc:
             self._check(rc, "mllm_i8_silu_mul")
