@@ -560,11 +560,9 @@ template <int MF, int NF, int WM, int WN, int OCC> constexpr tile_kind kind_of(f
     return {C::TT, C::TR, OCC, step, each, tail, go_tiles<MF, NF, WM, WN, OCC>};
 }
 const tile_kind kinds[] = {
-    kind_of<4, 4, 2, 2, 1>(0.0906f, 0.507f, 10.09f),
-    kind_of<2, 4, 2, 2, 1>(0.0899f, 0.2054f, 6.625f),
-    kind_of<2, 2, 2, 2, 2>(0.0f, 0.2337f, 1.912f),
-    kind_of<1, 2, 2, 2, 3>(0.0f, 0.1574f, 1.201f),
-    kind_of<1, 1, 1, 4, 3>(0.0422f, 0.0907f, 1.022f)};
+    kind_of<4, 4, 2, 2, 1>(0.150f, 0.440f, 10.0f), kind_of<2, 4, 2, 2, 1>(0.102f, 0.217f, 5.81f),
+    kind_of<2, 2, 2, 2, 2>(0.001f, 0.232f, 1.57f), kind_of<1, 2, 2, 2, 3>(0.0015f, 0.16f, 1.29f),
+    kind_of<1, 1, 1, 4, 3>(0.042f, 0.095f, 0.89f)};
 
 struct plan {
     const tile_kind *kind;         // or null:
@@ -573,8 +571,8 @@ struct plan {
 };
 
 // The kernel that an estimate of their times in microseconds, from sizes alone, puts first; its constants are fitted to
-// the kernels' times over 17 to 4096 tokens and nine matrices from 512 x 2048 to 32000 x 2048 and 1024 x 14336, where its
-// choice is 1 % slower than the best on average and 23 % at most.
+// the kernels' times at 1 to 4096 tokens and nine matrices from 512 x 2048 to 32000 x 2048 and 1024 x 14336, every tile
+// with K split up to twelve times.  There its choice is 0.8 % slower than the best on average, 11 % at most.
 plan plan_of(int T, int R, int kb, int cols)
 {
     plan best{};
@@ -582,12 +580,12 @@ plan plan_of(int T, int R, int kb, int cols)
     const float mb = (float)cols * R * 1e-6f;
     if (T <= 16) {
         const int n = (R + 15) / 16, turns = (cols + 1023) / 1024;
-        least = 2.9f + std::max((n + 511) / 512 * (0.6f + turns * 0.33f) + turns * (n / 512.0f) * (0.74f + T / 64.0f), mb / (5.3f - 0.08f * T));
+        least = 2.16f + std::max((n + 511) / 512 * (0.667f + turns * 0.315f) + turns * (n / 512.0f) * (0.977f + T * 0.0173f), mb / (4.13f - 0.0104f * T));
     }
     if (T <= 64) {
         const int n = (R + 31) / 32, turns = (cols + 1023) / 1024;
-        const float us = T <= 32 ? (T <= 16 ? 4.0f : 3.4f) + std::max(turns * 0.67f, mb / 5.3f) + n / 256.0f * 0.5f
-                                 : 4.0f + std::max(turns * 1.0f, mb / 4.2f) + n / 256.0f * 1.2f;
+        const float us = T <= 32 ? (T <= 16 ? 3.43f : 3.23f) + std::max(turns * 0.511f, mb / 6.14f) + n / 256.0f * 0.411f
+                                 : 4.14f + std::max(turns * 0.845f, mb / 5.01f) + n / 256.0f * 2.08f;
         if (us < least) {
             least = us;
             best.few = T <= 32 ? 1 : 2;
@@ -605,8 +603,8 @@ plan plan_of(int T, int R, int kb, int cols)
             if (p.splits != want || n > (want > 1 ? k.at_once() : 1l << 30)) continue;
             const int most = (int)((n + 255) / 256), full = most / k.per_cu, rest = most % k.per_cu;
             float us = full * (p.per * (k.step + k.per_cu * k.each) + k.tail) + (rest ? p.per * (k.step + rest * k.each) + k.tail : 0.0f);
-            us = 3.088f + std::max(us, (float)cols * ((float)R + T) / 5.7e6f);
-            if (want > 1) us += 3.422f + (float)n * k.TT * k.TR * 8 / 6.818e6f;
+            us = 2.96f + std::max(us, (float)cols * ((float)R + T) / 5.54e6f);
+            if (want > 1) us += 3.36f + (float)n * k.TT * k.TR * 8 / 6.3e6f;
             if (us < least) {
                 least = us;
                 best = p;
