@@ -663,7 +663,8 @@ MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_
  * token's results are the same bits whatever T is.  x: T rows of 8-bit integers (-128 among them)
  * at multiples of 16 bytes (x and x_ld; what lies behind a row's n_cols up to
  * the next multiple of 16 bytes may be read and has no part in the result).
- * Any T: few tokens stream the weights once, many run on tiles.  Workspace:
+ * Any T (a product of more than 10^11 results may be refused): few tokens
+ * stream the weights once, many run on tiles.  Workspace:
  * mllm_i8_gemm_workspace_size bytes, 16-byte aligned (NULL where that is 0);
  * one for T tokens serves every smaller T, and calls that overlap need one
  * each.  Results are the same from call to call. */

@@ -25,6 +25,15 @@ __host__ __device__ inline long i8_at(long kb, int r, int k)
     return ((r >> 5) * kb + (k >> 6)) * 2048 + ((k >> 4) & 3) * 512 + (r & 31) * 16 + (k & 15);
 }
 
+// A launch of `blocks` workgroups, more than fit the 2^32 lanes of one dimension too: block() of the kernel is below
+// blocks or behind them.
+constexpr long kI8Blocks = 1l << 21;
+inline dim3 i8_grid(long blocks, unsigned y = 1)
+{
+    return dim3((unsigned)(blocks < kI8Blocks ? blocks : kI8Blocks), y, (unsigned)((blocks + kI8Blocks - 1) / kI8Blocks));
+}
+__device__ __forceinline__ long i8_block() { return (long)blockIdx.z * gridDim.x + blockIdx.x; }
+
 inline bool i8_real(int type) { return type == MLLM_F32 || type == MLLM_F16 || type == MLLM_BF16; }
 
 // One or two floats as elements of the type.  A sum or product is a number of 32 bits before it is one of 16: the

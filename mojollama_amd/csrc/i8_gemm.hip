@@ -548,6 +548,7 @@ struct tile_kind {
     long at_once() const { return 256l * per_cu; }                       // workgroups that the GPU holds: splits go no further
 };
 constexpr int kMostSplits = 12;
+constexpr long kMostBlocks = (1l << 24) - 1;                         // of 256 lanes: the lanes of a launch stay below 2^32
 template <int MF, int NF, int WM, int WN, int OCC> void go_tiles(const gemm_args &a, int grid, hipStream_t st)
 {
     hipLaunchKernelGGL((k_i8_tiles<MF, NF, WM, WN, OCC>), dim3(grid), dim3(64 * WM * WN), 0, st, a);
@@ -566,7 +567,7 @@ const tile_kind kinds[] = {
 
 struct plan {
     const tile_kind *kind;         // or null:
-    int few;                       // 0: k_i8_few, 1, 2: k_i8_stream<few>
+    int few;                       // 0: no kernel, 1: k_i8_few, 2, 3: k_i8_stream<few - 1>
     int nt, nr, splits, per;
 };
 
@@ -578,17 +579,18 @@ plan plan_of(int T, int R, int kb, int cols)
     plan best{};
     float least = INFINITY;
     const float mb = (float)cols * R * 1e-6f;
-    if (T <= 16) {
+    if (T <= 16 && R < 1 << 26) {
         const int n = (R + 15) / 16, turns = (cols + 1023) / 1024;
         least = 2.16f + std::max((n + 511) / 512 * (0.667f + turns * 0.315f) + turns * (n / 512.0f) * (0.977f + T * 0.0173f), mb / (4.13f - 0.0104f * T));
+        best.few = 1;
     }
-    if (T <= 64) {
+    if (T <= 64 && R < 1 << 26) {
         const int n = (R + 31) / 32, turns = (cols + 1023) / 1024;
-        const float us = T <= 32 ? (T <= 16 ? 3.43f : 3.23f) + std::max(turns * 0.511f, mb / 6.14f) + n / 256.0f * 0.411f
+        const float us = T <= 32 ? (T <= 16 ? 3.85f : 3.23f) + std::max(turns * 0.511f, mb / 6.14f) + n / 256.0f * 0.411f
                                  : 4.14f + std::max(turns * 0.845f, mb / 5.01f) + n / 256.0f * 2.08f;
         if (us < least) {
             least = us;
-            best.few = T <= 32 ? 1 : 2;
+            best.few = T <= 32 ? 2 : 3;
         }
     }
     const int quads = kb / 4;
@@ -600,7 +602,7 @@ plan plan_of(int T, int R, int kb, int cols)
             p.per = (quads + want - 1) / want * 4;
             p.splits = (kb + p.per - 1) / p.per;
             const long n = (long)p.nt * p.nr * want;
-            if (p.splits != want || n > (want > 1 ? k.at_once() : 1l << 30)) continue;
+            if (p.splits != want || n > (want > 1 ? k.at_once() : kMostBlocks)) continue;
             const int most = (int)((n + 255) / 256), full = most / k.per_cu, rest = most % k.per_cu;
             float us = full * (p.per * (k.step + k.per_cu * k.each) + k.tail) + (rest ? p.per * (k.step + rest * k.each) + k.tail : 0.0f);
             us = 2.96f + std::max(us, (float)cols * ((float)R + T) / 5.54e6f);
@@ -660,15 +662,15 @@ MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t
     if (far) {
         a.nt = (T + 31) / 32;
         a.nr = (n_rows + 31) / 32;
-        if ((long)a.nt * a.nr > 1l << 30) return pk_fail(who, "T * n_rows is too large for one call");
+        if ((long)a.nt * a.nr > kMostBlocks) return pk_fail(who, "T * n_rows is too large for one call");
         hipLaunchKernelGGL(k_i8_far, dim3(a.nt * a.nr), dim3(64), 0, st, a);
     } else if (p.kind) {
         p.kind->go(a, p.nt * p.nr * p.splits, st);
-    } else if (p.few) {
+    } else if (p.few > 1) {
         const int grid = (n_rows + 31) / 32;
-        if (p.few == 1) hipLaunchKernelGGL((k_i8_stream<1, 8>), dim3(grid), dim3(512), 0, st, a);
+        if (p.few == 2) hipLaunchKernelGGL((k_i8_stream<1, 8>), dim3(grid), dim3(512), 0, st, a);
         else hipLaunchKernelGGL((k_i8_stream<2, 8>), dim3(grid), dim3(512), 0, st, a);
-    } else if (T <= 16) {
+    } else if (p.few) {
         const int grid = (n_rows + 15) / 16;
         // many workgroups hide each other's ends: eight waves each then (32000 x 2048, one token: 17.3 -> 14.9 us), few
         // are done sooner with sixteen (2048 x 5632: 7.0 -> 5.4 us)

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int L = per_wave ? 64 : blockDim.x, at = per_wave ? lane : threadIdx.x;
-    const long t = per_wave ? (long)blockIdx.x * waves + wave : blockIdx.x;
+    const long t = per_wave ? i8_block() * waves + wave : i8_block();
     if (t >= (PACK ? a.T_pad : a.T)) return;             // a whole wave, or the whole workgroup
     const bool real = !PACK || t < a.T;
     float y[NV][8];
@@ -368,7 +368,7 @@ template <int KIND, int XT, int RT, bool PACK> void go_rows(const row_args &a, h
                                                 : vecs <= 512 ? 512 : 1024;
     const int grid = per_wave ? (rows + 3) / 4 : rows;
     const int nv = per_wave ? (vecs + 63) / 64 : (vecs + threads - 1) / threads;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, a, per_wave); };
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, i8_grid(grid), dim3(threads), 0, st, a, per_wave); };
     if (nv <= 1) go(k_i8_rows<KIND, XT, RT, 1, PACK>);
     else if (nv == 2) go(k_i8_rows<KIND, XT, RT, 2, PACK>);
     else if (nv <= 4 || threads > 256) go(k_i8_rows<KIND, XT, RT, 4, PACK>);
@@ -380,8 +380,8 @@ template <int KIND, int XT, int RT, bool PACK> void go_rows(const row_args &a, h
 __global__ __launch_bounds__(256) void k_i8_pack(const int8_t *w, long w_ld, int n_rows, int n_cols, long kb, int8_t *packed)
 {
     const int u = blockIdx.y * 256 + threadIdx.x;        // chunk of 16 columns
-    const int r = blockIdx.x;
-    if (u >= kb * 4) return;
+    const int r = (int)i8_block();
+    if (u >= kb * 4 || r >= (n_rows + 31) / 32 * 32) return;
     raw<16> c{};
     if (r < n_rows) {
         const int8_t *p = w + r * w_ld + 16l * u;
@@ -398,7 +398,7 @@ template <int TYPE>
 __global__ __launch_bounds__(256) void k_i8_dequant(const int8_t *q, long q_ld, const float *scale, int T, int n, void *out,
                                                     long out_ld, int lpr_log)
 {
-    const long t = (long)blockIdx.x * (256 >> lpr_log) + (threadIdx.x >> lpr_log);
+    const long t = i8_block() * (256 >> lpr_log) + (threadIdx.x >> lpr_log);
     if (t >= T) return;
     const int lpr = 1 << lpr_log, lane = threadIdx.x & (lpr - 1);
     const float s = scale[t];
@@ -473,7 +473,7 @@ MLLM_API int mllm_i8_dequant(const int8_t *q, long q_ld, const float *scale, int
     while (lpr_log < 8 && 1 << lpr_log < vecs) lpr_log++;
     const int rows = 256 >> lpr_log, grid_y = std::min((vecs + (4 << lpr_log) - 1) / (4 << lpr_log), 1 << 14);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long)T + rows - 1) / rows), grid_y), dim3(256), 0, (hipStream_t)stream, q,
+        hipLaunchKernelGGL(kernel, i8_grid(((long)T + rows - 1) / rows, grid_y), dim3(256), 0, (hipStream_t)stream, q,
                            q_ld, scale, T, n, out, out_ld, lpr_log);
     };
     type == MLLM_F32 ? go(k_i8_dequant<MLLM_F32>) : type == MLLM_BF16 ? go(k_i8_dequant<MLLM_BF16>) : go(k_i8_dequant<MLLM_F16>);
@@ -541,7 +541,7 @@ MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_
     const int rows = (int)i8_rblocks(n_rows) * 32;
     hipStream_t st = (hipStream_t)stream;
     if (type == MLLM_I8) {
-        hipLaunchKernelGGL(k_i8_pack, dim3(rows, (unsigned)((kb * 4 + 255) / 256)), dim3(256), 0, st, (const int8_t *)w, w_ld,
+        hipLaunchKernelGGL(k_i8_pack, i8_grid(rows, (unsigned)((kb * 4 + 255) / 256)), dim3(256), 0, st, (const int8_t *)w, w_ld,
                            n_rows, n_cols, kb, (int8_t *)packed);
         return done(who);
     }

@@ -230,6 +230,19 @@ def test_many_results(dev):
     assert torch.equal(out[at], (q[at].double() @ w.double().T.contiguous()).float().bfloat16())
 
 
+@pytest.mark.parametrize("R", [(1 << 26) - 16, (1 << 26) + 1])
+def test_very_many_weight_rows(dev, R):
+    """Rows on both sides of where the kernels of few tokens end."""
+    C = 16
+    g = torch.Generator(device="cuda").manual_seed(4)
+    w = torch.randint(-128, 128, (R, C), dtype=torch.int8, device="cuda", generator=g)
+    q = torch.randint(-128, 128, (2, C), dtype=torch.int8, device="cuda", generator=g)
+    W = dev.i8_weights(w, torch.ones(R, device="cuda"))
+    out = dev.i8_gemm(W, q, torch.ones(2, device="cuda"), out_dtype=torch.float32)
+    at = torch.tensor([0, 1, 1 << 20, (1 << 25) + 7, R - 17, R - 1], device="cuda")
+    assert torch.equal(out[:, at].double(), q.double() @ w[at].double().T.contiguous())
+
+
 def test_far_rows(dev):
     """Rows of x and out beyond 2^31 bytes from the first."""
     T, C, R = 40, 100, 70

@@ -250,6 +250,20 @@ def test_many_elements(dev):
     assert torch.equal(dev.i8_dequant(q, s)[at], dev.i8_dequant(q1, s1))
 
 
+@pytest.mark.parametrize("T,n", [((1 << 26) + 70, 8), ((1 << 24) + 5, 1032)])
+def test_very_many_rows(dev, T, n):
+    """More rows than one dimension of a launch has workgroups for."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.empty((T, n), dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, (1 << 21) - 1, 1 << 21, 1 << 23, T - 2, T - 1], device="cuda")
+    rows = torch.randn((len(at), n), device="cuda", generator=g).bfloat16()
+    x[at] = rows
+    (q, s), (q1, s1) = dev.i8_quantize(x), dev.i8_quantize(rows)
+    assert torch.equal(q[at], q1) and torch.equal(s[at], s1)
+    del x
+    assert torch.equal(dev.i8_dequant(q, s)[at], dev.i8_dequant(q1, s1))
+
+
 def test_refused_tensors(dev):
     x, w = torch.zeros((3, 64), device="cuda"), torch.ones(64, device="cuda")
     cpu = torch.zeros((3, 64))
