@@ -339,6 +339,7 @@ class DeviceOps:
         self.so = so or load_kernels()
         # the current device as the runtime has it (no call here makes it the first to ask: tensors are there by then)
         self._cur_raw = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self._stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._int8, self._f32 = torch.int8, torch.float32
         self._reals = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
         self._types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}
@@ -745,14 +746,14 @@ class DeviceOps:
 
     def _at(self, t, what, cur, T, n):
         """(address, row stride) of a [T, n] tensor on the current GPU (cur) whose last dimension is dense."""
-        st = t.stride()
-        if t.shape != (T, n) or t.get_device() != cur or (st[1] != 1 and n > 1):
+        if t.shape != (T, n) or t.get_device() != cur:
             if t.get_device() != cur:
                 self._elsewhere(t, what)
-            if t.shape != (T, n):
-                raise ValueError(f"{what}: [{T}, {n}] is needed, got {list(t.shape)}")
+            raise ValueError(f"{what}: [{T}, {n}] is needed, got {list(t.shape)}")
+        ld, dense = t.stride()
+        if dense != 1 and n > 1:
             raise ValueError(f"{what}: the last dimension is not dense")
-        return t.data_ptr(), st[0] if T > 1 else n
+        return t.data_ptr(), ld if T > 1 else n
 
     def _codes(self, t, what, cur, T, n):
         """_at of int8."""
@@ -795,7 +796,7 @@ class DeviceOps:
             q, scale = self._i8_new(q, scale, T, n)
         qp, ql = self._codes(q, "q", cur, T, n)
         sp = self._floats(scale, "scale", cur, T)
-        rc = self.so.mllm_i8_quantize(xt, xp, xl, T, n, qp, ql, sp, self._raw_stream(cur))
+        rc = self.so.mllm_i8_quantize(xt, xp, xl, T, n, qp, ql, sp, self._stream_of(cur))
         if rc:
             self._check(rc, "mllm_i8_quantize")
         return q, scale
@@ -809,7 +810,7 @@ class DeviceOps:
             out = self.torch.empty((T, n), dtype=out_dtype or self.torch.bfloat16, device="cuda")
         ot = self._real(out, "out")
         op, ol = self._at(out, "out", cur, T, n)
-        rc = self.so.mllm_i8_dequant(qp, ql, self._floats(scale, "scale", cur, T), T, n, ot, op, ol, self._raw_stream(cur))
+        rc = self.so.mllm_i8_dequant(qp, ql, self._floats(scale, "scale", cur, T), T, n, ot, op, ol, self._stream_of(cur))
         if rc:
             self._check(rc, "mllm_i8_dequant")
         return out
@@ -842,7 +843,7 @@ class DeviceOps:
         qp, ql = self._codes(q, "q", cur, T, n)
         sp = self._floats(scale, "scale", cur, T)
         rc = self.so.mllm_i8_rms_norm(xt, xp, xl, rt, rp, rl, op, ol, wt, w.data_ptr(), eps, T, n, qp, ql, sp,
-                                      self._raw_stream(cur))
+                                      self._stream_of(cur))
         if rc:
             self._check(rc, "mllm_i8_rms_norm")
         return q, scale
@@ -859,7 +860,7 @@ class DeviceOps:
             q, scale = self._i8_new(q, scale, T, n)
         qp, ql = self._codes(q, "q", cur, T, n)
         sp = self._floats(scale, "scale", cur, T)
-        rc = self.so.mllm_i8_silu_mul(gt, gp, gl, up_, ul, T, n, qp, ql, sp, self._raw_stream(cur))
+        rc = self.so.mllm_i8_silu_mul(gt, gp, gl, up_, ul, T, n, qp, ql, sp, self._stream_of(cur))
         if rc:
             self._check(rc, "mllm_i8_silu_mul")
         return q, scale
@@ -896,7 +897,7 @@ class DeviceOps:
             self._elsewhere(ws, "workspace")
         rc = self.so.mllm_i8_gemm(weights._packed, weights._scale, qp, ql, self._floats(scale, "scale", cur, T), T, R,
                                   weights.n_cols, self._floats(bias, "bias", cur, R), ot, op, ol, ws.data_ptr(), ws.nbytes,
-                                  self._raw_stream(cur))
+                                  self._stream_of(cur))
         if rc:
             self._check(rc, "mllm_i8_gemm")
         return out
