@@ -5,7 +5,7 @@
 // along K.  A block holds [column chunk of 16][row][16 bytes], so that the 64 lanes of one load take 1 KB
 // in lane order and hold a v_mfma_i32_32x32x32_i8 operand (row lane % 32, chunk lane / 32), and the lanes
 // of v_mfma_i32_16x16x64_i8 (row lane % 16, chunk lane / 16) runs of 256 bytes.  Rows and columns are
-// padded with zeros (columns to 256): what a kernel reads of x behind its last column has no part in a sum.
+// padded with zeros (columns to 512): what a kernel reads of x behind its last column has no part in a sum.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -17,7 +17,7 @@
 
 constexpr int kI8MaxCols = 131071;         // 128 * 128 * 131071 < 2^31
 
-__host__ __device__ inline long i8_kblocks(int n_cols) { return ((long)n_cols + 255) / 256 * 4; }
+__host__ __device__ inline long i8_kblocks(int n_cols) { return ((long)n_cols + 511) / 512 * 8; }
 __host__ __device__ inline long i8_rblocks(int n_rows) { return ((long)n_rows + 31) / 32; }
 // Byte of element (r, k).
 __host__ __device__ inline long i8_at(long kb, int r, int k)

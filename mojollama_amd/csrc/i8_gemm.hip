@@ -26,7 +26,7 @@ struct gemm_args {
     const float *ws, *xs, *bias;
     void *out;
     long x_ld, out_ld;
-    int kb;                        // blocks of 64 columns, a multiple of four
+    int kb;                        // blocks of 64 columns, a multiple of eight
     int T, R, K, type;
     int nt, nr;                    // tiles along tokens and rows
     int splits, per;               // K in `splits` runs of `per` blocks
@@ -204,10 +204,13 @@ __device__ __forceinline__ work_tile tile_at(const gemm_args &a, int b, int n)
     return {z, p * a.panel + i - r * wide, r};
 }
 
-// A workgroup of WM x WN waves makes a tile of 32 MF WM tokens x 32 NF WN rows, a wave 32 MF x 32 NF of it.  K goes by
+// WM x WN waves make a tile of 32 MF WM tokens x 32 NF WN rows, a wave 32 MF x 32 NF of it.  K goes by
 // 64 columns a step.  Both operands come to LDS past the registers: the weights of a step into one of four buffers, up
 // to four steps ahead; x for two steps at once, so that a row is read in whole lines of 128 bytes (64 bytes at a time
-// cost twice the L2 traffic), into one of two.
+// cost twice the L2 traffic), into one of two.  Where tiles are fewer than CUs a step is as long as its latency: KG = 2
+// groups of waves, with buffers of their own, take half of K each, and the second hands its sums to the first by way of
+// LDS (256 x 4096 x 4096 with weights from memory: 15.9 -> 13.9 us, 512: 17.6 -> 16.8; for tiles of 128 x 128 and more,
+// whose steps are bound by their products, no gain).
 template <int MF, int NF, int WM, int WN> struct tile_of {
     static constexpr int waves = WM * WN, TT = 32 * MF * WM, TR = 32 * NF * WN;
     // 1 KB pieces of two steps of x, of a step of weights, and a wave's
@@ -218,20 +221,22 @@ template <int MF, int NF, int WM, int WN> struct tile_of {
 // Slot of a row's chunk of 16 bytes is chunk ^ swz(row): the reads of 16 rows, one chunk each, meet distinct banks.
 __device__ __forceinline__ int swz(int row) { return (row ^ (row >> 3 & 3)) & 7; }
 
-template <int MF, int NF, int WM, int WN, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void k_i8_tiles(gemm_args a)
+template <int MF, int NF, int WM, int WN, int KG, int OCC>
+__global__ __launch_bounds__(64 * WM * WN * KG, OCC) void k_i8_tiles(gemm_args a)
 {
     using C = tile_of<MF, NF, WM, WN>;
     // buffers of their own each: the compiler then knows which loads a read may meet
-    __shared__ __attribute__((aligned(1024))) uint8_t x0[C::xp * 1024], x1[C::xp * 1024], w0[C::wp * 1024], w1[C::wp * 1024],
-        w2[C::wp * 1024], w3[C::wp * 1024];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int XB = C::xp * 1024, WB = C::wp * 1024;
+    __shared__ __attribute__((aligned(1024))) uint8_t x0[KG * XB], x1[KG * XB], w0[KG * WB], w1[KG * WB], w2[KG * WB], w3[KG * WB];
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = all / C::waves, wave = all - group * C::waves;
     const int wm = wave % WM, wn = wave / WM, l = lane & 31, h = lane >> 5;
     const work_tile wt = tile_at(a, blockIdx.x, gridDim.x);
     const int z = wt.z, tile = wt.r * a.nt + wt.t, t0 = wt.t * C::TT, r0 = wt.r * C::TR;
-    const int s_beg = z * a.per, s_end = min(a.kb, s_beg + a.per);      // multiples of four
+    const int most = min(a.kb - z * a.per, a.per), steps = most / KG;   // multiples of four
+    const int s_beg = z * a.per + group * steps, s_end = s_beg + steps;
     __shared__ scales<C::TT, C::TR> sc;
-    scales_of<C::TT, C::TR, 64 * C::waves> have;
+    scales_of<C::TT, C::TR, 64 * C::waves * KG> have;
     if (a.splits == 1) get_scales(a, t0, r0, have, threadIdx.x);
 
     // ---- loads: a piece of x is 8 tokens x 128 columns (lane: token lane / 8, slot lane % 8), of the weights 1 KB as
@@ -255,14 +260,14 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_i8_tiles(gemm_args a)
         const int more = xs + 2 < s_end;
 #pragma unroll
         for (int p = 0; p < C::px; p++) {
-            to_lds(xr, to + 1024 * (p * C::waves + wave), xo[p], 0);
+            to_lds(xr, to + group * XB + 1024 * (p * C::waves + wave), xo[p], 0);
             xo[p] += 128 * more;
         }
         xs += 2 * more;
     };
     auto load_w = [&](uint8_t *to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < C::pw; p++) to_lds(wr, to + 1024 * (p * C::waves + wave), wo[p], ws * 2048);
+        for (int p = 0; p < C::pw; p++) to_lds(wr, to + group * WB + 1024 * (p * C::waves + wave), wo[p], ws * 2048);
         ws += ws + 1 < s_end;
     };
     i32x16 acc[MF][NF];
@@ -277,9 +282,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_i8_tiles(gemm_args a)
     for (int j = 0; j < 4; j++) xa[j] = l * 128 + 16 * ((2 * j + h) ^ swz(l));
     auto get = [&](const uint8_t *fx, const uint8_t *fw, auto j, frags &f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NF; n++) f.w[n] = *(const i32x4 *)(fw + (wn * NF + n) * 2048 + (j & 1) * 1024 + lane * 16);
+        for (int n = 0; n < NF; n++) f.w[n] = *(const i32x4 *)(fw + group * WB + (wn * NF + n) * 2048 + (j & 1) * 1024 + lane * 16);
 #pragma unroll
-        for (int m = 0; m < MF; m++) f.x[m] = *(const i32x4 *)(fx + (wm * MF + m) * 4096 + xa[j]);
+        for (int m = 0; m < MF; m++) f.x[m] = *(const i32x4 *)(fx + group * XB + (wm * MF + m) * 4096 + xa[j]);
     };
     auto multiply = [&](const frags &f) __attribute__((always_inline)) {
 #pragma unroll
@@ -334,6 +339,35 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_i8_tiles(gemm_args a)
     } while (s < s_end);
     wait_mem<0>();
     __builtin_amdgcn_s_barrier();
+    if constexpr (KG > 1) {
+        // the second group's sums to the first, by way of LDS: a wave's 4 KB pieces in its weights' buffers
+        static_assert(KG == 2 && MF * NF * 4 * C::waves <= KG * 4 * C::wp, "the sums fit the weights' buffers");
+        constexpr int each_buffer = KG * WB / (4096 * C::waves);         // pieces of a wave that a buffer takes
+        static_assert(each_buffer >= 1 && MF * NF <= 4 * each_buffer, "");
+        auto piece = [&](int i) __attribute__((always_inline)) {
+            uint8_t *b = i / each_buffer == 0 ? w0 : i / each_buffer == 1 ? w1 : i / each_buffer == 2 ? w2 : w3;
+            return b + (wave * each_buffer + i % each_buffer) * 4096 + lane * 16;
+        };
+        each<MF * NF>([&](auto i) __attribute__((always_inline)) {
+            if (group == 1) {
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *(i32x4 *)(piece(i) + g * 1024) = (i32x4){acc[i / NF][i % NF][4 * g], acc[i / NF][i % NF][4 * g + 1],
+                                                              acc[i / NF][i % NF][4 * g + 2], acc[i / NF][i % NF][4 * g + 3]};
+            }
+        });
+        __syncthreads();
+        if (group == 1) return;
+        each<MF * NF>([&](auto i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const i32x4 v = *(const i32x4 *)(piece(i) + g * 1024);
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[i / NF][i % NF][4 * g + k] += v[k];
+            }
+        });
+        wait_mem<0>();
+    }
 
     if (a.splits > 1) {
         int *p = a.part + (((long)z * a.nt * a.nr + tile) * C::waves + wave) * (MF * NF * 1024) + lane * 4;
@@ -348,7 +382,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_i8_tiles(gemm_args a)
         return;
     }
     static_assert(C::waves == 4 && room_bytes<NF>() <= C::wp * 1024, "the tail of a wave fits a buffer of weights");
-    uint8_t *room = wave == 0 ? w0 : wave == 1 ? w1 : wave == 2 ? w2 : w3;
+    uint8_t *room = KG > 1 ? (wave < 2 ? x0 : x1) + (wave & 1) * room_bytes<NF>()
+                           : wave == 0 ? w0 : wave == 1 ? w1 : wave == 2 ? w2 : w3;
+    static_assert(KG == 1 || 2 * room_bytes<NF>() <= KG * XB, "x's buffers hold the tails of four waves");
     const int c = wn * NF * 32 + lane % (4 * NF) * 8;
     float rs[8], bias[8];
 #pragma unroll
@@ -541,29 +577,35 @@ __global__ __launch_bounds__(64) void k_i8_far(gemm_args a)
 
 // ------------------------------------------------------------------------------------ the choice
 struct tile_kind {
-    int TT, TR, per_cu;            // workgroups of it that a CU holds
+    int TT, TR, groups, per_cu;    // groups of waves, workgroups of it that a CU holds
     float step, each, tail;        // microseconds of a step of K, of each workgroup in it, of a workgroup beside
     void (*go)(const gemm_args &, int grid, hipStream_t);
-    bool fits(int T) const { return TT < 64 || TT < 2 * T; }             // not mostly empty
+    // A tile is not mostly empty.  Up to 32 tokens the time is that of the weights' stream, which two groups do not
+    // shorten: 16 tokens of 11264 x 2048 take them 9.3 us, k_i8_stream 7.4.
+    bool fits(int T) const { return groups > 1 ? T > 32 && TT < 2 * T : TT < 64 || TT < 2 * T; }
     long at_once() const { return 256l * per_cu; }                       // workgroups that the GPU holds: splits go no further
 };
 constexpr int kMostSplits = 12;
 constexpr long kMostBlocks = (1l << 24) - 1;                         // of 256 lanes: the lanes of a launch stay below 2^32
-template <int MF, int NF, int WM, int WN, int OCC> void go_tiles(const gemm_args &a, int grid, hipStream_t st)
+template <int MF, int NF, int WM, int WN, int KG, int OCC> void go_tiles(const gemm_args &a, int grid, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_i8_tiles<MF, NF, WM, WN, OCC>), dim3(grid), dim3(64 * WM * WN), 0, st, a);
+    hipLaunchKernelGGL((k_i8_tiles<MF, NF, WM, WN, KG, OCC>), dim3(grid), dim3(64 * WM * WN * KG), 0, st, a);
     if (a.splits > 1)
         hipLaunchKernelGGL((k_i8_join<MF, NF, WM, WN>), dim3(a.nt * a.nr * MF * WM * WN), dim3(64), 0, st, a);
 }
-template <int MF, int NF, int WM, int WN, int OCC> constexpr tile_kind kind_of(float step, float each, float tail)
+template <int MF, int NF, int WM, int WN, int KG, int OCC> constexpr tile_kind kind_of(float step, float each, float tail)
 {
     using C = tile_of<MF, NF, WM, WN>;
-    return {C::TT, C::TR, OCC, step, each, tail, go_tiles<MF, NF, WM, WN, OCC>};
+    return {C::TT, C::TR, KG, OCC, step, each, tail, go_tiles<MF, NF, WM, WN, KG, OCC>};
 }
 const tile_kind kinds[] = {
-    kind_of<4, 4, 2, 2, 1>(0.150f, 0.440f, 10.0f), kind_of<2, 4, 2, 2, 1>(0.102f, 0.217f, 5.81f),
-    kind_of<2, 2, 2, 2, 2>(0.001f, 0.232f, 1.57f), kind_of<1, 2, 2, 2, 3>(0.0015f, 0.16f, 1.29f),
-    kind_of<1, 1, 1, 4, 3>(0.042f, 0.095f, 0.89f)};
+    kind_of<4, 4, 2, 2, 1, 1>(0.13f, 0.512f, 8.64f),
+    kind_of<2, 4, 2, 2, 1, 1>(0.0809f, 0.23f, 7.35f),
+    kind_of<2, 2, 2, 2, 1, 2>(0.0019f, 0.25f, 1.09f),
+    kind_of<1, 2, 2, 2, 1, 3>(0.000255f, 0.193f, 0.328f),
+    kind_of<1, 1, 1, 4, 1, 3>(0.0236f, 0.1075f, 1.9f),
+    kind_of<1, 2, 2, 2, 2, 1>(0.00935f, 0.157f, 1.18f),
+    kind_of<1, 1, 1, 4, 2, 1>(0.00668f, 0.1247f, 1.01f)};
 
 struct plan {
     const tile_kind *kind;         // or null:
@@ -573,7 +615,7 @@ struct plan {
 
 // The kernel that an estimate of their times in microseconds, from sizes alone, puts first; its constants are fitted to
 // the kernels' times at 1 to 4096 tokens and nine matrices from 512 x 2048 to 32000 x 2048 and 1024 x 14336, every tile
-// with K split up to twelve times.  There its choice is 0.8 % slower than the best on average, 11 % at most.
+// with K split up to twelve times.  There its choice is 0.6 % slower than the best on average, 10 % at most.
 plan plan_of(int T, int R, int kb, int cols)
 {
     plan best{};
@@ -581,32 +623,33 @@ plan plan_of(int T, int R, int kb, int cols)
     const float mb = (float)cols * R * 1e-6f;
     if (T <= 16 && R < 1 << 26) {
         const int n = (R + 15) / 16, turns = (cols + 1023) / 1024;
-        least = 2.16f + std::max((n + 511) / 512 * (0.667f + turns * 0.315f) + turns * (n / 512.0f) * (0.977f + T * 0.0173f), mb / (4.13f - 0.0104f * T));
+        least = 1.78f + std::max((n + 511) / 512 * (0.749f + turns * 0.285f) + turns * (n / 512.0f) * (1.05f + T * 0.0357f),
+                                 mb / (6.88f - 0.016f * T));
         best.few = 1;
     }
     if (T <= 64 && R < 1 << 26) {
         const int n = (R + 31) / 32, turns = (cols + 1023) / 1024;
-        const float us = T <= 32 ? (T <= 16 ? 3.85f : 3.23f) + std::max(turns * 0.511f, mb / 6.14f) + n / 256.0f * 0.411f
-                                 : 4.14f + std::max(turns * 0.845f, mb / 5.01f) + n / 256.0f * 2.08f;
+        const float us = T <= 32 ? (T <= 16 ? 4.25f : 3.5f) + std::max(turns * 0.4f, mb / 6.22f) + n / 256.0f * 0.0897f
+                                 : 3.79f + std::max(turns * 0.85f, mb / 5.64f) + n / 256.0f * 3.82f;
         if (us < least) {
             least = us;
             best.few = T <= 32 ? 2 : 3;
         }
     }
-    const int quads = kb / 4;
+    const int units = kb / 8;
     for (const tile_kind &k : kinds) {
         if (!k.fits(T)) continue;
         for (int want : {1, 2, 3, 4, 6, 8, kMostSplits}) {
             plan p{&k, 0, (T + k.TT - 1) / k.TT, (R + k.TR - 1) / k.TR, 0, 0};
-            if (want > quads) continue;
-            p.per = (quads + want - 1) / want * 4;
+            if (want > units) continue;
+            p.per = (units + want - 1) / want * 8;
             p.splits = (kb + p.per - 1) / p.per;
             const long n = (long)p.nt * p.nr * want;
             if (p.splits != want || n > (want > 1 ? k.at_once() : kMostBlocks)) continue;
             const int most = (int)((n + 255) / 256), full = most / k.per_cu, rest = most % k.per_cu;
             float us = full * (p.per * (k.step + k.per_cu * k.each) + k.tail) + (rest ? p.per * (k.step + rest * k.each) + k.tail : 0.0f);
-            us = 2.96f + std::max(us, (float)cols * ((float)R + T) / 5.54e6f);
-            if (want > 1) us += 3.36f + (float)n * k.TT * k.TR * 8 / 6.3e6f;
+            us = 2.35f + std::max(us, (float)cols * ((float)R + T) / 5.52e6f);
+            if (want > 1) us += 4.56f + (float)n * k.TT * k.TR * 8 / 5.51e6f;
             if (us < least) {
                 least = us;
                 best = p;
@@ -621,8 +664,8 @@ long sums_of(int T, int R, int kb)
 {
     long most = 0;
     for (const tile_kind &k : kinds) {
-        const long nr = (R + k.TR - 1) / k.TR, n = std::min((long)std::min(kb / 4, kMostSplits) * ((T + k.TT - 1) / k.TT) * nr, k.at_once());
-        if (k.fits(T) && kb > 4 && 2 * nr <= k.at_once()) most = std::max(most, n * k.TT * k.TR * 4);
+        const long nr = (R + k.TR - 1) / k.TR, n = std::min((long)std::min(kb / 8, kMostSplits) * ((T + k.TT - 1) / k.TT) * nr, k.at_once());
+        if (k.fits(T) && kb > 8 && 2 * nr <= k.at_once()) most = std::max(most, n * k.TT * k.TR * 4);
     }
     return most;
 }

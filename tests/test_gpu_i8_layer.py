@@ -74,7 +74,7 @@ def batch(lens, new, seed):
 
 def product(q, s, W, bias=None):
     """Codes of the weights read back from the packed blocks [rows / 32][cols / 64][chunk][row][16]."""
-    kb = (W.n_cols + 255) // 256 * 4
+    kb = (W.n_cols + 511) // 512 * 8
     w = W.packed.view(torch.int8).view(-1, kb, 4, 32, 16).permute(0, 3, 1, 2, 4).reshape(-1, kb * 64)[:W.n_rows, :W.n_cols]
     y = (q.cpu().double() @ w.cpu().double().T) * s.cpu().double()[:, None] * W.scale.cpu().double()
     return y if bias is None else y + bias.cpu().double()

@@ -93,8 +93,8 @@ def test_nothing(so):
 
 
 def test_sizes(so):
-    assert so.mllm_i8_packed_size(1, 1) == 32 * 256
-    assert so.mllm_i8_packed_size(33, 257) == 64 * 512
+    assert so.mllm_i8_packed_size(1, 1) == 32 * 512
+    assert so.mllm_i8_packed_size(33, 513) == 64 * 1024
     assert so.mllm_i8_packed_size(40, 131071) == 64 * 131072
     for rows, cols in ((0, 5), (5, 0), (-1, 5), (5, 131072)):
         assert so.mllm_i8_packed_size(rows, cols) == -1 and so.mllm_i8_gemm_workspace_size(3, rows, cols) == -1

@@ -16,8 +16,8 @@ import pytest
 from mojollama_amd import kernels
 from test_gemm16_waits import OBJDUMP, code_objects
 
-# (MF, NF, WM, WN) of the tiles: 32 MF WM tokens x 32 NF WN rows
-TILES = [(4, 4, 2, 2), (2, 4, 2, 2), (2, 2, 2, 2), (1, 2, 2, 2), (1, 1, 1, 4)]
+# (MF, NF, WM, WN, KG) of the tiles: 32 MF WM tokens x 32 NF WN rows, KG groups of waves
+TILES = [(4, 4, 2, 2, 1), (2, 4, 2, 2, 1), (2, 2, 2, 2, 1), (1, 2, 2, 2, 1), (1, 1, 1, 4, 1), (1, 2, 2, 2, 2), (1, 1, 1, 4, 2)]
 
 
 @pytest.fixture(scope="module")
@@ -31,7 +31,7 @@ def bodies(tmp_path_factory):
     f = tmp_path_factory.mktemp("co") / "i8_gemm.co"
     f.write_bytes(obj[0])
     text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", str(f)], capture_output=True, text=True, check=True).stdout
-    return {tuple(map(int, re.findall(r"Li(\d+)E", name)[:4])): body.splitlines()
+    return {tuple(map(int, re.findall(r"Li(\d+)E", name)[:5])): body.splitlines()
             for name, body in re.findall(r"^[0-9a-f]+ <(_Z\S*10k_i8_tilesI\S*?)>:\n(.*?)(?=^\S|\Z)", text, re.M | re.S)}
 
 
@@ -66,7 +66,7 @@ def events(lines):
 
 @pytest.mark.parametrize("tile", TILES)
 def test_loop(bodies, tile):
-    MF, NF, WM, WN = tile
+    MF, NF, WM, WN, _ = tile
     px, pw = 32 * MF * WM // 8 // (WM * WN), 32 * NF * WN // 16 // (WM * WN)
     ev = events(bodies[tile])
     # the loop of K: the jump back over the most matrix instructions
