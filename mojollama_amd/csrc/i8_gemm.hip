@@ -599,13 +599,13 @@ template <int MF, int NF, int WM, int WN, int KG, int OCC> constexpr tile_kind k
     return {C::TT, C::TR, KG, OCC, step, each, tail, go_tiles<MF, NF, WM, WN, KG, OCC>};
 }
 const tile_kind kinds[] = {
-    kind_of<4, 4, 2, 2, 1, 1>(0.13f, 0.512f, 8.64f),
-    kind_of<2, 4, 2, 2, 1, 1>(0.0809f, 0.23f, 7.35f),
-    kind_of<2, 2, 2, 2, 1, 2>(0.0019f, 0.25f, 1.09f),
-    kind_of<1, 2, 2, 2, 1, 3>(0.000255f, 0.193f, 0.328f),
-    kind_of<1, 1, 1, 4, 1, 3>(0.0236f, 0.1075f, 1.9f),
-    kind_of<1, 2, 2, 2, 2, 1>(0.00935f, 0.157f, 1.18f),
-    kind_of<1, 1, 1, 4, 2, 1>(0.00668f, 0.1247f, 1.01f)};
+    kind_of<4, 4, 2, 2, 1, 1>(0.37f, 0.202f, 10.7f),
+    kind_of<2, 4, 2, 2, 1, 1>(0.134f, 0.26f, 5.23f),
+    kind_of<2, 2, 2, 2, 1, 2>(0.000872f, 0.265f, 2.08f),
+    kind_of<1, 2, 2, 2, 1, 3>(0.000546f, 0.274f, 0.0339f),
+    kind_of<1, 1, 1, 4, 1, 3>(0.0854f, 0.121f, 0.0782f),
+    kind_of<1, 2, 2, 2, 2, 1>(0.00158f, 0.175f, 2.41f),
+    kind_of<1, 1, 1, 4, 2, 1>(0.0051f, 0.156f, 0.805f)};
 
 struct plan {
     const tile_kind *kind;         // or null:
@@ -614,8 +614,9 @@ struct plan {
 };
 
 // The kernel that an estimate of their times in microseconds, from sizes alone, puts first; its constants are fitted to
-// the kernels' times at 1 to 4096 tokens and nine matrices from 512 x 2048 to 32000 x 2048 and 1024 x 14336, every tile
-// with K split up to twelve times.  There its choice is 0.6 % slower than the best on average, 10 % at most.
+// the kernels' times with weights from memory, at 1 to 4096 tokens and seventeen matrices from 512 x 2048 to
+// 32000 x 2048 and 1024 x 14336, every tile with K split up to twelve times (3540 times).  There its choice is 0.6 %
+// slower than the best on average, 18 % at most.
 plan plan_of(int T, int R, int kb, int cols)
 {
     plan best{};
@@ -623,14 +624,14 @@ plan plan_of(int T, int R, int kb, int cols)
     const float mb = (float)cols * R * 1e-6f;
     if (T <= 16 && R < 1 << 26) {
         const int n = (R + 15) / 16, turns = (cols + 1023) / 1024;
-        least = 1.78f + std::max((n + 511) / 512 * (0.749f + turns * 0.285f) + turns * (n / 512.0f) * (1.05f + T * 0.0357f),
-                                 mb / (6.88f - 0.016f * T));
+        least = 2.11f + std::max((n + 511) / 512 * (0.711f + turns * 0.38f) + turns * (n / 512.0f) * (0.669f + T * 0.0419f),
+                                 mb / (4.46f - 0.0333f * T));
         best.few = 1;
     }
     if (T <= 64 && R < 1 << 26) {
         const int n = (R + 31) / 32, turns = (cols + 1023) / 1024;
-        const float us = T <= 32 ? (T <= 16 ? 4.25f : 3.5f) + std::max(turns * 0.4f, mb / 6.22f) + n / 256.0f * 0.0897f
-                                 : 3.79f + std::max(turns * 0.85f, mb / 5.64f) + n / 256.0f * 3.82f;
+        const float us = T <= 32 ? 2.19f + std::max(turns * 1.14f, mb / 5.66f) + n / 256.0f * (0.376f + turns * T * 0.00271f)
+                                 : 1.79f + std::max(turns * 2.02f, mb / 4.28f) + n / 256.0f * 2.1f;
         if (us < least) {
             least = us;
             best.few = T <= 32 ? 2 : 3;
@@ -648,8 +649,8 @@ plan plan_of(int T, int R, int kb, int cols)
             if (p.splits != want || n > (want > 1 ? k.at_once() : kMostBlocks)) continue;
             const int most = (int)((n + 255) / 256), full = most / k.per_cu, rest = most % k.per_cu;
             float us = full * (p.per * (k.step + k.per_cu * k.each) + k.tail) + (rest ? p.per * (k.step + rest * k.each) + k.tail : 0.0f);
-            us = 2.35f + std::max(us, (float)cols * ((float)R + T) / 5.52e6f);
-            if (want > 1) us += 4.56f + (float)n * k.TT * k.TR * 8 / 5.51e6f;
+            us = 2.54f + std::max(us, (float)cols * ((float)R + T) / 5.38e6f);
+            if (want > 1) us += 4.44f + (float)n * k.TT * k.TR * 8 / 7.49e6f;
             if (us < least) {
                 least = us;
                 best = p;
