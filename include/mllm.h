@@ -618,12 +618,13 @@ MLLM_API int mllm_pages_copy(const mllm_page_plane *planes, int n_planes, int n_
 
 /* ------------------------- layers in 8-bit integers: a scale per row and token
  * A quantised row stands for scale * q[i], i < n, with 8-bit integers q and an
- * fp32 scale.  T, n and n_rows are at most 2^30.  The calls below that form one from values y[i] take
+ * fp32 scale.  T, n and n_rows are at most 2^30.  The calls below that form one
+ * from values y[i] take
  *   q[i] = y[i] * (127 * (1 / max|y|)) to the nearest integer (ties to even),
  *   scale = max|y| / 127,
- * in fp32, operation by operation; a row of zeros has scale 0 and zeros; a row that holds an
- * infinity or a NaN has scale NaN and zeros, so that every product with it is
- * NaN.  T rows of x lie x_ld elements apart (at least n; x_ld of codes in
+ * in fp32, operation by operation; a row of zeros has scale 0 and zeros; a row
+ * that holds an infinity or a NaN has scale NaN and zeros, so that every product
+ * with it is NaN.  T rows of x lie x_ld elements apart (at least n; x_ld of codes in
  * bytes), T = 0 does nothing, n is positive.  Rows need no alignment beyond
  * their elements' own; wide loads and stores are used at any address.  type:
  * MLLM_F32, MLLM_F16 or MLLM_BF16.  What lies between the rows of an output
@@ -660,9 +661,10 @@ MLLM_API int mllm_i8_pack(int type, const void *w, long w_ld, int n_rows, int n_
 /* out[t][r] = (sum_k x[t][k] w[r][k]) * x_scale[t] * w_scale[r] (+ bias[r],
  * fp32, optional), the sums exact in 32-bit integers, the rest in fp32 in that
  * order (the second product and the bias as one fma), then rounded to type: a
- * token's results are the same bits whatever T is.  x: T rows of 8-bit integers (-128 among them)
- * at multiples of 16 bytes (x and x_ld; what lies behind a row's n_cols up to
- * the next multiple of 16 bytes may be read and has no part in the result).
+ * token's results are the same bits whatever T is.  x: T rows of 8-bit integers
+ * (-128 among them) at multiples of 16 bytes (x and x_ld; what lies between the
+ * rows, and behind the last up to the next multiple of 16 bytes, may be read and
+ * has no part in the result).
  * Any T (a product of more than 10^11 results may be refused): few tokens
  * stream the weights once, many run on tiles.  Workspace:
  * mllm_i8_gemm_workspace_size bytes, 16-byte aligned (NULL where that is 0);
