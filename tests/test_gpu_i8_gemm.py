@@ -105,6 +105,15 @@ def test_large(dev, T, R, C):
     case(dev, T, R, C, "bf16", bias=True)
 
 
+@pytest.mark.parametrize("T,R,C", [(4395, 2808, 588), (803, 16265, 542), (2722, 900, 13500), (2538, 1589, 1056), (213, 5577, 11771),
+                                   (3235, 962, 69), (598, 5345, 67), (3216, 41, 8198), (4278, 138, 74), (105, 8620, 65),
+                                   (1203, 41, 3636), (556, 1800, 5351), (4341, 129, 1744), (1502, 45, 10297), (393, 473, 19424)])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_ragged_tiles(dev, T, R, C, out):
+    """Tiles of every size with ragged ends in each direction, K whole and split."""
+    case(dev, T, R, C, out, bias=True, ld=5, extra=1)
+
+
 @pytest.mark.parametrize("T", [1, 20, 150, 400])
 @pytest.mark.parametrize("x,w", [(-128, -128), (127, -128), (127, 127)])
 def test_largest_sums(dev, T, x, w):
