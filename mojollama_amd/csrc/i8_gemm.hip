@@ -9,8 +9,9 @@
 //
 // Measured (MI355X, bf16 out, codes of normal values): 8192 tokens x 8192 x 8192 in 416 us, 2640 TOPS, where a
 // loop of these matrix instructions on registers alone reaches 3400 (4500 with codes of zero, as this product
-// comes to 3900 with them: what bounds it is power); 1024 tokens x 4096 x 4096 in 22.7 us; 64 in 9 to 10.5;
-// one in 5.8, 2.9 TB/s, of which the launch is 2.2.
+// comes to 3900 with them: what bounds it is power); with weights from memory (in the last cache) 1024 tokens x
+// 4096 x 4096 in 22.5 us (21.2), 256 in 13.1 (10.5), 64 in 10.5 (8.4), 16 in 6.6 (5.7), one in 6.2 (5.4), of which the
+// launch is 2.2.
 #include <algorithm>
 #include <type_traits>
 #include "i8.h"
@@ -478,8 +479,10 @@ template <int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
 
 // 32 weight rows x 32 TF tokens a workgroup of W waves, which take blocks of 128 columns in turn and join their sums in
 // LDS.  A wave's block of x comes to its own part of LDS in whole lines and its weights to registers, two blocks under
-// way; waves meet at the end alone.  (32 tokens x 4096 x 4096: 6.9 us, 8.0 with x from the caches; 16 x 8192 x 8192:
-// 15.1 us, 4.4 TB/s, 19.4 with 16 rows a workgroup.  96 and 128 tokens would be bound by LDS: 12.6 and 14 us, tiles 11.)
+// way; waves meet at the end alone.  (32 tokens x 4096 x 4096 with weights in the last cache: 6.4 us, 8.0 with x from the
+// caches; 16 x 8192 x 8192 from memory: 14.5 us, 4.6 TB/s, 19.4 with 16 rows a workgroup.  96 and 128 tokens would be
+// bound by LDS: 12.6 and 14 us, tiles 11.  64 rows a workgroup: 48 tokens x 14336 x 4096 18.0 us for 21.6, but tiles take
+// 17.6, and 10 to 60 % slower where rows are fewer.)
 template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_stream(gemm_args a)
 {
     constexpr int XB = TF * 4096, LOADS = 4 * TF + 4;            // bytes and loads of a block
