@@ -780,9 +780,10 @@ class DeviceOps:
 
     def _i8_new(self, q, scale, T, n):
         """The outputs of the calls that quantise, where they are not given: rows of codes at multiples of 16 bytes, as
-        i8_gemm takes them."""
+        i8_gemm takes them; long ones at whole lines (1000 tokens x 2048 x 2048: 9.0 us, 9.9 with rows 16 bytes off)."""
         if q is None:
-            q = self.torch.empty((T, (n + 15) // 16 * 16), dtype=self._int8, device="cuda")[:, :n]
+            step = 128 if n >= 1024 else 16
+            q = self.torch.empty((T, (n + step - 1) // step * step), dtype=self._int8, device="cuda")[:, :n]
         if scale is None:
             scale = self.torch.empty(T, dtype=self._f32, device="cuda")
         return q, scale
