@@ -230,9 +230,10 @@ __device__ __forceinline__ void load(const row_args &a, long t, int e, int left,
     if constexpr (KIND == NORM_RES || KIND == SILU) r = ld8<size_of(RT)>(a.res, t * a.res_ld + e, left);
 }
 
-// The norm's factor with squares and their sum in 64 bits; every wave of the row forms it alike.
+// The norm's factor with squares and their sum in 64 bits, where it may itself leave fp32 (eps 0 and a row below 2^-128);
+// every wave of the row forms it alike.
 template <int KIND, int XT, int RT>
-__device__ float far_factor(const row_args &a, long t, int lane)
+__device__ double far_factor(const row_args &a, long t, int lane)
 {
     double sum = 0.0;
     for (int e = 8 * lane; e < a.n; e += 512) {
@@ -244,7 +245,7 @@ __device__ float far_factor(const row_args &a, long t, int lane)
         for (int i = 0; i < 8; i++) sum += (double)h[i] * h[i];
     }
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    return (float)(1.0 / sqrt(sum / a.n + (double)a.eps));
+    return 1.0 / sqrt(sum / a.n + (double)a.eps);
 }
 
 // A row over L = blockDim.x lanes (PER_WAVE: a row per wave).  NV vectors of eight elements a lane stay in
@@ -305,17 +306,14 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
     }
     const row_step s = step_of(__builtin_amdgcn_readfirstlane(m));
     // squares that leave fp32, or vanish in it where eps does not stand above them, are summed again in 64 bits
-    float s_factor = 1.0f, mean = sq / (float)a.n;
+    float step = s.most / 127.0f;
     if constexpr (KIND == NORM || KIND == NORM_RES) {
+        const float mean = sq / (float)a.n;
         if (real && !s.bad && m != 0 && (!(mean < 0x1p100f) || (mean < 0x1p-100f && a.eps < 0x1p-100f)))
-            s_factor = far_factor<KIND, XT, RT>(a, t, lane);
-        else s_factor = 1.0f / sqrtf(mean + a.eps);
+            step = (float)(s.most * far_factor<KIND, XT, RT>(a, t, lane) / 127.0);
+        else step = s.most * (1.0f / sqrtf(mean + a.eps)) / 127.0f;
     }
-    if (at == 0 && real) {
-        float k = s.most;
-        k *= s_factor;
-        a.scale[t] = s.bad ? NAN : m == 0 ? 0.0f : k / 127.0f;
-    }
+    if (at == 0 && real) a.scale[t] = s.bad ? NAN : m == 0 ? 0.0f : step;
     const int n = PACK ? a.n_pad : a.n;
     auto put = [&](int e, const float (&z)[8]) {
         const uint2 c = codes(z, s);
