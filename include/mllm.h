@@ -641,7 +641,9 @@ MLLM_API int mllm_i8_dequant(const int8_t *q, long q_ld, const float *scale, int
  * goes to res_out (res NULL: h = x, nothing is stored).  res_out may be res, or
  * x where res_type is type, in the same stride.  w [n]: w_type MLLM_F32 or any
  * of the three.  eps is finite and not negative.  The norm's factor is one
- * number per row, so it enters the scale alone: q is formed from w h. */
+ * number per row, so it enters the scale alone: q is formed from w h, times a
+ * power of two where w h itself would leave fp32.  The row holds an infinity
+ * where y does. */
 MLLM_API int mllm_i8_rms_norm(int type, const void *x, long x_ld, int res_type, const void *res, long res_ld,
                               void *res_out, long res_out_ld, int w_type, const void *w, float eps, int T, int n,
                               int8_t *q, long q_ld, float *scale, void *stream);

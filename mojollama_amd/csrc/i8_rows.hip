@@ -6,7 +6,8 @@
 // these kernels where there are many rows (norm of 8192 x 4096 with residual, 16 bits: 47 us, 5.0 TB/s; silu of
 // 4096 x 11264: 52 us, 4.4 TB/s, its exponentials beside it; the card copies 4 GiB at 4.7).  A few rows take the
 // launch and one memory round trip (3 to 5 us).  The norm's factor 1 / sqrt(mean + eps) is one number per row: it
-// enters the scale alone, and the codes do not wait for it.
+// enters the scale alone, and the codes do not wait for it.  A row of a norm whose products w h, squares or values would
+// leave fp32 though y does not is formed again in 64 bits, behind the rest (far_norm).
 #include <algorithm>
 #include <type_traits>
 #include "i8.h"
@@ -142,6 +143,13 @@ __device__ __forceinline__ uint2 codes(const float (&y)[8], const row_step &s)
     return make_uint2(four(f[0], f[1], f[2], f[3]), four(f[4], f[5], f[6], f[7]));
 }
 
+// One of them, pre in y already.
+__device__ __forceinline__ int8_t code(float y, float inv)
+{
+#pragma clang fp contract(off)
+    return (int8_t)(__float_as_uint(y * inv + 12582912.0f) & 255);
+}
+
 // g / d, 1 <= d <= 2^100: the reciprocal with one Newton step, the quotient with its remainder taken back (the rounded
 // quotient but for about one in a million, there its neighbour), in six instructions for the ten of a division that
 // serves every number.
@@ -181,10 +189,10 @@ __device__ __forceinline__ void weigh(const row_args &a, int e, int left, float 
     else times<MLLM_F16>(a.w, e, left, y);
 }
 
-// y of elements e .. e + 7 of row t; sq gains the squares of h.
+// y of elements e .. e + 7 of row t; sq gains the squares of h, bits the bits of h.
 template <int KIND, int XT, int RT>
 __device__ __forceinline__ void form(const row_args &a, const raw8<XT> &xr, const raw8<RT> &rr, int e, long t, int left,
-                                     bool store, float (&y)[8], float &sq)
+                                     bool store, float (&y)[8], float &sq, uint32_t &bits)
 {
     to_f32<XT>(xr, y);
     if constexpr (KIND == SILU) {
@@ -215,10 +223,16 @@ __device__ __forceinline__ void form(const row_args &a, const raw8<XT> &xr, cons
         const raw8<RT> h = from_f32<RT>(y);
         if (store) st8<size_of(RT)>(a.res_out, t * a.res_out_ld + e, left, h);
         to_f32<RT>(h, y);
+        // of the words as they are stored: four to a vector of 16-bit elements
+#pragma unroll
+        for (int i = 0; i < 2 * size_of(RT); i++) bits |= h.w[i];
     }
     if constexpr (KIND == NORM || KIND == NORM_RES) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) sq = fmaf(y[i], y[i], sq);
+        for (int i = 0; i < 8; i++) {
+            sq = fmaf(y[i], y[i], sq);
+            if constexpr (KIND == NORM) bits |= __float_as_uint(y[i]);
+        }
         weigh(a, e, left, y);
     }
 }
@@ -230,22 +244,70 @@ __device__ __forceinline__ void load(const row_args &a, long t, int e, int left,
     if constexpr (KIND == NORM_RES || KIND == SILU) r = ld8<size_of(RT)>(a.res, t * a.res_ld + e, left);
 }
 
-// The norm's factor with squares and their sum in 64 bits, where it may itself leave fp32 (eps 0 and a row below 2^-128);
-// every wave of the row forms it alike.
-template <int KIND, int XT, int RT>
-__device__ double far_factor(const row_args &a, long t, int lane)
+// What a norm keeps in fp32 for a row: its largest |w h| (bits m) with room below and above for the smaller ones, for the
+// factor and for y, and the mean square, beside eps.
+__device__ __forceinline__ bool near_one(uint32_t m, float mean, float eps)
 {
-    double sum = 0.0;
-    for (int e = 8 * lane; e < a.n; e += 512) {
-        float h[8];
-        // the stored sum (x or res may be where it went): the barrier of the row's maximum lies between
-        if constexpr (KIND == NORM_RES) to_f32<RT>(ld8<size_of(RT)>(a.res_out, t * a.res_out_ld + e, a.n - e), h);
-        else to_f32<XT>(ld8<size_of(XT)>(a.x, t * a.x_ld + e, a.n - e), h);
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum += (double)h[i] * h[i];
+    return m >= __float_as_uint(0x1p-100f) && m < __float_as_uint(0x1p77f) && mean < 0x1p100f &&
+           (mean >= 0x1p-100f || eps >= 0x1p-100f);
+}
+
+__device__ __forceinline__ float element(const void *p, int type, long at)
+{
+    if (type == MLLM_F32) return ((const float *)p)[at];
+    return type == MLLM_BF16 ? __uint_as_float((uint32_t)((const uint16_t *)p)[at] << 16) : (float)((const _Float16 *)p)[at];
+}
+
+// f(e, h, w h) of the elements of a lane, one by one (few registers beside the row's), in 64 bits, where they are exact
+// and in range.  h is the stored sum where there is one (x or res may be where it went): this lane's own.
+template <int KIND, int XT, int RT, class F> __device__ __forceinline__ void far_each(const row_args &a, long t, int at, int L, F &&f)
+{
+    for (int b = 8 * at; b < a.n; b += 8 * L)
+#pragma unroll 1
+        for (int e = b; e < min(b + 8, a.n); e++) {
+            const double h = KIND == NORM_RES ? element(a.res_out, RT, t * a.res_out_ld + e) : element(a.x, XT, t * a.x_ld + e);
+            f(e, h, h * element(a.w, a.w_type, e));
+        }
+}
+
+// A norm's row that is neither near_one nor of zeros.  The codes are those of w h times a power of two that takes the
+// largest to between 1 and 2: of the same steps in fp32 as elsewhere, with nothing out of range.
+template <int KIND, int XT, int RT>
+__device__ void far_norm(const row_args &a, int per_wave)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = per_wave ? 1 : blockDim.x >> 6;
+    const int L = per_wave ? 64 : blockDim.x, at = per_wave ? lane : threadIdx.x;
+    const long t = per_wave ? i8_block() * (blockDim.x >> 6) + wave : i8_block();
+    double most = 0.0, sum = 0.0;
+    far_each<KIND, XT, RT>(a, t, at, L, [&](int, double h, double y) {
+        sum += h * h;
+        most = fmax(most, fabs(y) < INFINITY ? fabs(y) : INFINITY);                  // a NaN is as bad
+    });
+    for (int d = 32; d > 0; d >>= 1) {
+        sum += __shfl_xor(sum, d, 64);
+        most = fmax(most, __shfl_xor(most, d, 64));
     }
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    return 1.0 / sqrt(sum / a.n + (double)a.eps);
+    if (waves > 1) {
+        __shared__ double sums[16], mosts[16];
+        if (lane == 0) {
+            sums[wave] = sum;
+            mosts[wave] = most;
+        }
+        __syncthreads();
+        sum = most = 0.0;
+        for (int i = 0; i < waves; i++) {
+            sum += sums[i];
+            most = fmax(most, mosts[i]);
+        }
+    }
+    const double y_most = most == 0.0 ? 0.0 : most / sqrt(sum / a.n + (double)a.eps);
+    const bool bad = !((float)y_most < INFINITY), none = bad || most == 0.0;
+    if (at == 0) a.scale[t] = bad ? NAN : (float)(y_most / 127.0);
+    const double pre = none ? 0.0 : ldexp(1.0, -ilogb(most));
+    const float inv = none ? 0.0f : 1.0f / (float)(most * pre) * 127.0f;
+    far_each<KIND, XT, RT>(a, t, at, L, [&](int e, double, double y) {
+        a.q[t * a.q_ld + e] = none ? 0 : code((float)(y * pre), inv);
+    });
 }
 
 // A row over L = blockDim.x lanes (PER_WAVE: a row per wave).  NV vectors of eight elements a lane stay in
@@ -262,6 +324,7 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
     raw8<XT> x[NV];
     raw8<RT> r[NV];
     float sq = 0.0f;
+    uint32_t bits = 0;
     top mm;
     if (real) {
 #pragma unroll
@@ -274,13 +337,13 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
             const int e = 8 * (v * L + at);
 #pragma unroll
             for (int i = 0; i < 8; i++) y[v][i] = 0.0f;
-            if (e < a.n) form<KIND, XT, RT>(a, x[v], r[v], e, t, a.n - e, true, y[v], sq);
+            if (e < a.n) form<KIND, XT, RT>(a, x[v], r[v], e, t, a.n - e, true, y[v], sq, bits);
             mm.add(y[v]);
         }
         for (int e = 8 * (NV * L + at); e < a.n; e += 8 * L) {
             float z[8];
             load<KIND, XT, RT>(a, t, e, a.n - e, x[0], r[0]);
-            form<KIND, XT, RT>(a, x[0], r[0], e, t, a.n - e, true, z, sq);
+            form<KIND, XT, RT>(a, x[0], r[0], e, t, a.n - e, true, z, sq, bits);
             mm.add(z);
         }
     }
@@ -305,13 +368,20 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
         }
     }
     const row_step s = step_of(__builtin_amdgcn_readfirstlane(m));
-    // squares that leave fp32, or vanish in it where eps does not stand above them, are summed again in 64 bits
     float step = s.most / 127.0f;
+    // The row is not for fp32.  (Its type decides how the row's branch is compiled, and so the registers of all that is
+    // before: a norm with residual of 8192 x 4096 takes 52 us with int, 47 with bool; of 2048 x 16384 56 with bool, 53
+    // with int; one without of 4096 x 8192 32.8 with bool, 30 with int.)
+    std::conditional_t<KIND == NORM || NV == 8, int, bool> away = false;
     if constexpr (KIND == NORM || KIND == NORM_RES) {
         const float mean = sq / (float)a.n;
-        if (real && !s.bad && m != 0 && (!(mean < 0x1p100f) || (mean < 0x1p-100f && a.eps < 0x1p-100f)))
-            step = (float)(s.most * far_factor<KIND, XT, RT>(a, t, lane) / 127.0);
-        else step = s.most * (1.0f / sqrtf(mean + a.eps)) / 127.0f;
+        away = !near_one(m, mean, a.eps);
+        if (m == 0) {                                    // padding, unless it is 0 in fp32 only
+            away = __any((bits & (KIND == NORM || RT == MLLM_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu)) != 0);
+            if (!per_wave && waves > 1) away = __syncthreads_or(away);
+        }
+        away = __builtin_amdgcn_readfirstlane(away);     // one branch for the row
+        step = s.most * (1.0f / sqrtf(mean + a.eps)) / 127.0f;
     }
     if (at == 0 && real) a.scale[t] = s.bad ? NAN : m == 0 ? 0.0f : step;
     const int n = PACK ? a.n_pad : a.n;
@@ -345,11 +415,14 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
                 weigh(a, e, a.n - e, z);
             } else {
                 load<KIND, XT, RT>(a, t, e, a.n - e, x[0], r[0]);
-                form<KIND, XT, RT>(a, x[0], r[0], e, t, a.n - e, false, z, no);
+                form<KIND, XT, RT>(a, x[0], r[0], e, t, a.n - e, false, z, no, bits);
             }
         }
         put(e, z);
     }
+    // behind all else, where the row's registers are free: its lanes write over their codes
+    if constexpr (KIND == NORM || KIND == NORM_RES)
+        if (away) far_norm<KIND, XT, RT>(a, per_wave);
 }
 
 template <int KIND, int XT, int RT, bool PACK> void go_rows(const row_args &a, hipStream_t st)
