@@ -204,12 +204,14 @@ __device__ __forceinline__ void form(const row_args &a, const raw8<XT> &xr, cons
             least = fminf(least, g[i]);
             y[i] = quotient(g[i], 1.0f + expf(-g[i]));
         }
-        // far below zero, where e^-g goes out of the quotient's reach, 1 + e^-g is e^-g
+        // far below zero, where e^-g goes out of the quotient's reach, 1 + e^-g is e^-g: g h u h with h = e^(g / 2), in this
+        // order, so that nothing leaves fp32 that the result does not
         if (__any(least < -69.0f)) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float h = expf(0.5f * g[i]);
-                y[i] = g[i] < -69.0f ? g[i] * h * h : y[i];
+                y[i] = g[i] < -69.0f ? g[i] * h * u[i] : y[i];
+                u[i] = g[i] < -69.0f ? h : u[i];
             }
         }
 #pragma unroll

@@ -1,4 +1,5 @@
-"""The ends of fp32 in the rows of layers in 8-bit integers (mllm_i8_rms_norm), against the formulas in 64 bits."""
+"""The ends of fp32 in the rows of layers in 8-bit integers (mllm_i8_rms_norm, _silu_mul), against the formulas in 64
+bits."""
 import math
 
 import pytest
@@ -106,3 +107,24 @@ def test_norm_values_beyond_fp32(dev, n):
     q, scale = dev.i8_rms_norm(x.cuda(), torch.zeros(n, device="cuda"), 0.0)
     finite = torch.tensor([0, 1, 4, 5, 6, 7], device="cuda")
     assert not q.any() and not scale[finite].any() and scale[2:4].isnan().all()
+
+
+@pytest.mark.parametrize("n", [1, 9, 700, 40000])
+@pytest.mark.parametrize("least,most,up", [(-80.0, -69.5, 1.0), (-103.0, -88.0, 1e30), (-120.0, -104.0, 1e38), (-150.0, -60.0, 1e35)])
+def test_silu_of_far_gates(dev, n, least, most, up):
+    """Gates whose silu is below fp32's normal numbers, or below all of them, and an up that takes the product back into
+    range.  Roundings of y there: e^(g / 2), within one step, twice (four halves), and three products."""
+    g = torch.Generator().manual_seed(n)
+    gate = least + (most - least) * torch.rand((4, n), generator=g)
+    gate[:, 0] = most
+    u = (0.5 + torch.rand((4, n), generator=g)) * up
+    u[:, 0] = 1.5 * up
+    q, scale = dev.i8_silu_mul(gate.cuda(), u.cuda())
+    a = gate.double()
+    e = torch.exp(a)
+    y = a * e / (1 + e) * u.double()
+    top = y.abs().amax(1)
+    assert (top > 2.0 ** -100).all()
+    off = (q.cpu().double() - 127 * y / top[:, None]).abs().max().item()
+    assert off <= 0.5 + 127 * U * (2 * 7 + 3) * 1.01, off
+    assert ((scale.cpu().double() - top / 127).abs() <= U * (7 + 1) * 1.01 * top / 127).all()
