@@ -776,6 +776,8 @@ class DeviceOps:
         s = t.shape
         if len(s) != 2:
             raise ValueError(f"{what}: [tokens, elements], got {list(s)}")
+        if max(s) > 1 << 30:                     # the entries take 32-bit sizes
+            raise ValueError(f"{what}: at most 2^30 in each dimension, got {list(s)}")
         return s
 
     def _i8_new(self, q, scale, T, n):
@@ -873,7 +875,7 @@ class DeviceOps:
 
     def i8_gemm_workspace(self, weights, T):
         """A workspace for i8_gemm calls of up to T tokens."""
-        n = self.so.mllm_i8_gemm_workspace_size(T, weights.n_rows, weights.n_cols)
+        n = self.so.mllm_i8_gemm_workspace_size(T, weights.n_rows, weights.n_cols) if 0 <= T <= 1 << 30 else -1
         if n < 0:
             raise ValueError("i8_gemm_workspace: sizes that are not served")
         return self.torch.empty(max(n, 256), dtype=self.torch.uint8, device="cuda")
