@@ -496,6 +496,13 @@ class DeviceOps:
     def _elsewhere(self, t, what):
         raise ValueError(f"{what}: a tensor on {t.device}, not on the current GPU")
 
+    def _room(self, ws, cur):
+        """A workspace's address and bytes are what its entry writes to: on the current GPU (cur), with nothing between."""
+        if ws.get_device() != cur:
+            self._elsewhere(ws, "workspace")
+        if not ws.is_contiguous():
+            raise ValueError("workspace: a dense tensor is needed")
+
     @staticmethod
     def _made_here(cur, *handles):
         for h in handles:
@@ -616,8 +623,8 @@ class DeviceOps:
             sk = sinks.data_ptr()
         if ws is None:
             ws = self.paged_attn_workspace(kv, T, B, NH, max_len, window)
-        elif ws.get_device() != cur:
-            self._elsewhere(ws, "workspace")
+        else:
+            self._room(ws, cur)
         return qt, qp, ql, out, ot, op, ol, ws, sk
 
     def paged_attn_decode(self, kv, q, lens, max_len, NH, scale=None, window=0, sinks=None, seqs=None, out=None,
@@ -682,8 +689,8 @@ class DeviceOps:
             status = torch.empty(1, dtype=torch.int32, device="cuda")
         if ws is None:
             ws = self.pages_workspace(m, n)
-        elif ws.get_device() != cur:
-            self._elsewhere(ws, "workspace")
+        else:
+            self._room(ws, cur)
         return status, self._ints(status, "status", cur, 1), ws
 
     def _pages_in(self, planes, n_pages, cur):
@@ -896,8 +903,8 @@ class DeviceOps:
         op, ol = self._at(out, "out", cur, T, R)
         if ws is None:
             ws = self.i8_gemm_workspace(weights, T)
-        elif ws.get_device() != cur:
-            self._elsewhere(ws, "workspace")
+        else:
+            self._room(ws, cur)
         rc = self.so.mllm_i8_gemm(weights._packed, weights._scale, qp, ql, self._floats(scale, "scale", cur, T), T, R,
                                   weights.n_cols, self._floats(bias, "bias", cur, R), ot, op, ol, ws.data_ptr(), ws.nbytes,
                                   self._stream_of(cur))

@@ -41,3 +41,34 @@ def test_workspace(dev, T):
 
 def test_largest(dev):
     assert tuple(dev._sizes(rows(1 << 30, 1), "x")) == (1 << 30, 1) and tuple(dev._sizes(rows(1, 1 << 30), "x")) == (1, 1 << 30)
+
+
+def test_workspaces_lie_densely(dev):
+    """A workspace's address and bytes go to the entries: what is not dense would be written beyond itself.  (The
+    entries stand in for themselves here: nothing is launched.)"""
+    class Entries:
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    class Here(torch.Tensor):
+        """On GPU 0, as far as the checks ask."""
+        get_device = lambda self: 0  # noqa: E731
+
+    ops = K.DeviceOps(Entries())
+    ops._cur_raw = ops._cur = lambda: 0
+    ops._stream_of = ops._raw_stream = lambda cur: None
+    t = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype).as_subclass(Here)  # noqa: E731
+    dense = t(64, 16, dtype=torch.uint8)
+    apart = [dense[:, :8], dense[::2], torch.zeros(1, dtype=torch.uint8).as_subclass(Here).expand(1 << 40)]
+    w = SimpleNamespace(n_rows=8, n_cols=16, _device=0, _packed=0, _scale=0)
+    kv = SimpleNamespace(_device=0, head_dim=16)
+    m = SimpleNamespace(_device=0)
+    ints = t(3, dtype=torch.int32)
+    calls = [lambda ws: ops.i8_gemm(w, t(2, 16, dtype=torch.int8), t(2), out=t(2, 8), ws=ws),
+             lambda ws: ops._attn(kv, t(2, 32), 2, 2, 2, 16, 0, None, t(2, 32), None, ws, 0),
+             lambda ws: ops._pages_args(m, 3, ints[:1], ws, 0)]
+    for call in calls:
+        call(dense)
+        for ws in apart:
+            with pytest.raises(ValueError, match="workspace"):
+                call(ws)
