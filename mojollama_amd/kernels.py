@@ -339,7 +339,7 @@ class DeviceOps:
         self.so = so or load_kernels()
         # the current device as the runtime has it (no call here makes it the first to ask: tensors are there by then)
         self._cur_raw = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        self._stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", lambda cur: torch.cuda.current_stream(cur).cuda_stream)
         self._int8, self._f32 = torch.int8, torch.float32
         self._reals = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
         self._types = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float8_e4m3fn: T_E4M3}
@@ -480,7 +480,7 @@ class DeviceOps:
         return self.torch.cuda.current_device()
 
     def _raw_stream(self, cur):
-        return self.torch._C._cuda_getCurrentRawStream(cur)
+        return self._stream_of(cur)
 
     def _type(self, t, what, cur):
         """mllm type of a tensor on the current GPU (cur) whose last dimension is dense."""

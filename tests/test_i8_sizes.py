@@ -72,3 +72,11 @@ def test_workspaces_lie_densely(dev):
         for ws in apart:
             with pytest.raises(ValueError, match="workspace"):
                 call(ws)
+
+
+def test_streams_without_the_raw_call(monkeypatch):
+    """A torch whose runtime does not hand out raw streams: the current stream's handle, from every call."""
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=1000 + device))
+    ops = K.DeviceOps(SimpleNamespace())
+    assert ops._stream_of(3) == 1003 and ops._raw_stream(2) == 1002
