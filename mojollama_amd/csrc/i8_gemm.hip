@@ -557,7 +557,8 @@ template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_stream(g
 __global__ __launch_bounds__(64) void k_i8_far(gemm_args a)
 {
     const int lane = threadIdx.x, l = lane & 31, h = lane >> 5;
-    const unsigned tile = blockIdx.x;
+    const long tile = i8_block();
+    if (tile >= (long)a.nt * a.nr) return;
     const int r0 = (int)(tile / a.nt) * 32, t0 = (int)(tile % a.nt) * 32;
     const int8_t *w = a.w + (long)(r0 >> 5) * a.kb * 2048 + lane * 16;
     const int8_t *x = a.x + (long)min(t0 + l, a.T - 1) * a.x_ld;
@@ -709,8 +710,9 @@ MLLM_API int mllm_i8_gemm(const void *packed, const float *w_scale, const int8_t
     if (far) {
         a.nt = (T + 31) / 32;
         a.nr = (n_rows + 31) / 32;
-        if ((long)a.nt * a.nr > kMostBlocks) return pk_fail(who, "T * n_rows is too large for one call");
-        hipLaunchKernelGGL(k_i8_far, dim3(a.nt * a.nr), dim3(64), 0, st, a);
+        const long blocks = (long)a.nt * a.nr;
+        if (blocks > kI8Blocks * 65535) return pk_fail(who, "T * n_rows is too large for one call");
+        hipLaunchKernelGGL(k_i8_far, i8_grid(blocks), dim3(64), 0, st, a);
     } else if (p.kind) {
         p.kind->go(a, p.nt * p.nr * p.splits, st);
     } else if (p.few > 1) {
