@@ -478,8 +478,10 @@ template <int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
 }
 
 // 32 weight rows x 32 TF tokens a workgroup of W waves, which take blocks of 128 columns in turn and join their sums in
-// LDS.  A wave's block of x comes to its own part of LDS in whole lines and its weights to registers, two blocks under
-// way; waves meet at the end alone.  (32 tokens x 4096 x 4096 with weights in the last cache: 6.4 us, 8.0 with x from the
+// LDS.  A wave's block of x comes to its own part of LDS in whole lines and its weights to registers, asked for two blocks
+// ahead; waves meet at the end alone.  The loads stand behind a condition, so that the compiler takes a block's weights for
+// the youngest loads and waits for all: in every other block the next one's loads are waited for too, and a pair of blocks
+// takes a round trip to memory.  (32 tokens x 4096 x 4096 with weights in the last cache: 6.4 us, 8.0 with x from the
 // caches; 16 x 8192 x 8192 from memory: 14.5 us, 4.6 TB/s, 19.4 with 16 rows a workgroup.  96 and 128 tokens would be
 // bound by LDS: 12.6 and 14 us, tiles 11.  64 rows a workgroup: 48 tokens x 14336 x 4096 18.0 us for 21.6, but tiles take
 // 17.6, and 10 to 60 % slower where rows are fewer.)
@@ -513,8 +515,8 @@ template <int TF, int W> __global__ __launch_bounds__(64 * W) void k_i8_stream(g
     i32x4 w0[4], w1[4];
     if (wave < nb) load(x0, w0, wave);
     if (wave + W < nb) load(x1, w1, wave + W);
-    // block b: its loads have landed (those of block b + W, if there is one, may be under way); when its operands are
-    // read, its buffer takes block b + 2 W
+    // block b: its x has landed (the loads of block b + W, if there is one, may be under way as far as x goes; the weights
+    // have the compiler's waits); when its operands are read, its buffer takes block b + 2 W
     auto block = [&](uint8_t *x, i32x4 (&wf)[4], int b) __attribute__((always_inline)) {
         if (b + W < nb) wait_mem<LOADS>();
         else wait_mem<0>();
