@@ -7,11 +7,13 @@
 // Every kernel multiplies weights (MFMA rows) by tokens (MFMA columns): a lane then holds four neighbouring
 // output channels of one token.
 //
-// Measured (MI355X, bf16 out, codes of normal values): 8192 tokens x 8192 x 8192 in 416 us, 2640 TOPS, where a
-// loop of these matrix instructions on registers alone reaches 3400 (4500 with codes of zero, as this product
+// Measured (MI355X, bf16 out, codes of normal values): 8192 tokens x 8192 x 8192 in 418 to 423 us, 2600 to 2630 TOPS,
+// where a loop of these matrix instructions on registers alone reaches 3400 (4500 with codes of zero, as this product
 // comes to 3900 with them: what bounds it is power); with weights from memory (in the last cache) 1024 tokens x
-// 4096 x 4096 in 22.5 us (21.2), 256 in 13.1 (10.5), 64 in 10.5 (8.4), 16 in 6.6 (5.7), one in 6.2 (5.4), of which the
-// launch is 2.2.
+// 4096 x 4096 in 22.7 us (22.8), 256 in 13.7 (11.0), 64 in 11.1 (8.7), 32 in 8.7 (6.5), 16 in 6.9 (5.9), one in 6.4 (4.6),
+// of which the launch is 2.2.  From 20 tokens to 1000 against 4096 x 4096 (3000 against 2880 x 2880) it takes 1.7 to 5
+// times what its bytes or products need: K is split only where a second launch to join the sums (4.4 us and their traffic)
+// pays, so tiles are small, or fewer than CUs.  Tiles walk K to its next 512: 8192 x 8192 x 64 takes 65 us, x 256 67.5.
 #include <algorithm>
 #include <type_traits>
 #include "i8.h"
@@ -210,7 +212,7 @@ __device__ __forceinline__ work_tile tile_at(const gemm_args &a, int b, int n)
 // to four steps ahead; x for two steps at once, so that a row is read in whole lines of 128 bytes (64 bytes at a time
 // cost twice the L2 traffic), into one of two.  Where tiles are fewer than CUs a step is as long as its latency: KG = 2
 // groups of waves, with buffers of their own, take half of K each, and the second hands its sums to the first by way of
-// LDS (256 x 4096 x 4096 with weights from memory: 15.9 -> 13.9 us, 512: 17.6 -> 16.8; for tiles of 128 x 128 and more,
+// LDS (256 x 4096 x 4096 with weights from memory: 15.9 -> 13.7 us, 512: 17.6 -> 16.5; for tiles of 128 x 128 and more,
 // whose steps are bound by their products, no gain).
 template <int MF, int NF, int WM, int WN> struct tile_of {
     static constexpr int waves = WM * WN, TT = 32 * MF * WM, TR = 32 * NF * WN;
@@ -481,7 +483,7 @@ template <int W> __global__ __launch_bounds__(64 * W) void k_i8_few(gemm_args a)
 // LDS.  A wave's block of x comes to its own part of LDS in whole lines and its weights to registers, asked for two blocks
 // ahead; waves meet at the end alone.  The loads stand behind a condition, so that the compiler takes a block's weights for
 // the youngest loads and waits for all: in every other block the next one's loads are waited for too, and a pair of blocks
-// takes a round trip to memory.  (32 tokens x 4096 x 4096 with weights in the last cache: 6.4 us, 8.0 with x from the
+// takes a round trip to memory.  (32 tokens x 4096 x 4096 with weights in the last cache: 6.5 us, 8.0 with x from the
 // caches; 16 x 8192 x 8192 from memory: 14.5 us, 4.6 TB/s, 19.4 with 16 rows a workgroup.  96 and 128 tokens would be
 // bound by LDS: 12.6 and 14 us, tiles 11.  64 rows a workgroup: 48 tokens x 14336 x 4096 18.0 us for 21.6, but tiles take
 // 17.6, and 10 to 60 % slower where rows are fewer.)
@@ -584,7 +586,7 @@ __global__ __launch_bounds__(64) void k_i8_far(gemm_args a)
 // ------------------------------------------------------------------------------------ the choice
 struct tile_kind {
     int TT, TR, groups, per_cu;    // groups of waves, workgroups of it that a CU holds
-    float step, each, tail;        // microseconds of a step of K, of each workgroup in it, of a workgroup beside
+    float step, each, tail;        // for a step of K, each workgroup in it, a workgroup beside (see plan_of)
     void (*go)(const gemm_args &, int grid, hipStream_t);
     // A tile is not mostly empty.  Up to 32 tokens the time is that of the weights' stream, which two groups do not
     // shorten: 16 tokens of 11264 x 2048 take them 9.3 us, k_i8_stream 7.4.
@@ -621,8 +623,9 @@ struct plan {
 
 // The kernel that an estimate of their times in microseconds, from sizes alone, puts first; its constants are fitted to
 // the kernels' times with weights from memory, at 1 to 4096 tokens and seventeen matrices from 512 x 2048 to
-// 32000 x 2048 and 1024 x 14336, every tile with K split up to twelve times (3540 times).  There its choice is 0.6 %
-// slower than the best on average, 18 % at most.
+// 32000 x 2048 and 1024 x 14336, every tile with K split up to twelve times (3540 times).  On these same times its choice
+// is 0.6 % slower than the best on average, 18 % at most; sizes outside them were not measured with every kernel.  The
+// constants were fitted together: a kind's step, each and tail make up its time as a sum and measure nothing alone.
 plan plan_of(int T, int R, int kb, int cols)
 {
     plan best{};

@@ -3,11 +3,13 @@
 //
 // y[i] of a row, its largest |y| and (norm) the sum of squares are formed in one pass over memory and stay
 // in registers; the codes are rounded from there: memory is read and written once, which is what bounds
-// these kernels where there are many rows (norm of 8192 x 4096 with residual, 16 bits: 47 us, 5.0 TB/s; silu of
-// 4096 x 11264: 52 us, 4.4 TB/s, its exponentials beside it; the card copies 4 GiB at 4.7).  A few rows take the
-// launch and one memory round trip (3 to 5 us).  The norm's factor 1 / sqrt(mean + eps) is one number per row: it
-// enters the scale alone, and the codes do not wait for it.  A row of a norm whose products w h, squares or values would
-// leave fp32 though y does not is formed again in 64 bits, behind the rest (far_norm).
+// these kernels where there are many rows (norm of 8192 x 4096 with residual, 16 bits: 45 to 47 us in a loop of launches,
+// 5.0 to 5.2 TB/s, 50 in a profiler's trace; silu of 4096 x 11264: 50 to 55 us, 4.2 to 4.7 TB/s, 57 in the trace, its
+// exponentials beside it; the card copies 4 GiB at 4.7).  Rows wider than 16384 elements take one workgroup a CU, whose
+// barrier nothing hides (silu of 4096 x 18944: 111 us, 3.5 TB/s).  A few rows take the launch and one memory round trip (3
+// to 5 us).  The norm's factor 1 / sqrt(mean + eps) is one number per row: it enters the scale alone, and the codes do not
+// wait for it.  A row of a norm whose products w h, squares or values would leave fp32 though y does not is formed again in
+// 64 bits, behind the rest (far_norm).
 #include <algorithm>
 #include <type_traits>
 #include "i8.h"
@@ -466,7 +468,7 @@ __global__ __launch_bounds__(256) void k_i8_pack(const int8_t *w, long w_ld, int
 }
 
 // Back to values: 2^lpr_log lanes a row, eight codes of each of four vectors a lane (four loads under way; 8192 x 4096
-// to 16 bits: 22.4 us, 4.5 TB/s).
+// to 16 bits: 21 to 22 us, 4.5 to 4.7 TB/s).
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_i8_dequant(const int8_t *q, long q_ld, const float *scale, int T, int n, void *out,
                                                     long out_ld, int lpr_log)

@@ -783,13 +783,14 @@ class DeviceOps:
         s = t.shape
         if len(s) != 2:
             raise ValueError(f"{what}: [tokens, elements], got {list(s)}")
-        if max(s) > 1 << 30:                     # the entries take 32-bit sizes
+        T, n = s
+        if T > 1073741824 or n > 1073741824:     # the entries take 32-bit sizes
             raise ValueError(f"{what}: at most 2^30 in each dimension, got {list(s)}")
-        return s
+        return T, n
 
     def _i8_new(self, q, scale, T, n):
         """The outputs of the calls that quantise, where they are not given: rows of codes at multiples of 16 bytes, as
-        i8_gemm takes them; long ones at whole lines (1000 tokens x 2048 x 2048: 9.0 us, 9.9 with rows 16 bytes off)."""
+        i8_gemm takes them; long ones at whole lines (1000 tokens x 2048 x 2048: 9.5 us, 9.9 with rows 16 bytes off)."""
         if q is None:
             step = 128 if n >= 1024 else 16
             q = self.torch.empty((T, (n + step - 1) // step * step), dtype=self._int8, device="cuda")[:, :n]
@@ -903,7 +904,7 @@ class DeviceOps:
         op, ol = self._at(out, "out", cur, T, R)
         if ws is None:
             ws = self.i8_gemm_workspace(weights, T)
-        else:
+        elif ws.get_device() != cur or not ws.is_contiguous():
             self._room(ws, cur)
         rc = self.so.mllm_i8_gemm(weights._packed, weights._scale, qp, ql, self._floats(scale, "scale", cur, T), T, R,
                                   weights.n_cols, self._floats(bias, "bias", cur, R), ot, op, ol, ws.data_ptr(), ws.nbytes,
