@@ -374,7 +374,7 @@ __global__ __launch_bounds__(NV > 4 ? 256 : 1024) void k_i8_rows(row_args a, int
     const row_step s = step_of(__builtin_amdgcn_readfirstlane(m));
     float step = s.most / 127.0f;
     // The row is not for fp32.  (Its type decides how the row's branch is compiled, and so the registers of all that is
-    // before: a norm with residual of 8192 x 4096 takes 52 us with int, 47 with bool; of 2048 x 16384 56 with bool, 53
+    // before: a norm with residual of 8192 x 4096 takes 52 us with int, 47 with bool; of 2048 x 16384 56 with bool, 55
     // with int; one without of 4096 x 8192 32.8 with bool, 30 with int.)
     std::conditional_t<KIND == NORM || NV == 8, int, bool> away = false;
     if constexpr (KIND == NORM || KIND == NORM_RES) {
